@@ -15,6 +15,8 @@ LIB_PATH = os.environ.get("SPCONVB_LIB") or os.path.join(_PKG, "lib", "libspconv
 
 OK = 0
 F16, I8 = 0, 1
+F32 = 2  # the 4-bit calls only
+MXFP4, NVFP4 = 0, 1
 ACT_NONE, ACT_RELU = 0, 1
 ST_HASH_FULL, ST_DUPLICATE, ST_OVERFLOW, ST_TIMEOUT, ST_COORD_RANGE = 1, 2, 4, 8, 16
 FLAG_PREZEROED = 1
@@ -31,6 +33,16 @@ class ConvParams(C.Structure):
         ("mid_kind", C.c_int32), ("mid_inv_scale", C.c_float), ("mid_scale", C.c_float),
         ("res_relu", C.c_int32), ("force_simt", C.c_int32), ("wait_test", C.c_int32),
         ("n_in_ptr", C.c_void_p), ("cap_in", C.c_uint32),
+    ]
+
+
+class Fp4Params(C.Structure):
+    """spconvb_fp4_params (include/spconvb_fp4.h)."""
+    _fields_ = [
+        ("format", C.c_int32), ("cin", C.c_int32), ("cout", C.c_int32), ("kvol", C.c_int32),
+        ("alpha", C.c_float), ("act", C.c_int32), ("out_fp4", C.c_int32), ("out_format", C.c_int32),
+        ("out_tensor_scale", C.c_float), ("out_scales", C.c_void_p), ("res", C.c_void_p),
+        ("res_relu", C.c_int32), ("wait_test", C.c_int32),
     ]
 
 
@@ -119,6 +131,22 @@ SYMBOLS.update({
     "spconvb_cp_task_detections": (C.c_int, [C.POINTER(CpParams), C.c_int32, _VP, C.c_int32,
                                              C.POINTER(_VP), C.POINTER(_VP)]),
     "spconvb_cp_rotated_iou": (C.c_int, [_VP, _VP, C.c_int32, _VP, _VP]),
+})
+
+SYMBOLS.update({
+    "spconvb_fp4_code_pitch": (C.c_uint32, [C.c_int32]),
+    "spconvb_fp4_scale_pitch": (C.c_uint32, [C.c_int32, C.c_int32]),
+    "spconvb_fp4_quantize": (C.c_int, [C.c_int32, _VP, C.c_int32, C.c_float, C.c_int32, C.c_float,
+                                       _VP, C.c_uint32, _VP, _VP, _VP]),
+    "spconvb_fp4_dequantize": (C.c_int, [C.c_int32, _VP, _VP, C.c_int32, C.c_float, C.c_int32, _VP,
+                                         C.c_uint32, _VP, _VP]),
+    "spconvb_fp4_packed_bytes": (C.c_size_t, [C.c_int32] * 4),
+    "spconvb_fp4_pack_weights": (C.c_int, [C.c_int32] * 4 + [_VP] * 4),
+    "spconvb_fp4_linear": (C.c_int, [C.POINTER(Fp4Params), _VP, _VP, _VP, C.c_uint32, _VP, _VP,
+                                     _VP, _VP, _VP]),
+    "spconvb_fp4_conv_supported": (C.c_int, [C.c_int32] * 3),
+    "spconvb_fp4_conv": (C.c_int, [C.POINTER(Fp4Params), _VP, _VP, _VP, C.c_uint32, _VP,
+                                   C.c_uint32, _VP, _VP, _VP, _VP, _VP]),
 })
 
 _LIB = None

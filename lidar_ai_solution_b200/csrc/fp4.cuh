@@ -1,0 +1,120 @@
+// Microscaled 4-bit floating point: sizes of the layout, and the arithmetic that every kernel applies when it
+// makes or reads codes and block scales.
+#pragma once
+#include "common.cuh"
+#include "spconvb_fp4.h"
+
+namespace spconvb {
+namespace fp4 {
+
+__host__ __device__ inline uint32_t cpad(uint32_t channels) { return (channels + 63u) & ~63u; }
+__host__ __device__ inline uint32_t code_pitch(uint32_t channels) { return cpad(channels) / 2; }
+__host__ __device__ inline uint32_t scale_pitch(int format, uint32_t channels) {
+  return format == SPCONVB_MXFP4 ? 4u * ((cpad(channels) + 127u) / 128u) : cpad(channels) / 16u;
+}
+inline bool format_ok(int f) { return f == SPCONVB_MXFP4 || f == SPCONVB_NVFP4; }
+inline bool channels_ok(int c) { return c >= 1 && c <= SPCONVB_FP4_MAX_CHANNELS; }
+// A tensor scale is a positive, finite, normal number; the format without one takes 1.
+inline bool tensor_scale_ok(int format, float g) {
+  return format == SPCONVB_MXFP4 ? g == 1.f : g >= 1.17549435e-38f && g <= 3.4e38f / 448.f;
+}
+
+// K is walked in chunks of 256 channels (128 bytes of codes a row), four MMAs of 64 channels each.  An MMA reads the
+// scales of its 64 channels as bytes of one 32-bit word a row: four of 16 channels (NVFP4), or two of 32
+// (MXFP4), in the lower or the upper half of a word that covers 128 channels.  Rows of 64 channels have their word for themselves.
+constexpr uint32_t kChunkK = 256;
+constexpr uint32_t kAtomBytes = 512;  // the scale words of 128 rows: word of row r at (r % 32) * 16 + (r / 32) * 4
+__host__ __device__ inline uint32_t steps_per_word(int format, uint32_t cp) {
+  return format == SPCONVB_MXFP4 && cp != 64u ? 2u : 1u;
+}
+__host__ __device__ inline uint32_t words_per_chunk(int format, uint32_t cp) {
+  return 4u / steps_per_word(format, cp);
+}
+
+// The block scale of a block whose largest magnitude is `amax` (the bits of a float >= 0, infinity or NaN): its byte,
+// and S in fp32.  x / S of MXFP4 is a multiplication by a power of two.
+__device__ __forceinline__ uint32_t scale_mx(uint32_t amax_bits, float& s) {
+  const uint32_t e = amax_bits >> 23;  // 0 for zero and subnormals, whose scale is the smallest one anyway
+  const uint32_t byte = e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+  s = byte == 0u ? 5.8774717541114375e-39f : __uint_as_float(byte << 23);  // 2^-127 is a subnormal number
+  return byte;
+}
+__device__ __forceinline__ uint32_t scale_nv(uint32_t amax_bits, float tensor_scale, float& s) {
+  if (amax_bits >= 0x7f800000u) {
+    s = 0.f;
+    return 0x7fu;
+  }
+  const float t = __fdiv_rn(__uint_as_float(amax_bits), __fmul_rn(6.f, tensor_scale));
+  uint16_t two;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(t));
+  uint32_t half2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(half2) : "h"(two));
+  s = __fmul_rn(__half2float(__ushort_as_half((uint16_t)half2)), tensor_scale);
+  return two & 0xffu;
+}
+// S of a stored byte.
+__device__ __forceinline__ float scale_value(int format, uint32_t byte, float tensor_scale) {
+  if (format == SPCONVB_MXFP4)
+    return byte == 255u ? __uint_as_float(0x7fffffffu)
+                        : (byte == 0u ? 5.8774717541114375e-39f : __uint_as_float(byte << 23));
+  uint32_t half2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(half2) : "h"((uint16_t)byte));
+  return __fmul_rn(__half2float(__ushort_as_half((uint16_t)half2)), tensor_scale);
+}
+
+// Eight values, already divided by S, to eight codes: round to nearest even, saturate at 6.
+__device__ __forceinline__ uint32_t codes8(const float (&q)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+  return r;
+}
+// Eight codes to fp16 pairs (exact).
+__device__ __forceinline__ void values8(uint32_t codes, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(codes));
+}
+
+// x / S of a block.  MXFP4: times 2^-e, exact.  NVFP4: the correctly rounded quotient, so that a value on the border
+// between two codes is found there: reciprocal, product, and one correction with the exact remainder (Markstein 1990), where
+// nothing in it can overflow or lose bits; else the division itself.
+struct Divider {
+  float s, r;
+  bool exact_scale, plain;
+};
+__device__ __forceinline__ Divider divider(int format, float s, uint32_t amax_bits) {
+  Divider d;
+  d.s = s;
+  d.exact_scale = format == SPCONVB_MXFP4;
+  if (d.exact_scale) {
+    // 2^-e; e = -127 .. 125, so its exponent field lies in 2 .. 254
+    d.r = s < 1.1754944e-38f ? 1.7014118346046923e38f : __uint_as_float((254u << 23) - __float_as_uint(s));
+    d.plain = true;
+  } else {
+    d.r = __frcp_rn(s);
+    d.plain = s > 1e-27f && s < 1e27f && __uint_as_float(amax_bits) < 1e30f &&
+              __uint_as_float(amax_bits) * d.r < 1e30f;
+  }
+  return d;
+}
+__device__ __forceinline__ float divide(const Divider& d, float x) {
+  if (d.exact_scale) return __fmul_rn(x, d.r);
+  if (!d.plain) return __fdiv_rn(x, d.s);
+  const float q = __fmul_rn(x, d.r);
+  return __fmaf_rn(__fmaf_rn(-q, d.s, x), d.r, q);
+}
+
+}  // namespace fp4
+}  // namespace spconvb

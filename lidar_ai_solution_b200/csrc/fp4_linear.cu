@@ -1,0 +1,581 @@
+// 4-bit rows times 4-bit weights:  out[r, c] = act(alpha * sum_k x[r, k] W[c, k] + bias[c]).
+//
+// A tile is 128 rows (M, accumulator lanes) by TN output channels (N, accumulator columns).  K goes by chunks of
+// 256 channels: 128 bytes of codes a row, which is one swizzle atom, and four MMAs of 64 channels.  Roles of the
+// warps of a CTA (one an SM, walking over tiles):
+//
+//   0-7    epilogue: a lane owns a row; a warp its quadrant of 32 rows and half of the tile's channels
+//   8      allocates tensor memory; copies the chunk's scales there and issues its MMAs
+//   9      one lane: TMA of the rows' codes, bulk copies of the weights' image (codes and scales lie ready in it)
+//   10-13  the rows' scales, a row a lane: four chunks ahead in registers, then as words into the order that the
+//          copy to tensor memory wants.  (They are kept row by row in memory, so that a convolution can gather them.)
+//
+// Scales in tensor memory have a place for every stage of the ring: a stage is filled again only when the MMAs that
+// read its scales are complete, so no copy overwrites scales that are in use.
+//
+// Few rows: the K axis is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
+// always in the same order.
+#include "fp4_umma.cuh"
+#include "pdl.cuh"
+
+namespace spconvb {
+namespace fp4 {
+namespace {
+
+constexpr int kEpiWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kScaleWarp0 = 10;
+constexpr int kCtaThreads = 32 * 14;
+constexpr uint32_t kTileM = 128;
+constexpr uint32_t kTmemCols = 512;
+
+struct LinearArgs {
+  const uint8_t* scales;
+  uint32_t spitch, nchunk, last_steps;
+  const uint32_t* n_ptr;
+  uint32_t cap;
+  const uint8_t* wpk;
+  uint32_t record;  // bytes of a block of 128 channels of a chunk in the weights' image
+  const float* bias;
+  uint8_t* out;
+  uint8_t* out_scales;
+  uint32_t* status;
+  uint32_t cout, out_cpitch, out_spitch;
+  float alpha, out_ts;
+  int act, out_mode;  // 0: fp16, 1: MXFP4, 2: NVFP4
+  int store;          // bytes of fp16 output that may be stored at once: 32, 16 or 2
+  uint32_t split;     // CTAs of a cluster that share a tile's K
+  int wait_test;
+};
+
+template <int FMT, int TN>
+struct Shape {
+  static constexpr uint32_t kWords = FMT == SPCONVB_MXFP4 ? 2 : 4;  // scale words a row and chunk
+  static constexpr uint32_t kBlocks = TN > 128 ? TN / 128 : 1;      // blocks of 128 channels of the image
+  static constexpr uint32_t kSf = kWords * kAtomBytes;
+  static constexpr uint32_t kA = kTileM * 128, kB = TN * 128;
+  static constexpr uint32_t kOffB = kA, kOffSfb = kA + kB, kOffSfa = kOffSfb + kBlocks * kSf;
+  static constexpr uint32_t kStage = kOffSfa + kSf;  // a multiple of 1024
+  static constexpr uint32_t kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);
+  static constexpr uint32_t kBuffers = TN == 256 ? 1 : 2;  // accumulators
+  static constexpr uint32_t kSfCols = kWords * 4 * (1 + kBlocks);
+  static constexpr uint32_t kSmem = kStages * kStage + 1024 + 512;
+  static_assert(kStage % 1024 == 0, "stages start on swizzle atoms");
+  static_assert(kBuffers * TN + kStages * kSfCols <= kTmemCols, "tensor memory");
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+__device__ __forceinline__ void st32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "l"(p)
+               : "memory");
+}
+
+// 32 channels of one row from fp32 sums to memory.  `col` is a multiple of 32; the row exists.
+__device__ __forceinline__ void emit32(const LinearArgs& a, float (&y)[32], uint64_t row, uint32_t col) {
+  const float lo = a.act == SPCONVB_ACT_RELU ? 0.f : -INFINITY;
+  // (ReLU keeps a NaN: fmaxf would drop it)
+  auto act = [&](float v) { return v < lo ? lo : v; };
+  if (a.bias && col + 32u <= a.cout && ((uintptr_t)a.bias & 15u) == 0u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = __ldg((const float4*)(a.bias + col) + i);
+      y[4 * i] = act(fmaf(y[4 * i], a.alpha, b.x));
+      y[4 * i + 1] = act(fmaf(y[4 * i + 1], a.alpha, b.y));
+      y[4 * i + 2] = act(fmaf(y[4 * i + 2], a.alpha, b.z));
+      y[4 * i + 3] = act(fmaf(y[4 * i + 3], a.alpha, b.w));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const bool there = col + i < a.cout;
+      y[i] = there ? act(fmaf(y[i], a.alpha, a.bias ? __ldg(a.bias + col + i) : 0.f)) : 0.f;
+    }
+  }
+  if (a.out_mode == 0) {
+    __half* o = (__half*)a.out + row * a.cout + col;
+    uint32_t h[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __half2 p = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+      h[i] = *(const uint32_t*)&p;
+    }
+    if (a.store == 32) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (col + 16u * i < a.cout) st32(o + 16 * i, h + 8 * i);
+    } else if (a.store == 16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (col + 8u * i < a.cout)
+          ((uint4*)o)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (col + i < a.cout) ((uint16_t*)o)[i] = (uint16_t)(h[i / 2] >> (16 * (i % 2)));
+    }
+    return;
+  }
+  if (col / 2u >= a.out_cpitch) return;
+  uint32_t amax[2] = {0u, 0u}, c[4], byte[2];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) amax[i / 16] = max(amax[i / 16], __float_as_uint(y[i]) & 0x7fffffffu);
+  const bool mx = a.out_mode == 1;
+  if (mx) amax[0] = amax[1] = max(amax[0], amax[1]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float s;
+    byte[h] = mx ? scale_mx(amax[h], s) : scale_nv(amax[h], a.out_ts, s);
+    const bool none = amax[h] >= 0x7f800000u || s == 0.f;
+    const Divider d = divider(mx ? SPCONVB_MXFP4 : SPCONVB_NVFP4, s, amax[h]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = divide(d, y[16 * h + 8 * e + i]);
+      c[2 * h + e] = none ? 0u : codes8(q);
+    }
+  }
+  *(uint4*)(a.out + row * a.out_cpitch + col / 2u) = make_uint4(c[0], c[1], c[2], c[3]);
+  uint8_t* so = a.out_scales + row * a.out_spitch;
+  if (mx) {
+    so[col / 32u] = (uint8_t)byte[0];
+    // bytes behind the last block of rows of an odd number of 64 channels
+    if (col / 2u + 16u == a.out_cpitch && (a.out_cpitch & 32u)) so[col / 32u + 1u] = so[col / 32u + 2u] = 0;
+  } else {
+    *(uint16_t*)(so + col / 16u) = (uint16_t)(byte[0] | byte[1] << 8);
+  }
+}
+
+__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int FMT, int TN>
+__global__ void __launch_bounds__(kCtaThreads, 1)
+fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_map) {
+  using S = Shape<FMT, TN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+  const uint32_t s0 = smem_u32(smem);
+  uint64_t* bars = (uint64_t*)(smem + S::kStages * S::kStage);
+  uint32_t* tmem_holder = (uint32_t*)(bars + 2 * S::kStages + 4);
+  volatile uint32_t* abort_flag = tmem_holder + 1;
+  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::kStages;
+  const uint32_t bar_tfull = bar_empty + 8 * S::kStages, bar_tempty = bar_tfull + 16;
+  const int warp = threadIdx.x >> 5;
+  const uint32_t lane = threadIdx.x & 31;
+
+  if (threadIdx.x < S::kStages) {
+    mbar_init(bar_full + 8 * threadIdx.x, 1 + 4);  // the copies' bytes, the four scale warps
+    mbar_init(bar_empty + 8 * threadIdx.x, 1);
+    if (threadIdx.x < 2) {
+      mbar_init(bar_tfull + 8 * threadIdx.x, 1);
+      mbar_init(bar_tempty + 8 * threadIdx.x, kEpiWarps);
+    }
+    if (threadIdx.x == 0) *abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait_and_trigger();
+  const uint32_t n = min(load_in_order(a.n_ptr), a.cap);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  const uint32_t tiles_n = (a.cout + TN - 1) / TN;
+  const uint32_t tiles = ((n + kTileM - 1) / kTileM) * tiles_n;
+  // this CTA's tiles and its part of K
+  const uint32_t rank = a.split > 1u ? blockIdx.x % a.split : 0u;
+  const uint32_t tile0 = a.split > 1u ? blockIdx.x / a.split : blockIdx.x;
+  const uint32_t tile_step = a.split > 1u ? gridDim.x / a.split : gridDim.x;
+  const uint32_t c0 = a.nchunk * rank / a.split, c1 = a.nchunk * (rank + 1u) / a.split;
+  float part[TN / 2];  // with a split: this thread's sums, over the cluster's barrier
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      uint32_t s = 0, ph = 1, it = 0;
+      bool on = true;
+      for (uint32_t tile = tile0; on && tile < tiles; tile += tile_step) {
+        const uint32_t tm = tile / tiles_n, tn = tile % tiles_n;
+        for (uint32_t c = c0; c < c1; ++c, ++it) {
+          if (!mbar_wait(bar_empty + 8 * s, ph, abort_flag, a.status, 21u) ||
+              (a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) {
+            on = false;
+            break;
+          }
+          const uint32_t st = s0 + s * S::kStage, bar = bar_full + 8 * s;
+          const uint32_t blk = tn * TN / 128u;
+          const uint8_t* w = a.wpk + ((uint64_t)blk * a.nchunk + c) * a.record;
+          if (TN == 256) {
+            const bool two = blk * 128u + 128u < a.cout;
+            mbar_expect_tx(bar, S::kA + (two ? 2u : 1u) * (128u * 128u + S::kSf));
+            tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
+            bulk_g2s(st + S::kOffB, w, 128u * 128u, bar);
+            bulk_g2s(st + S::kOffSfb, w + 128u * 128u, S::kSf, bar);
+            if (two) {
+              const uint8_t* w2 = w + (uint64_t)a.nchunk * a.record;
+              bulk_g2s(st + S::kOffB + 128u * 128u, w2, 128u * 128u, bar);
+              bulk_g2s(st + S::kOffSfb + S::kSf, w2 + 128u * 128u, S::kSf, bar);
+            }
+          } else if (TN == 128) {
+            mbar_expect_tx(bar, S::kA + S::kB + S::kSf);
+            tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
+            bulk_g2s(st + S::kOffB, w, S::kB + S::kSf, bar);
+          } else {
+            mbar_expect_tx(bar, S::kA + S::kB + S::kSf);
+            tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
+            bulk_g2s(st + S::kOffB, w + (tn * TN % 128u) * 128u, S::kB, bar);
+            bulk_g2s(st + S::kOffSfb, w + 128u * 128u, S::kSf, bar);
+          }
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kScaleWarp0) {
+    const uint32_t r = threadIdx.x - 32u * kScaleWarp0;
+    const uint32_t dst = S::kOffSfa + (r % 32u) * 16u + (r / 32u) * 4u;
+    constexpr uint32_t W = S::kWords;
+    const bool vec = a.spitch % (4u * W) == 0u;  // a chunk's words lie whole inside the row
+    auto load = [&](uint32_t tile, uint32_t c, uint32_t (&v)[W]) {
+#pragma unroll
+      for (uint32_t w = 0; w < W; ++w) v[w] = 0u;
+      const uint64_t row = (uint64_t)(tile / tiles_n) * kTileM + r;
+      if (tile >= tiles || row >= n) return;
+      const uint8_t* p = a.scales + row * a.spitch + c * (4u * W);
+      if (vec && W == 4) {
+        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[W - 2]), "=r"(v[W - 1])
+                     : "l"(p)
+                     : "memory");
+      } else if (vec) {
+        asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p) : "memory");
+      } else {
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w)
+          if (c * (4u * W) + 4u * w < a.spitch) v[w] = load_in_order((const uint32_t*)p + w);
+      }
+    };
+    // a cursor for the loads, four chunks ahead of the one for the stages
+    uint32_t lt = tile0, lc = c0, tile = tile0, c = c0, s = 0, ph = 1;
+    auto next = [&](uint32_t& t, uint32_t& k) {
+      if (++k == c1) {
+        k = c0;
+        t += tile_step;
+      }
+    };
+    auto step = [&](uint32_t (&v)[W]) -> bool {
+      if (tile >= tiles) return false;
+      // as one warp: where a wait runs out, it may have for some lanes and not for others
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph, abort_flag, a.status, 22u))) return false;
+      const uint32_t at = s0 + s * S::kStage + dst;
+#pragma unroll
+      for (uint32_t w = 0; w < W; ++w)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + w * kAtomBytes), "r"(v[w]) : "memory");
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_full + 8 * s);
+      load(lt, lc, v);
+      next(lt, lc);
+      next(tile, c);
+      if (++s == S::kStages) {
+        s = 0;
+        ph ^= 1u;
+      }
+      return true;
+    };
+    if (c0 < c1) {
+      uint32_t v0[W], v1[W], v2[W], v3[W];
+      load(lt, lc, v0);
+      next(lt, lc);
+      load(lt, lc, v1);
+      next(lt, lc);
+      load(lt, lc, v2);
+      next(lt, lc);
+      load(lt, lc, v3);
+      next(lt, lc);
+      while (step(v0) && step(v1) && step(v2) && step(v3)) {
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    const bool leader = elect_one();
+    const uint64_t d0 = make_smem_desc(s0);
+    const uint32_t desc_hi = (uint32_t)(d0 >> 32);
+    const uint64_t f0 = scale_desc(s0);
+    const uint32_t sf_hi = (uint32_t)(f0 >> 32);
+    bool alive = true;
+    uint32_t s = 0, ph = 0, tl = 0;
+    for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++tl) {
+      const uint32_t buf = S::kBuffers == 1 ? 0u : tl & 1u, use = S::kBuffers == 1 ? tl : tl >> 1;
+      alive = alive && mbar_wait_spin(bar_tempty + 8 * buf, (use & 1u) ^ 1u, abort_flag, a.status, 23u);
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t d_tmem = tmem + buf * TN;
+      // TN = 64: the tile's channels are the lower or the upper half of the block's
+      const uint32_t sfb_off = TN == 64 ? (tile % tiles_n % 2u) * 2u : 0u;
+      uint32_t accumulate = 0u;
+      for (uint32_t c = c0; c < c1; ++c) {
+        alive = alive && (mbar_test_wait(bar_full + 8 * s, ph) ||
+                          mbar_wait_spin(bar_full + 8 * s, ph, abort_flag, a.status, 24u));
+        __syncwarp();
+        const uint32_t issue = leader && alive ? 1u : 0u;
+        tc_fence_after();
+        const uint32_t st = s * S::kStage;
+        const uint32_t sf_lo = (uint32_t)f0 + (st >> 4);
+        const uint32_t sfa = tmem + S::kBuffers * TN + s * S::kSfCols, sfb = sfa + S::kWords * 4u;
+#pragma unroll
+        for (uint32_t w = 0; w < S::kWords; ++w) {
+          copy_scales_if(issue, sfa + 4u * w, sf_lo + ((S::kOffSfa + w * kAtomBytes) >> 4), sf_hi);
+#pragma unroll
+          for (uint32_t b = 0; b < S::kBlocks; ++b)
+            copy_scales_if(issue, sfb + 4u * (w * S::kBlocks + b),
+                           sf_lo + ((S::kOffSfb + b * S::kSf + w * kAtomBytes) >> 4), sf_hi);
+        }
+        const uint32_t steps = c + 1u == a.nchunk ? a.last_steps : 4u;
+        const uint32_t a_lo = (uint32_t)d0 + (st >> 4), b_lo = a_lo + (S::kOffB >> 4);
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+          constexpr uint32_t kPer = FMT == SPCONVB_MXFP4 ? 2u : 1u;
+          const uint32_t w = k / kPer;
+          umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, a_lo + 2u * k, b_lo + 2u * k, desc_hi,
+                              idesc_of<FMT>(TN, (k % kPer) * 2u), sfa + 4u * w,
+                              sfb + 4u * w * S::kBlocks + sfb_off, k == 0 ? accumulate : 1u);
+        }
+        accumulate = 1u;
+        tc_commit_if(issue, bar_empty + 8 * s);
+        if (++s == S::kStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      tc_commit_if(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
+    }
+    __syncwarp();
+  } else {
+    const uint32_t q = (uint32_t)warp & 3u, half = (uint32_t)warp >> 2;
+    const uint32_t lane_row = 32u * q + lane;
+    uint32_t tl = 0;
+    for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++tl) {
+      const uint32_t buf = S::kBuffers == 1 ? 0u : tl & 1u, use = S::kBuffers == 1 ? tl : tl >> 1;
+      uint32_t ok = 1u;
+      if (lane == 0) ok = mbar_wait(bar_tfull + 8 * buf, use & 1u, abort_flag, a.status, 25u) ? 1u : 0u;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t row = (uint64_t)(tile / tiles_n) * kTileM + lane_row;
+      const uint32_t col0 = (tile % tiles_n) * TN + half * (TN / 2u);
+      const uint32_t taddr = tmem + ((32u * q) << 16) + buf * TN + half * (TN / 2u);
+#pragma unroll
+      for (uint32_t g = 0; g < TN / 64u; ++g) {
+        uint32_t v[32];
+        tmem_ld32(taddr + 32u * g, v);
+        tmem_ld_wait();
+        if (g + 1u == TN / 64u) {  // no more reads of this accumulator by this warp
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+        }
+        if (TN == 64 && a.split > 1u) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) part[i] = __uint_as_float(v[i]);
+        } else if (row < n && col0 + 32u * g < ((a.cout + 63u) & ~63u)) {
+          float y[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(v[i]);
+          emit32(a, y, row, col0 + 32u * g);
+        }
+      }
+    }
+  }
+
+  // A split's sums: every CTA but the first leaves its part in its own shared memory (no copy into it is in flight:
+  // the MMAs have read all there was), the first adds them up in the order of the ranks.
+  if (TN == 64 && a.split > 1u) {
+    const bool epi = warp < kEpiWarps && tile0 < tiles;
+    const uint32_t q = (uint32_t)warp & 3u, half = (uint32_t)warp >> 2, lane_row = 32u * q + lane;
+    const uint64_t row = (uint64_t)(tile0 / tiles_n) * kTileM + lane_row;
+    if (epi && rank != 0u && row < n) {
+#pragma unroll
+      for (uint32_t i = 0; i < 32u; ++i)
+        ((float*)smem)[(half * 32u + i) * kTileM + lane_row] = part[i];
+    }
+    __syncwarp();
+    cluster_sync();
+    if (epi && rank == 0u && row < n) {
+      for (uint32_t p = 1; p < a.split; ++p) {
+#pragma unroll
+        for (uint32_t i = 0; i < 32u; ++i)
+          part[i] += ld_peer(s0 + ((half * 32u + i) * kTileM + lane_row) * 4u, p);
+      }
+      float y[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) y[i] = part[i];
+      emit32(a, y, row, (tile0 % tiles_n) * TN + half * 32u);
+    }
+    __syncwarp();
+    cluster_sync();  // nobody leaves while its part is read
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // give copies already issued a bounded time to land before the CTA exits
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 50000ull) {
+    }
+    __syncthreads();
+  }
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeTiled)p;
+  }();
+  return fn;
+}
+
+template <int FMT, int TN>
+int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, cudaStream_t st) {
+  using S = Shape<FMT, TN>;
+  static bool attr_done[64] = {};
+  int dev = 0;
+  SPCONVB_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+    SPCONVB_CUDA_TRY(cudaFuncSetAttribute(fp4_linear_kernel<FMT, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)S::kSmem));
+    if (dev >= 0 && dev < 64) attr_done[dev] = true;
+  }
+  if (a.split > 1u) {
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = a.split;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles * a.split);
+    cfg.blockDim = dim3(kCtaThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    SPCONVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_linear_kernel<FMT, TN>, a, map));
+    return SPCONVB_OK;
+  }
+  const uint32_t grid = tiles < (uint32_t)kSmCount ? tiles : (uint32_t)kSmCount;
+  SPCONVB_CUDA_TRY(launch_pdl(fp4_linear_kernel<FMT, TN>, dim3(grid), dim3(kCtaThreads), S::kSmem, st, a, map));
+  return SPCONVB_OK;
+}
+
+template <int FMT>
+int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream_t st) {
+  const uint64_t tm = (rows + kTileM - 1) / kTileM;
+  auto tiles = [&](uint32_t tn) { return tm * ((a.cout + tn - 1) / tn); };
+  a.split = 1;
+  // the widest tile that still gives every SM one
+  if (a.cout > 128u && tiles(256) >= (uint64_t)kSmCount)
+    return launch_linear<FMT, 256>(a, map, (uint32_t)tiles(256), st);
+  if (a.cout > 64u && tiles(128) >= (uint64_t)kSmCount)
+    return launch_linear<FMT, 128>(a, map, (uint32_t)tiles(128), st);
+  const uint64_t t = tiles(64);
+  if (t < (uint64_t)kSmCount) {
+    uint32_t split = (uint32_t)((uint64_t)kSmCount / t);
+    if (split > 8u) split = 8u;
+    if (split > a.nchunk) split = a.nchunk;
+    a.split = split;
+  }
+  return launch_linear<FMT, 64>(a, map, (uint32_t)t, st);
+}
+
+}  // namespace
+}  // namespace fp4
+}  // namespace spconvb
+
+using namespace spconvb;
+using namespace spconvb::fp4;
+
+extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes, const void* scales, const uint32_t* n_ptr,
+                                  uint32_t launch_rows, const void* packed, const float* bias, void* out, uint32_t* status,
+                                  void* stream) {
+  if (!p || !codes || !scales || !n_ptr || !packed || !out || launch_rows < 1 || launch_rows > 0x7fffff00u)
+    return SPCONVB_E_ARG;
+  if (!format_ok(p->format) || !channels_ok(p->cin) || !channels_ok(p->cout) || p->kvol != 1 || p->res)
+    return SPCONVB_E_ARG;
+  if (p->act != SPCONVB_ACT_NONE && p->act != SPCONVB_ACT_RELU) return SPCONVB_E_ARG;
+  if (p->out_fp4 && (!p->out_scales || !format_ok(p->out_format) || !tensor_scale_ok(p->out_format, p->out_tensor_scale)))
+    return SPCONVB_E_ARG;
+  if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)packed) & 15u || (uintptr_t)out & (p->out_fp4 ? 15u : 1u) ||
+      (p->out_fp4 && (uintptr_t)p->out_scales & 15u) || (uintptr_t)bias & 3u)
+    return SPCONVB_E_ARG;
+  if (((uint64_t)launch_rows + kTileM - 1) / kTileM * (((uint64_t)p->cout + 63) / 64) > 0x7fffffffu)
+    return SPCONVB_E_RANGE;  // more tiles than a 32-bit number counts
+  LinearArgs a{};
+  const uint32_t cp = cpad((uint32_t)p->cin);
+  a.scales = (const uint8_t*)scales;
+  a.spitch = scale_pitch(p->format, (uint32_t)p->cin);
+  a.nchunk = (cp + kChunkK - 1) / kChunkK;
+  a.last_steps = (cp - (a.nchunk - 1) * kChunkK) / 64u;
+  a.n_ptr = n_ptr;
+  a.cap = launch_rows;
+  a.wpk = (const uint8_t*)packed;
+  a.record = 128u * 128u + words_per_chunk(p->format, cp) * kAtomBytes;
+  a.bias = bias;
+  a.out = (uint8_t*)out;
+  a.out_scales = (uint8_t*)p->out_scales;
+  a.status = status;
+  a.cout = (uint32_t)p->cout;
+  a.alpha = p->alpha;
+  a.act = p->act;
+  a.wait_test = p->wait_test;
+  if (p->out_fp4) {
+    a.out_mode = p->out_format == SPCONVB_MXFP4 ? 1 : 2;
+    a.out_ts = p->out_tensor_scale;
+    a.out_cpitch = code_pitch(a.cout);
+    a.out_spitch = scale_pitch(p->out_format, a.cout);
+  }
+  const uint64_t bits = (uint64_t)(uintptr_t)out | 2ull * a.cout;
+  a.store = bits % 32u == 0u ? 32 : (bits % 16u == 0u ? 16 : 2);
+
+  EncodeTiled encode = encode_tiled();
+  if (!encode) return SPCONVB_E_UNSUPPORTED;
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {cp / 2u, launch_rows}, strides[1] = {cp / 2u};
+  const cuuint32_t box[2] = {128, kTileM}, ones[2] = {1, 1};
+  if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, ones,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return SPCONVB_E_ARG;
+  return p->format == SPCONVB_MXFP4 ? launch_shape<SPCONVB_MXFP4>(a, map, launch_rows, (cudaStream_t)stream)
+                                    : launch_shape<SPCONVB_NVFP4>(a, map, launch_rows, (cudaStream_t)stream);
+}

@@ -1,0 +1,83 @@
+// The block-scaled tensor-core instructions of the 4-bit products, and the tensor-memory copy of their scales.
+#pragma once
+#include <cuda.h>
+
+#include "fp4.cuh"
+#include "umma_common.cuh"
+
+namespace spconvb {
+namespace fp4 {
+
+using namespace umma_detail;
+
+// Instruction descriptor of kind::mxf4 / kind::mxf4nvf4: [4,6) half of the scale word of B, [7,10) A format and [10,12)
+// B format (1 = e2m1), [17,23) N >> 3, [23] scale format (0 = e4m3, 1 = e8m0), [27,29) M >> 7, [29,31) half of the scale
+// word of A; both operands K-major, K = 64.
+template <int FMT>
+__device__ __forceinline__ constexpr uint32_t idesc_of(uint32_t n, uint32_t sf_id) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) |
+         ((FMT == SPCONVB_MXFP4 ? 1u : 0u) << 23) | (1u << 27) | (sf_id << 29);
+}
+
+// One MMA, M = 128, K = 64, by predicate from one lane of a converged warp.
+template <int FMT>
+__device__ __forceinline__ void umma_scaled_if(uint32_t issue, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                               uint32_t desc_hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                               uint32_t accumulate) {
+  if (FMT == SPCONVB_MXFP4) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%7], [%8], p;\n\t}" ::"r"(
+            d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(issue), "r"(sfa), "r"(sfb)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], da, db, %4, [%7], [%8], p;\n\t}" ::"r"(
+            d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(issue), "r"(sfa), "r"(sfb)
+        : "memory");
+  }
+}
+
+// 128 rows of scale words (512 bytes: row r's word at (r % 32) * 16 + (r / 32) * 4) into four columns of tensor memory, the
+// word of row r in lane r % 32 (of every quadrant of lanes) and column r / 32.
+__device__ __forceinline__ void copy_scales_if(uint32_t issue, uint32_t tmem, uint32_t desc_lo, uint32_t desc_hi) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b64 d;\n\tsetp.ne.b32 q, %3, 0;\n\tmov.b64 d, {%1, %2};\n\t"
+      "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem),
+      "r"(desc_lo), "r"(desc_hi), "r"(issue)
+      : "memory");
+}
+// Its shared-memory descriptor: no swizzle, groups of 8 rows of 16 bytes 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) |
+         ((uint64_t)1 << 46);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+}  // namespace fp4
+}  // namespace spconvb

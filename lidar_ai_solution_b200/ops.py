@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import cabi
-from .cabi import ACT_NONE, ACT_RELU, F16, I8  # noqa: F401
+from .cabi import ACT_NONE, ACT_RELU, F16, F32, I8, MXFP4, NVFP4  # noqa: F401
 
 
 # torch's own way to the current stream's handle, a microsecond cheaper a call; not a public one
@@ -274,3 +274,191 @@ def voxelize(points, params, status=None):
                                           _ptr(n_ptr), cabi.FLAG_CLEAR_TAIL, _ptr(status),
                                           _stream()), "voxelize")
     return feat, idx, n_ptr
+
+
+# ------------------------------------------------------------- 4-bit floating point
+_FP4_KIND = {torch.float16: F16, torch.float32: F32, torch.int8: I8}
+
+
+class Fp4Rows:
+    """Rows in 4 bits: ``codes`` uint8 [rows, cpad / 2], ``scales`` uint8 [rows, pitch], the format
+    (``MXFP4`` or ``NVFP4``), the channels, and the tensor scale (1 for ``MXFP4``)."""
+
+    __slots__ = ("codes", "scales", "channels", "fmt", "tensor_scale")
+
+    def __init__(self, codes, scales, channels, fmt, tensor_scale=1.0):
+        lib = cabi.lib()
+        cp, sp = lib.spconvb_fp4_code_pitch(channels), lib.spconvb_fp4_scale_pitch(fmt, channels)
+        if cp == 0 or sp == 0:
+            raise ValueError("no 4-bit rows of %d channels in format %s" % (channels, fmt))
+        for t, pitch in ((codes, cp), (scales, sp)):
+            if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != pitch or not t.is_contiguous():
+                raise ValueError("codes and scales are contiguous uint8 [rows, %d] and [rows, %d]" % (cp, sp))
+        if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
+            raise ValueError("codes and scales of different rows or devices")
+        self.codes, self.scales, self.channels = codes, scales, int(channels)
+        self.fmt, self.tensor_scale = fmt, float(tensor_scale)
+
+    @classmethod
+    def empty(cls, rows, channels, fmt, tensor_scale=1.0, device="cuda"):
+        lib = cabi.lib()
+        return cls(torch.empty((rows, lib.spconvb_fp4_code_pitch(channels)), dtype=torch.uint8, device=device),
+                   torch.empty((rows, lib.spconvb_fp4_scale_pitch(fmt, channels)), dtype=torch.uint8, device=device),
+                   channels, fmt, tensor_scale)
+
+
+def _on_current_device(*tensors):
+    """The library enqueues on the current device's stream: what it is given has to lie there."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != here):
+            raise ValueError("a tensor on %s where the current CUDA device's is wanted" % t.device)
+
+
+def _count_of(n_ptr):
+    if n_ptr.dtype != torch.int32 or n_ptr.numel() < 1:
+        raise ValueError("a row count is an int32 in device memory (device_count)")
+
+
+def _rows_of(t, what, dtypes, rows=None, channels=None, device=None):
+    if t.dtype not in dtypes or t.dim() != 2 or not t.is_contiguous():
+        raise ValueError("%s: a contiguous [rows, channels] tensor of %s" % (what, "/".join(map(str, dtypes))))
+    if rows is not None and t.shape != (rows, channels):
+        raise ValueError("%s: %s where [%d, %d] is wanted" % (what, tuple(t.shape), rows, channels))
+    if device is not None and t.device != device:
+        raise ValueError("%s: on %s and not on %s" % (what, t.device, device))
+
+
+def fp4_quantize(x, n_ptr, fmt, tensor_scale=1.0, in_scale=1.0, out=None):
+    """Rows [rows, channels] fp16, fp32 or int8 (times ``in_scale``) to :class:`Fp4Rows`; ``out``:
+    rows to write into, whose format and tensor scale have to be the same."""
+    _rows_of(x, "x", tuple(_FP4_KIND))
+    _count_of(n_ptr)
+    _on_current_device(x, n_ptr)
+    rows, ch = x.shape
+    if out is None:
+        out = Fp4Rows.empty(rows, ch, fmt, tensor_scale, x.device)
+    elif (out.codes.shape[0], out.channels, out.fmt, out.tensor_scale, out.codes.device) != (
+            rows, ch, fmt, float(tensor_scale), x.device):
+        raise ValueError("out: rows of another shape, format, scale or device")
+    if rows:
+        cabi.check(cabi.lib().spconvb_fp4_quantize(fmt, _ptr(x), _FP4_KIND[x.dtype], in_scale, ch,
+                                                   tensor_scale, _ptr(n_ptr), rows, _ptr(out.codes),
+                                                   _ptr(out.scales), _stream()), "fp4_quantize")
+    return out
+
+
+def fp4_dequantize(q, n_ptr, out_kind=F16, out=None):
+    """What the codes and scales of ``q`` stand for: [rows, channels] fp16 or fp32."""
+    _count_of(n_ptr)
+    _on_current_device(q.codes, n_ptr)
+    rows = q.codes.shape[0]
+    dt = torch.float32 if out_kind == F32 else torch.float16
+    if out is None:
+        out = torch.empty((rows, q.channels), dtype=dt, device=q.codes.device)
+    else:
+        _rows_of(out, "out", (dt,), rows, q.channels, q.codes.device)
+    if rows:
+        cabi.check(cabi.lib().spconvb_fp4_dequantize(q.fmt, _ptr(q.codes), _ptr(q.scales), q.channels,
+                                                     q.tensor_scale, out_kind, _ptr(n_ptr), rows,
+                                                     _ptr(out), _stream()), "fp4_dequantize")
+    return out
+
+
+class Fp4Weights:
+    """One layer's weights in 4 bits, laid out for ``fp4_linear`` (kvol 1) and ``fp4_conv``.  ``w``:
+    [cout, kvol, cin] or [cout, cin], a tensor or an array of fp16 or fp32; ``rows``: the same
+    weights quantised already, as :class:`Fp4Rows` of cout * kvol rows (``w`` is then the
+    shape).  ``bias``: [cout] or None."""
+
+    def __init__(self, w, fmt, tensor_scale=1.0, bias=None, rows=None, device="cuda"):
+        lib = cabi.lib()
+        if rows is None:
+            w = torch.as_tensor(w).to(device)
+            if w.dtype not in (torch.float16, torch.float32):
+                raise ValueError("weights in fp16 or fp32")
+            shape = w.shape
+        else:
+            shape = tuple(w)
+        if len(shape) == 2:
+            shape = (shape[0], 1, shape[1])
+        if len(shape) != 3:
+            raise ValueError("weights are [cout, kvol, cin] or [cout, cin]")
+        self.cout, self.kvol, self.cin = (int(v) for v in shape)
+        self.fmt, self.tensor_scale = fmt, float(tensor_scale)
+        nbytes = lib.spconvb_fp4_packed_bytes(fmt, self.cin, self.cout, self.kvol)
+        if nbytes == 0:
+            raise ValueError("no 4-bit weights [%d, %d, %d] in format %s" % (self.cout, self.kvol, self.cin, fmt))
+        flat = self.cout * self.kvol
+        if rows is None:
+            n = device_count(flat, w.device)
+            rows = fp4_quantize(w.reshape(flat, self.cin).contiguous(), n, fmt, tensor_scale)
+        elif (rows.codes.shape[0], rows.channels, rows.fmt, rows.tensor_scale) != (
+                flat, self.cin, fmt, self.tensor_scale):
+            raise ValueError("rows: of another shape, format or scale")
+        self.packed = torch.empty(nbytes, dtype=torch.uint8, device=rows.codes.device)
+        cabi.check(lib.spconvb_fp4_pack_weights(fmt, self.cin, self.cout, self.kvol, _ptr(rows.codes),
+                                                _ptr(rows.scales), _ptr(self.packed), _stream()), "fp4_pack")
+        self.bias = None
+        if bias is not None:
+            self.bias = torch.as_tensor(bias).to(rows.codes.device, torch.float32).contiguous()
+            if self.bias.shape != (self.cout,):
+                raise ValueError("bias is [cout]")
+
+
+def _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out):
+    if (q.fmt, q.channels) != (wts.fmt, wts.cin) or q.codes.device != wts.packed.device:
+        raise ValueError("rows and weights of different formats, channels or devices")
+    p = cabi.Fp4Params()
+    p.format, p.cin, p.cout, p.kvol = q.fmt, wts.cin, wts.cout, wts.kvol
+    p.alpha, p.act = q.tensor_scale * wts.tensor_scale, act
+    if out_fmt is None:
+        if out is None:
+            out = torch.empty((rows, wts.cout), dtype=torch.float16, device=q.codes.device)
+        else:
+            _rows_of(out, "out", (torch.float16,), rows, wts.cout, q.codes.device)
+        return p, out, out
+    if out is None:
+        out = Fp4Rows.empty(rows, wts.cout, out_fmt, out_tensor_scale, q.codes.device)
+    elif (out.codes.shape[0], out.channels, out.fmt, out.tensor_scale, out.codes.device) != (
+            rows, wts.cout, out_fmt, float(out_tensor_scale), q.codes.device):
+        raise ValueError("out: rows of another shape, format, scale or device")
+    p.out_fp4, p.out_format, p.out_tensor_scale = 1, out_fmt, out_tensor_scale
+    p.out_scales = out.scales.data_ptr()
+    return p, out, out.codes
+
+
+def fp4_linear(q, n_ptr, wts: Fp4Weights, act=ACT_NONE, out_fmt=None, out_tensor_scale=1.0, out=None,
+               status=None, wait_test=0):
+    """act(x W^T + bias) of 4-bit rows: fp16 [rows, cout], or :class:`Fp4Rows` of ``out_fmt``."""
+    _count_of(n_ptr)
+    _on_current_device(q.codes, n_ptr, status)
+    rows = q.codes.shape[0]
+    p, out, buf = _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out)
+    p.wait_test = wait_test
+    if rows:
+        cabi.check(cabi.lib().spconvb_fp4_linear(C.byref(p), _ptr(q.codes), _ptr(q.scales), _ptr(n_ptr), rows,
+                                                 _ptr(wts.packed), _ptr(wts.bias), _ptr(buf), _ptr(status),
+                                                 _stream()), "fp4_linear")
+    return out
+
+
+def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=False, out_fmt=None,
+             out_tensor_scale=1.0, out=None, status=None, launch_rows=0, wait_test=0):
+    """Sparse convolution of 4-bit rows over the map ``m`` [kvol, cap] (as ``conv_forward``): bias,
+    activation, fp16 residual [cap, cout]; fp16 [cap, cout] or :class:`Fp4Rows` of ``out_fmt``."""
+    if m.dtype != torch.int32 or m.dim() != 2 or m.shape[0] != wts.kvol or not m.is_contiguous():
+        raise ValueError("m is a contiguous int32 [kvol, cap]")
+    _count_of(n_out_ptr)
+    _on_current_device(q.codes, m, n_out_ptr, status)
+    cap = m.shape[1]
+    p, out, buf = _fp4_product(q, wts, act, cap, out_fmt, out_tensor_scale, out)
+    if res is not None:
+        _rows_of(res, "res", (torch.float16,), cap, wts.cout, q.codes.device)
+        p.res, p.res_relu = res.data_ptr(), int(res_relu)
+    p.wait_test = wait_test
+    if cap:
+        cabi.check(cabi.lib().spconvb_fp4_conv(C.byref(p), _ptr(q.codes), _ptr(q.scales), _ptr(m), cap,
+                                               _ptr(n_out_ptr), launch_rows, _ptr(wts.packed), _ptr(wts.bias),
+                                               _ptr(buf), _ptr(status), _stream()), "fp4_conv")
+    return out
