@@ -31,6 +31,32 @@ __host__ __device__ inline uint32_t words_per_chunk(int format, uint32_t cp) {
   return 4u / steps_per_word(format, cp);
 }
 
+// 32, 16 and 8 bytes in program order.
+__device__ __forceinline__ void st32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void ld32(const void* p, uint32_t* v) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 ld8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+
 // The block scale of a block whose largest magnitude is `amax` (the bits of a float >= 0, infinity or NaN): its byte,
 // and S in fp32.  x / S of MXFP4 is a multiplication by a power of two.
 __device__ __forceinline__ uint32_t scale_mx(uint32_t amax_bits, float& s) {
@@ -104,8 +130,9 @@ __device__ __forceinline__ Divider divider(int format, float s, uint32_t amax_bi
     d.plain = true;
   } else {
     d.r = __frcp_rn(s);
-    d.plain = s > 1e-27f && s < 1e27f && __uint_as_float(amax_bits) < 1e30f &&
-              __uint_as_float(amax_bits) * d.r < 1e30f;
+    // (a block without codes takes the short way too: what it gives is not used)
+    d.plain = s == 0.f || (s > 1e-27f && s < 1e27f && __uint_as_float(amax_bits) < 1e30f &&
+                           __uint_as_float(amax_bits) * d.r < 1e30f);
   }
   return d;
 }

@@ -2,22 +2,20 @@
 //
 //   out[o, :] = act(alpha * sum_k W[:, k, :] . in[map[k][o], :] + bias)  (+ residual)
 //
-// Weights on the M side (128 accumulator lanes are output channels; twice the same 64 where there are no more), up to
-// kTileRows voxel rows on the N side, K in chunks of 256 channels: 4, 2 or 1 taps of 64, 128 or 256 channels.  Roles of the warps
-// of a CTA (one an SM, walking over tiles whose height deals the rows out evenly):
+// Voxel rows on the M side (a tile is up to 128 of them, one an accumulator lane), output channels on the N side, K in chunks
+// of 256 channels: 4, 2 or 1 taps of 64, 128 or 256 channels.  Roles of the warps of a CTA (one an SM, walking over tiles
+// whose height deals the rows out evenly):
 //
-//   0-7    epilogue: a lane owns a channel, 16 rows a step
+//   0-7    epilogue: a lane owns a row; a warp its quadrant of 32 rows and half of the channels
 //   8      allocates tensor memory, copies the chunk's scales there, issues its MMAs
-//   9-20   producers, two groups that take the chunks in turn; a warp owns 32 rows, a thread one 16-byte segment of 8 of
-//          them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, zeros for missing neighbours,
-//          all of which arrive on the stage's barrier by themselves
-//   21     one lane: the weights, a bulk copy of codes and scales a chunk, or once where all chunks fit
+//   9      one lane: the weights, a bulk copy of codes and scales a chunk, or once where all chunks fit
+//   10-..  producers, kGroups groups of four warps that take the chunks in turn; a warp owns 32 rows, a thread one 16-byte
+//          segment of 8 of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, zeros for missing
+//          neighbours, all of which arrive on the stage's barrier by themselves
 //
 // Within the 32 rows of a warp, row 8 slot + i of the tile lies at 4 i + slot of the operand: the words of scales that
 // the 32 lanes write at the same time then lie in eight groups of four banks and not in two.
-//
-// Scales in tensor memory have a ring of their own, as deep as the accumulators leave room for; where it is shorter than the ring
-// of rows, the MMAs of the chunk that used a place last are waited for before its scales are overwritten.
+#include "fp4_epilogue.cuh"
 #include "fp4_umma.cuh"
 #include "pdl.cuh"
 
@@ -25,11 +23,10 @@ namespace spconvb {
 namespace fp4 {
 namespace {
 
-constexpr uint32_t kTileRows = 192;
-constexpr int kEpiWarps = 8, kMmaWarp = 8, kProdWarp0 = 9;
-constexpr int kProdWarps = 2 * kTileRows / 32;
-constexpr int kWeightWarp = kProdWarp0 + kProdWarps;
-constexpr int kCtaThreads = 32 * (kWeightWarp + 1);
+constexpr uint32_t kTileRows = 128;
+constexpr int kEpiWarps = 8, kMmaWarp = 8, kWeightWarp = 9, kProdWarp0 = 10;
+constexpr uint32_t kGroups = 2;
+constexpr int kCtaThreads = 32 * (kProdWarp0 + 4 * (int)kGroups);
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kRingBytes = 224 * 1024;
 constexpr size_t kSmemBytes = kRingBytes + 1024 + 512;
@@ -41,15 +38,9 @@ struct ConvArgs {
   uint32_t cap;
   const uint32_t* n_out_ptr;
   const uint8_t* wpk;
-  const float* bias;
-  const uint16_t* res;
-  uint8_t* out;
-  uint8_t* out_scales;
   uint32_t* status;
   int kvol;
-  uint32_t cout;
-  float alpha, out_ts;
-  int act, res_relu;
+  Output o;
   int wait_test;
 };
 
@@ -57,52 +48,8 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
 
-// The largest of 16 values over the lanes of each half warp: lane j (mod 16) gets that of value j.
-__device__ __forceinline__ uint32_t max_transposed(const uint32_t (&in)[16], uint32_t lane) {
-  uint32_t v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t keep = lane & 8u ? in[i + 8] : in[i], give = lane & 8u ? in[i] : in[i + 8];
-    v[i] = max(keep, __shfl_xor_sync(0xffffffffu, give, 8));
-  }
-#pragma unroll
-  for (int m = 4; m >= 1; m >>= 1) {
-#pragma unroll
-    for (int i = 0; i < m; ++i) {
-      const uint32_t keep = lane & m ? v[i + m] : v[i], give = lane & m ? v[i] : v[i + m];
-      v[i] = max(keep, __shfl_xor_sync(0xffffffffu, give, m));
-    }
-  }
-  return v[0];
-}
-
-// 16 x 16 nibbles transposed over the lanes of each half warp: nibble i of lane l becomes nibble l of lane i.
-__device__ __forceinline__ void transpose_nibbles(uint32_t (&w)[2], uint32_t lane) {
-  {
-    const bool up = lane & 8u;
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[0] : w[1], 8);
-    w[up ? 0 : 1] = got;
-  }
-  auto swap = [&](uint32_t m, uint32_t sh, uint32_t low) {  // `low`: the nibbles whose index has bit m clear
-    const bool up = lane & m;
-    const uint32_t give = up ? (w[0] & low) | (w[1] & low) << sh : (w[0] >> sh & low) | (w[1] & ~low);
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, give, m);
-    const uint32_t g0 = got & low, g1 = got >> sh & low;
-    if (up) {
-      w[0] = (w[0] & ~low) | g0;
-      w[1] = (w[1] & ~low) | g1;
-    } else {
-      w[0] = (w[0] & low) | g0 << sh;
-      w[1] = (w[1] & low) | g1 << sh;
-    }
-  };
-  swap(4u, 16u, 0x0000ffffu);
-  swap(2u, 8u, 0x00ff00ffu);
-  swap(1u, 4u, 0x0f0f0f0fu);
-}
-
-// CP: stored channels of an input row.  COUT: output channels, rounded up to 64 or 128.  OUT: 0 fp16, 1 MXFP4, 2 NVFP4.
-template <int FMT, int CP, int COUT, int OUT>
+// CP: stored channels of an input row.  COUT: output channels, rounded up to 64 or 128.  RES: with a residual.
+template <int FMT, int CP, int COUT, bool RES>
 __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs a) {
   constexpr int RB = CP / 2;                       // bytes of a row's codes
   constexpr int OPC = 128 / RB, SPO = RB / 16;     // taps a chunk, 16-byte segments a tap
@@ -110,8 +57,11 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   constexpr uint32_t WPT = W / OPC;                // and tap
   constexpr uint32_t kPitch = 4 * WPT;             // bytes of a row's scales
   constexpr uint32_t kSteps = 4 / W;               // MMAs a word
-  constexpr uint32_t kRep = 128 / COUT;
-  constexpr uint32_t kWeightBytes = 128 * 128 + W * kAtomBytes;
+  constexpr uint32_t kRecord = 128 * 128 + W * kAtomBytes;          // a chunk in the weights' image
+  constexpr uint32_t kWeightBytes = COUT * 128 + W * kAtomBytes;     // and in shared memory
+  constexpr uint32_t kRowStage = kTileRows * 128 + W * kAtomBytes, kSfOff = kTileRows * 128;
+  constexpr uint32_t kSfCols = 8 * W;  // of a stage in tensor memory: rows, weights
+  static_assert(2 * COUT + kMaxStages * kSfCols <= kTmemCols, "tensor memory");
 
   const int kbytes = a.kvol * RB;
   const int nchunk = (kbytes + 127) / 128;
@@ -143,17 +93,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   const uint32_t tile_rows = max(32u, ((per_cta + rounds - 1) / rounds + 31u) & ~31u);
   const uint32_t t32 = tile_rows >> 5;
   const uint32_t ntiles = (n_out + tile_rows - 1) / tile_rows;
-  const uint32_t natoms = (tile_rows + 127u) / 128u;
-  // Two rings share the buffer, rows with their scales and weights with theirs; low tiles get deeper ones.
-  const uint32_t sf_off = tile_rows * 128u, row_stage = sf_off + W * natoms * kAtomBytes;
-  const uint32_t fit = min((uint32_t)kMaxStages, kRingBytes / (kWeightBytes + row_stage));
+  // Two rings share the buffer, rows with their scales and weights with theirs.  Weights of which all chunks fit stay.
+  constexpr uint32_t kFit = kRingBytes / (kWeightBytes + kRowStage);
+  const uint32_t fit = min((uint32_t)kMaxStages, kFit);
   const bool resident = (uint32_t)nchunk <= fit;
   const uint32_t nwst = resident ? (uint32_t)nchunk : fit;
-  const uint32_t nst = min((uint32_t)kMaxStages, (kRingBytes - nwst * kWeightBytes) / row_stage);
+  const uint32_t nst = min((uint32_t)kMaxStages, (kRingBytes - nwst * kWeightBytes) / kRowStage);
   const uint32_t sW = smem_u32(smem), sR = sW + nwst * kWeightBytes;
-  // places for scales in tensor memory, behind the two accumulators
-  const uint32_t sf_cols = 4u * W * (1u + natoms);
-  const uint32_t nsf = min(nst, (kTmemCols - 2u * tile_rows) / sf_cols);
 
   if (threadIdx.x < kMaxStages) {
     mbar_init(bar_full + 8 * threadIdx.x, 32u * t32 + 1u);
@@ -180,7 +126,14 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       int j = 0;
       auto fetch = [&]() {
         mbar_expect_tx(bar_full + 8 * s, kWeightBytes);
-        bulk_g2s(sW + ws * kWeightBytes, a.wpk + (size_t)j * kWeightBytes, kWeightBytes, bar_full + 8 * s);
+        const uint8_t* src = a.wpk + (size_t)j * kRecord;
+        const uint32_t dst = sW + ws * kWeightBytes;
+        if (COUT == 128) {
+          bulk_g2s(dst, src, kWeightBytes, bar_full + 8 * s);
+        } else {
+          bulk_g2s(dst, src, COUT * 128, bar_full + 8 * s);
+          bulk_g2s(dst + COUT * 128, src + 128 * 128, W * kAtomBytes, bar_full + 8 * s);
+        }
         if (++s == nst) s = 0;
         if (++ws == nwst) ws = 0;
         if (++j == nchunk) {
@@ -203,7 +156,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   } else if (warp >= kProdWarp0) {
     // ------------------------------------------------------------ producers
     const uint32_t pw_all = (uint32_t)(warp - kProdWarp0);
-    const uint32_t grp = pw_all >= t32 ? 1u : 0u, pw = grp ? pw_all - t32 : pw_all;
+    const uint32_t grp = pw_all >> 2, pw = pw_all & 3u;
     const uint32_t seg = lane & 7u, slot = lane >> 3;
     const uint32_t seg_tap = seg / SPO, seg_in = seg % SPO;
     const uint32_t row_in_tile = pw * 32u + slot * 8u;
@@ -211,8 +164,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     // Scales: of the tap's SPO segments x 8 rows, this thread copies word `word` of rows part, part + kParts, ...
     constexpr uint32_t kParts = SPO / WPT;  // threads that share a word
     const uint32_t word = seg_in % WPT, part = seg_in / WPT;
-    const uint32_t sf_dst = sf_off + (seg_tap * WPT + word) * natoms * kAtomBytes + (pw >> 2) * kAtomBytes + (pw & 3u) * 4u +
-                            slot * 16u;
+    const uint32_t sf_dst = kSfOff + (seg_tap * WPT + word) * kAtomBytes + pw * 4u + slot * 16u;
 
     auto load_idx = [&](uint32_t tile, int j, int32_t (&v)[8]) {
       const int k = j * OPC + (int)seg_tap;
@@ -228,27 +180,24 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
         for (uint32_t i = 0; i < 8; ++i) v[i] = (live && row + i < n_out) ? __ldg(src + i) : -1;
       }
     };
-    auto advance2 = [&](uint32_t& tile, int& j) {  // two chunks on
-      j += 2;
+    auto advance = [&](uint32_t& tile, int& j, int by) {
+      j += by;
       while (j >= nchunk) {
         j -= nchunk;
         tile += gridDim.x;
       }
     };
     uint32_t tile = pw < t32 ? blockIdx.x : ntiles;  // a warp without rows has no chunks
-    int j = grp == 1u ? 1 : 0;
-    while (j >= nchunk) {
-      j -= nchunk;
-      tile += gridDim.x;
-    }
+    int j = 0;
+    advance(tile, j, (int)grp);
     uint32_t ntile = tile;
     int nj = j;
     uint32_t it = grp, s = grp % nst, ph = (grp / nst) & 1u;
-    const uint32_t first_thread = 32u * (kProdWarp0 + grp * t32);
+    const uint32_t first_thread = 32u * (kProdWarp0 + grp * 4u);
     auto step = [&](int32_t (&idx)[8]) -> bool {
       if (tile >= ntiles) return false;
       if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, abort_flag, a.status, 31u)) return false;
-      const uint32_t stage = sR + s * row_stage;
+      const uint32_t stage = sR + s * kRowStage;
       // what lies in K steps past the last tap is never read by an MMA
       const bool dead_seg = j == nchunk - 1 && (seg >> 1) >= last_steps;
       if (!dead_seg) {
@@ -274,10 +223,10 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       // the weights' arrival, where they are there already
       if (resident && tile != blockIdx.x && threadIdx.x == first_thread) mbar_arrive(bar_full + 8 * s);
       load_idx(ntile, nj, idx);
-      advance2(ntile, nj);
-      advance2(tile, j);
-      it += 2;
-      s += 2;
+      advance(ntile, nj, kGroups);
+      advance(tile, j, kGroups);
+      it += kGroups;
+      s += kGroups;
       if (s >= nst) {
         s -= nst;
         ph ^= 1u;
@@ -286,9 +235,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     };
     int32_t idx_a[8], idx_b[8];
     load_idx(ntile, nj, idx_a);
-    advance2(ntile, nj);
+    advance(ntile, nj, kGroups);
     load_idx(ntile, nj, idx_b);
-    advance2(ntile, nj);
+    advance(ntile, nj, kGroups);
     while (step(idx_a) && step(idx_b)) {
     }
     cp_async_wait_all();  // nothing of this thread may still be writing when the CTA exits
@@ -300,49 +249,37 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     const uint32_t desc_hi = (uint32_t)(wdesc0 >> 32);
     const uint32_t sf_hi = (uint32_t)(scale_desc(sW) >> 32), sfw0 = (uint32_t)scale_desc(sW), sfr0 = (uint32_t)scale_desc(sR);
     bool alive = true;
-    uint32_t s = 0, ws = 0, ph = 0, tl = 0, sf = 0, it = 0;
-    uint32_t os = 0, oph = 0;  // stage and phase of the chunk `nsf` before
+    uint32_t s = 0, ws = 0, ph = 0, tl = 0;
     for (uint32_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++tl) {
       const uint32_t buf = tl & 1u;
       alive = alive && mbar_wait_spin(bar_tempty + 8 * buf, ((tl >> 1) & 1u) ^ 1u, abort_flag, a.status, 32u);
       __syncwarp();
       tc_fence_after();
-      const uint32_t d_tmem = tmem_base + buf * tile_rows;
+      const uint32_t d_tmem = tmem_base + buf * COUT;
       uint32_t accumulate = 0u;
 #pragma unroll 1
       for (int j = 0; j < nchunk; ++j) {
         alive = alive && (mbar_test_wait(bar_full + 8 * s, ph) ||
                           mbar_wait_spin(bar_full + 8 * s, ph, abort_flag, a.status, 33u));
         __syncwarp();
-        if (it >= nsf && nsf < nst) {
-          alive = alive && (mbar_test_wait(bar_empty + 8 * os, oph) ||
-                            mbar_wait_spin(bar_empty + 8 * os, oph, abort_flag, a.status, 37u));
-          __syncwarp();
-          if (++os == nst) {
-            os = 0;
-            oph ^= 1u;
-          }
-        }
-        ++it;
         const uint32_t issue = leader && alive ? 1u : 0u;
         fence_proxy_async();  // rows come through the generic proxy, MMAs and copies read through the async one
         tc_fence_after();
-        const uint32_t w_at = (ws * kWeightBytes) >> 4, r_at = (s * row_stage) >> 4;
-        const uint32_t sfw = tmem_base + 2u * tile_rows + sf * sf_cols, sfr = sfw + 4u * W;
+        const uint32_t w_at = (ws * kWeightBytes) >> 4, r_at = (s * kRowStage) >> 4;
+        // a place for every stage: it is filled again only when the MMAs that read its scales are complete
+        const uint32_t sfr = tmem_base + 2u * COUT + s * kSfCols, sfw = sfr + 4u * W;
 #pragma unroll
         for (uint32_t w = 0; w < W; ++w) {
-          copy_scales_if(issue, sfw + 4u * w, sfw0 + w_at + ((128u * 128u + w * kAtomBytes) >> 4), sf_hi);
-          copy_scales_if(issue, sfr + 4u * w * natoms, sfr0 + r_at + ((sf_off + w * natoms * kAtomBytes) >> 4), sf_hi);
-          copy_scales_if(natoms == 2u ? issue : 0u, sfr + 8u * w + 4u,
-                         sfr0 + r_at + ((sf_off + (2u * w + 1u) * kAtomBytes) >> 4), sf_hi);
+          copy_scales_if(issue, sfr + 4u * w, sfr0 + r_at + ((kSfOff + w * kAtomBytes) >> 4), sf_hi);
+          copy_scales_if(issue, sfw + 4u * w, sfw0 + w_at + ((COUT * 128u + w * kAtomBytes) >> 4), sf_hi);
         }
         const uint32_t steps = j + 1 == nchunk ? last_steps : 4u;
         const uint32_t wd = (uint32_t)wdesc0 + w_at, rd = (uint32_t)rdesc0 + r_at;
 #pragma unroll
         for (uint32_t k = 0; k < 4u; ++k) {
           const uint32_t w = k / kSteps;
-          umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, wd + 2u * k, rd + 2u * k, desc_hi,
-                              idesc_of<FMT>(tile_rows, (k % kSteps) * 2u), sfw + 4u * w, sfr + 4u * w * natoms,
+          umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, rd + 2u * k, wd + 2u * k, desc_hi,
+                              idesc_of<FMT>(COUT, (k % kSteps) * 2u), sfr + 4u * w, sfw + 4u * w,
                               k == 0 ? accumulate : 1u);
         }
         accumulate = 1u;
@@ -352,121 +289,49 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
           ph ^= 1u;
         }
         if (++ws == nwst) ws = 0;
-        if (++sf == nsf) sf = 0;
       }
       tc_commit_if(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------- epilogue
-    // Accumulator lane m holds channel m % COUT of weight copy m / COUT; copy c takes cols_rep columns from c * cols_rep on,
-    // and the two warps of a lane quadrant its groups of 16 in turn.
-    const uint32_t q = (uint32_t)warp & 3u, part = (uint32_t)warp >> 2;
-    const uint32_t ch = (32u * q + lane) % COUT, copy = (32u * q) / COUT;
-    const uint32_t cols_rep = (t32 + kRep - 1u) / kRep * 32u;
-    const uint32_t first_col = copy * cols_rep;
-    const uint32_t cols = first_col < tile_rows ? min(cols_rep, tile_rows - first_col) : 0u;
-    const bool there = ch < a.cout;
-    const float bi = a.bias && there ? __ldg(a.bias + ch) : 0.f;
-    const float lo = a.act == SPCONVB_ACT_RELU ? 0.f : -INFINITY, lo2 = a.res_relu ? 0.f : -INFINITY;
+    const uint32_t q = (uint32_t)warp & 3u, half = (uint32_t)warp >> 2;
+    // lane 4 i + slot of a quadrant is row 8 slot + i of its 32
+    const uint32_t row_in_tile = 32u * q + (lane & 3u) * 8u + (lane >> 2);
+    constexpr uint32_t kSets = COUT / 64;  // sets of 32 channels of a warp
+    const uint32_t col0 = half * (COUT / 2u), most = (a.o.cout + 63u) & ~63u;
     uint32_t tl = 0;
     for (uint32_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++tl) {
       const uint32_t buf = tl & 1u;
+      const uint64_t row = (uint64_t)tile * tile_rows + row_in_tile;
+      const bool live = row_in_tile < tile_rows && row < n_out;
+      uint32_t res[kSets][16];
+      if (RES) {
+#pragma unroll
+        for (uint32_t g = 0; g < kSets; ++g)
+          if (live) load_residual(a.o, row, col0 + 32u * g, res[g]);
+      }
       uint32_t ok = 1u;
       if (lane == 0) ok = mbar_wait(bar_tfull + 8 * buf, (tl >> 1) & 1u, abort_flag, a.status, 34u) ? 1u : 0u;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((32u * q) << 16) + buf * tile_rows + first_col;
-      auto release = [&]() {  // no more reads of this accumulator by this warp
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
-      };
-      uint32_t col = 16u * part;
-      if (col >= cols) release();
-#pragma unroll 1
-      for (; col < cols; col += 32u) {
-        uint32_t v[16];
-        tmem_ld16(taddr + col, v);
-        // column 4 i + slot of a group of 32 is its row 8 slot + i
-        const uint64_t row0 = (uint64_t)tile * tile_rows + ((first_col + col) & ~31u) + (col & 16u ? 4u : 0u);
-        auto row_of = [&](uint32_t i) { return row0 + (i % 4u) * 8u + i / 4u; };
-        uint16_t r[16];
-        if (a.res) {
+      const uint32_t taddr = tmem_base + ((32u * q) << 16) + buf * COUT + col0;
 #pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) {
-            r[i] = 0;
-            if (there && row_of(i) < n_out) r[i] = (uint16_t)load_in_order(a.res + row_of(i) * a.cout + ch);
-          }
-        }
+      for (uint32_t g = 0; g < kSets; ++g) {
+        uint32_t v[32];
+        tmem_ld32(taddr + 32u * g, v);
         tmem_ld_wait();
-        if (col + 32u >= cols) release();
-        float y[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          y[i] = fmaf(__uint_as_float(v[i]), a.alpha, bi);
-          y[i] = y[i] < lo ? lo : y[i];  // keeps a NaN
+        if (g + 1u == kSets) {  // no more reads of this accumulator by this warp
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
         }
-        if (a.res) {
+        if (live && col0 + 32u * g < most) {
+          float y[32];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            y[i] = __fadd_rn(__half2float(__float2half_rn(y[i])), __half2float(__ushort_as_half(r[i])));
-            y[i] = y[i] < lo2 ? lo2 : y[i];
-          }
-        }
-        if (OUT == 0) {
-          __half* o = (__half*)a.out + row0 * a.cout + ch;
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i)
-            if (there && row_of(i) < n_out)
-              o[(size_t)((i % 4u) * 8u + i / 4u) * a.cout] = __float2half_rn(y[i]);
-        } else {
-          // Codes of 16 rows x 32 channels.  Lane j of each half warp finds the scale of row j; the codes, a lane a channel, are
-          // then transposed so that lane j stores 8 bytes of row j.
-          constexpr bool mx = OUT == 1;
-          uint32_t m[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (!there) y[i] = 0.f;
-            m[i] = __float_as_uint(y[i]) & 0x7fffffffu;
-          }
-          uint32_t amax = max_transposed(m, lane);
-          if (mx) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
-          float s;
-          const uint32_t byte = mx ? scale_mx(amax, s) : scale_nv(amax, a.out_ts, s);
-          const Divider mine = divider(mx ? SPCONVB_MXFP4 : SPCONVB_NVFP4, s, amax);
-          const uint32_t none = __ballot_sync(0xffffffffu, amax >= 0x7f800000u || s == 0.f);
-          const uint32_t plain = __ballot_sync(0xffffffffu, mine.plain);
-          uint32_t w[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float qv[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t from = (lane & 16u) + 8u * h + e;
-              Divider d;
-              d.r = __shfl_sync(0xffffffffu, mine.r, from);
-              d.s = mx ? 0.f : __shfl_sync(0xffffffffu, mine.s, from);
-              d.exact_scale = mx;
-              d.plain = (plain >> from) & 1u;
-              qv[e] = (none >> from) & 1u ? 0.f : divide(d, y[8 * h + e]);
-            }
-            w[h] = codes8(qv);
-          }
-          transpose_nibbles(w, lane);
-          const uint64_t row = row_of(lane & 15u);
-          if (row < n_out) {
-            const uint32_t ch0 = (32u * q) % COUT + (lane & 16u);
-            *(uint2*)(a.out + row * (COUT / 2u) + ch0 / 2u) = make_uint2(w[0], w[1]);
-            if (!mx) {
-              a.out_scales[row * (COUT / 16u) + ch0 / 16u] = (uint8_t)byte;
-            } else if (lane < 16u) {
-              uint8_t* so = a.out_scales + row * 4u + ch0 / 32u;
-              so[0] = (uint8_t)byte;
-              if (COUT == 64 && ch0 == 32u) so[1] = so[2] = 0;
-            }
-          }
+          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(v[i]);
+          emit32<RES>(a.o, y, row, col0 + 32u * g, res[g]);
         }
       }
     }
@@ -488,34 +353,33 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   }
 }
 
-template <int FMT, int CP, int COUT, int OUT>
+template <int FMT, int CP, int COUT, bool RES>
 int launch_conv(const ConvArgs& a, uint32_t launch_rows, cudaStream_t st) {
   static bool attr_done[64] = {};
   int dev = 0;
   SPCONVB_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    SPCONVB_CUDA_TRY(cudaFuncSetAttribute(fp4_conv_kernel<FMT, CP, COUT, OUT>,
+    SPCONVB_CUDA_TRY(cudaFuncSetAttribute(fp4_conv_kernel<FMT, CP, COUT, RES>,
                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
   const uint32_t tiles = (launch_rows + 31) / 32;  // the kernel picks the tile height
   const uint32_t grid = tiles < (uint32_t)kSmCount ? (tiles ? tiles : 1u) : (uint32_t)kSmCount;
-  SPCONVB_CUDA_TRY(launch_pdl(fp4_conv_kernel<FMT, CP, COUT, OUT>, dim3(grid), dim3(kCtaThreads), kSmemBytes, st, a));
+  SPCONVB_CUDA_TRY(launch_pdl(fp4_conv_kernel<FMT, CP, COUT, RES>, dim3(grid), dim3(kCtaThreads), kSmemBytes, st, a));
   return SPCONVB_OK;
 }
 template <int FMT, int CP, int COUT>
-int launch_out(int out, const ConvArgs& a, uint32_t rows, cudaStream_t st) {
-  if (out == 0) return launch_conv<FMT, CP, COUT, 0>(a, rows, st);
-  return out == 1 ? launch_conv<FMT, CP, COUT, 1>(a, rows, st) : launch_conv<FMT, CP, COUT, 2>(a, rows, st);
+int launch_res(const ConvArgs& a, uint32_t rows, cudaStream_t st) {
+  return a.o.res ? launch_conv<FMT, CP, COUT, true>(a, rows, st) : launch_conv<FMT, CP, COUT, false>(a, rows, st);
 }
 template <int FMT, int CP>
-int launch_cout(int out, const ConvArgs& a, uint32_t rows, cudaStream_t st) {
-  return a.cout <= 64u ? launch_out<FMT, CP, 64>(out, a, rows, st) : launch_out<FMT, CP, 128>(out, a, rows, st);
+int launch_cout(const ConvArgs& a, uint32_t rows, cudaStream_t st) {
+  return a.o.cout <= 64u ? launch_res<FMT, CP, 64>(a, rows, st) : launch_res<FMT, CP, 128>(a, rows, st);
 }
 template <int FMT>
-int launch_cin(uint32_t cp, int out, const ConvArgs& a, uint32_t rows, cudaStream_t st) {
-  if (cp == 64u) return launch_cout<FMT, 64>(out, a, rows, st);
-  return cp == 128u ? launch_cout<FMT, 128>(out, a, rows, st) : launch_cout<FMT, 256>(out, a, rows, st);
+int launch_cin(uint32_t cp, const ConvArgs& a, uint32_t rows, cudaStream_t st) {
+  if (cp == 64u) return launch_cout<FMT, 64>(a, rows, st);
+  return cp == 128u ? launch_cout<FMT, 128>(a, rows, st) : launch_cout<FMT, 256>(a, rows, st);
 }
 
 }  // namespace
@@ -538,37 +402,23 @@ int spconvb_fp4_conv(const spconvb_fp4_params* p, const void* codes, const void*
   if (!p || !codes || !scales || !map || !n_out_ptr || !packed || !out || cap < 1 || cap > 0x7fffff00u)
     return SPCONVB_E_ARG;
   if (!format_ok(p->format) || !channels_ok(p->cin) || !channels_ok(p->cout) || p->kvol < 1) return SPCONVB_E_ARG;
-  if (p->act != SPCONVB_ACT_NONE && p->act != SPCONVB_ACT_RELU) return SPCONVB_E_ARG;
-  if (p->out_fp4 && (!p->out_scales || !format_ok(p->out_format) || !tensor_scale_ok(p->out_format, p->out_tensor_scale)))
-    return SPCONVB_E_ARG;
-  if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)packed) & 15u || (uintptr_t)out & (p->out_fp4 ? 15u : 1u) ||
-      (p->out_fp4 && (uintptr_t)p->out_scales & 15u) || ((uintptr_t)bias | (uintptr_t)map) & 3u || (uintptr_t)p->res & 1u)
+  ConvArgs a{};
+  if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)packed) & 15u || (uintptr_t)map & 3u || !make_output(*p, bias, out, a.o))
     return SPCONVB_E_ARG;
   if (!spconvb_fp4_conv_supported(p->cin, p->cout, p->kvol)) return SPCONVB_E_UNSUPPORTED;
   if (launch_rows == 0 || launch_rows > cap) launch_rows = cap;
-  ConvArgs a{};
   a.codes = (const uint8_t*)codes;
   a.scales = (const uint8_t*)scales;
   a.map = map;
   a.cap = cap;
   a.n_out_ptr = n_out_ptr;
   a.wpk = (const uint8_t*)packed;
-  a.bias = bias;
-  a.res = (const uint16_t*)p->res;
-  a.out = (uint8_t*)out;
-  a.out_scales = (uint8_t*)p->out_scales;
   a.status = status;
   a.kvol = p->kvol;
-  a.cout = (uint32_t)p->cout;
-  a.alpha = p->alpha;
-  a.out_ts = p->out_fp4 ? p->out_tensor_scale : 1.f;
-  a.act = p->act;
-  a.res_relu = p->res_relu;
   a.wait_test = p->wait_test;
-  const int mode = !p->out_fp4 ? 0 : (p->out_format == SPCONVB_MXFP4 ? 1 : 2);
   const uint32_t cp = cpad((uint32_t)p->cin);
-  return p->format == SPCONVB_MXFP4 ? launch_cin<SPCONVB_MXFP4>(cp, mode, a, launch_rows, (cudaStream_t)stream)
-                                    : launch_cin<SPCONVB_NVFP4>(cp, mode, a, launch_rows, (cudaStream_t)stream);
+  return p->format == SPCONVB_MXFP4 ? launch_cin<SPCONVB_MXFP4>(cp, a, launch_rows, (cudaStream_t)stream)
+                                    : launch_cin<SPCONVB_NVFP4>(cp, a, launch_rows, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -15,6 +15,7 @@
 //
 // Few rows: the K axis is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
 // always in the same order.
+#include "fp4_epilogue.cuh"
 #include "fp4_umma.cuh"
 #include "pdl.cuh"
 
@@ -34,14 +35,8 @@ struct LinearArgs {
   uint32_t cap;
   const uint8_t* wpk;
   uint32_t record;  // bytes of a block of 128 channels of a chunk in the weights' image
-  const float* bias;
-  uint8_t* out;
-  uint8_t* out_scales;
   uint32_t* status;
-  uint32_t cout, out_cpitch, out_spitch;
-  float alpha, out_ts;
-  int act, out_mode;  // 0: fp16, 1: MXFP4, 2: NVFP4
-  int store;          // bytes of fp16 output that may be stored at once: 32, 16 or 2
+  Output o;
   uint32_t split;     // CTAs of a cluster that share a tile's K
   int wait_test;
 };
@@ -62,88 +57,6 @@ struct Shape {
   static_assert(kBuffers * TN + kStages * kSfCols <= kTmemCols, "tensor memory");
   static_assert(kSmem <= 232448, "shared memory");
 };
-
-__device__ __forceinline__ void st32(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "l"(p)
-               : "memory");
-}
-
-// 32 channels of one row from fp32 sums to memory.  `col` is a multiple of 32; the row exists.
-__device__ __forceinline__ void emit32(const LinearArgs& a, float (&y)[32], uint64_t row, uint32_t col) {
-  const float lo = a.act == SPCONVB_ACT_RELU ? 0.f : -INFINITY;
-  // (ReLU keeps a NaN: fmaxf would drop it)
-  auto act = [&](float v) { return v < lo ? lo : v; };
-  if (a.bias && col + 32u <= a.cout && ((uintptr_t)a.bias & 15u) == 0u) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 b = __ldg((const float4*)(a.bias + col) + i);
-      y[4 * i] = act(fmaf(y[4 * i], a.alpha, b.x));
-      y[4 * i + 1] = act(fmaf(y[4 * i + 1], a.alpha, b.y));
-      y[4 * i + 2] = act(fmaf(y[4 * i + 2], a.alpha, b.z));
-      y[4 * i + 3] = act(fmaf(y[4 * i + 3], a.alpha, b.w));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const bool there = col + i < a.cout;
-      y[i] = there ? act(fmaf(y[i], a.alpha, a.bias ? __ldg(a.bias + col + i) : 0.f)) : 0.f;
-    }
-  }
-  if (a.out_mode == 0) {
-    __half* o = (__half*)a.out + row * a.cout + col;
-    uint32_t h[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const __half2 p = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
-      h[i] = *(const uint32_t*)&p;
-    }
-    if (a.store == 32) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (col + 16u * i < a.cout) st32(o + 16 * i, h + 8 * i);
-    } else if (a.store == 16) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col + 8u * i < a.cout)
-          ((uint4*)o)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col + i < a.cout) ((uint16_t*)o)[i] = (uint16_t)(h[i / 2] >> (16 * (i % 2)));
-    }
-    return;
-  }
-  if (col / 2u >= a.out_cpitch) return;
-  uint32_t amax[2] = {0u, 0u}, c[4], byte[2];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) amax[i / 16] = max(amax[i / 16], __float_as_uint(y[i]) & 0x7fffffffu);
-  const bool mx = a.out_mode == 1;
-  if (mx) amax[0] = amax[1] = max(amax[0], amax[1]);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float s;
-    byte[h] = mx ? scale_mx(amax[h], s) : scale_nv(amax[h], a.out_ts, s);
-    const bool none = amax[h] >= 0x7f800000u || s == 0.f;
-    const Divider d = divider(mx ? SPCONVB_MXFP4 : SPCONVB_NVFP4, s, amax[h]);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float q[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = divide(d, y[16 * h + 8 * e + i]);
-      c[2 * h + e] = none ? 0u : codes8(q);
-    }
-  }
-  *(uint4*)(a.out + row * a.out_cpitch + col / 2u) = make_uint4(c[0], c[1], c[2], c[3]);
-  uint8_t* so = a.out_scales + row * a.out_spitch;
-  if (mx) {
-    so[col / 32u] = (uint8_t)byte[0];
-    // bytes behind the last block of rows of an odd number of 64 channels
-    if (col / 2u + 16u == a.out_cpitch && (a.out_cpitch & 32u)) so[col / 32u + 1u] = so[col / 32u + 2u] = 0;
-  } else {
-    *(uint16_t*)(so + col / 16u) = (uint16_t)(byte[0] | byte[1] << 8);
-  }
-}
 
 __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
   uint32_t remote;
@@ -196,13 +109,14 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
-  const uint32_t tiles_n = (a.cout + TN - 1) / TN;
+  const uint32_t tiles_n = (a.o.cout + TN - 1) / TN;
   const uint32_t tiles = ((n + kTileM - 1) / kTileM) * tiles_n;
   // this CTA's tiles and its part of K
   const uint32_t rank = a.split > 1u ? blockIdx.x % a.split : 0u;
   const uint32_t tile0 = a.split > 1u ? blockIdx.x / a.split : blockIdx.x;
   const uint32_t tile_step = a.split > 1u ? gridDim.x / a.split : gridDim.x;
   const uint32_t c0 = a.nchunk * rank / a.split, c1 = a.nchunk * (rank + 1u) / a.split;
+  const uint32_t no_res[16] = {};
   float part[TN / 2];  // with a split: this thread's sums, over the cluster's barrier
 
   if (warp == kLoadWarp) {
@@ -221,7 +135,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
           const uint32_t blk = tn * TN / 128u;
           const uint8_t* w = a.wpk + ((uint64_t)blk * a.nchunk + c) * a.record;
           if (TN == 256) {
-            const bool two = blk * 128u + 128u < a.cout;
+            const bool two = blk * 128u + 128u < a.o.cout;
             mbar_expect_tx(bar, S::kA + (two ? 2u : 1u) * (128u * 128u + S::kSf));
             tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
             bulk_g2s(st + S::kOffB, w, 128u * 128u, bar);
@@ -395,11 +309,11 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
         if (TN == 64 && a.split > 1u) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) part[i] = __uint_as_float(v[i]);
-        } else if (row < n && col0 + 32u * g < ((a.cout + 63u) & ~63u)) {
+        } else if (row < n && col0 + 32u * g < ((a.o.cout + 63u) & ~63u)) {
           float y[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(v[i]);
-          emit32(a, y, row, col0 + 32u * g);
+          emit32<false>(a.o, y, row, col0 + 32u * g, no_res);
         }
       }
     }
@@ -427,7 +341,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
       float y[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) y[i] = part[i];
-      emit32(a, y, row, (tile0 % tiles_n) * TN + half * 32u);
+      emit32<false>(a.o, y, row, (tile0 % tiles_n) * TN + half * 32u, no_res);
     }
     __syncwarp();
     cluster_sync();  // nobody leaves while its part is read
@@ -501,12 +415,12 @@ int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, c
 template <int FMT>
 int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream_t st) {
   const uint64_t tm = (rows + kTileM - 1) / kTileM;
-  auto tiles = [&](uint32_t tn) { return tm * ((a.cout + tn - 1) / tn); };
+  auto tiles = [&](uint32_t tn) { return tm * ((a.o.cout + tn - 1) / tn); };
   a.split = 1;
   // the widest tile that still gives every SM one
-  if (a.cout > 128u && tiles(256) >= (uint64_t)kSmCount)
+  if (a.o.cout > 128u && tiles(256) >= (uint64_t)kSmCount)
     return launch_linear<FMT, 256>(a, map, (uint32_t)tiles(256), st);
-  if (a.cout > 64u && tiles(128) >= (uint64_t)kSmCount)
+  if (a.o.cout > 64u && tiles(128) >= (uint64_t)kSmCount)
     return launch_linear<FMT, 128>(a, map, (uint32_t)tiles(128), st);
   const uint64_t t = tiles(64);
   if (t < (uint64_t)kSmCount) {
@@ -532,15 +446,10 @@ extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes
     return SPCONVB_E_ARG;
   if (!format_ok(p->format) || !channels_ok(p->cin) || !channels_ok(p->cout) || p->kvol != 1 || p->res)
     return SPCONVB_E_ARG;
-  if (p->act != SPCONVB_ACT_NONE && p->act != SPCONVB_ACT_RELU) return SPCONVB_E_ARG;
-  if (p->out_fp4 && (!p->out_scales || !format_ok(p->out_format) || !tensor_scale_ok(p->out_format, p->out_tensor_scale)))
-    return SPCONVB_E_ARG;
-  if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)packed) & 15u || (uintptr_t)out & (p->out_fp4 ? 15u : 1u) ||
-      (p->out_fp4 && (uintptr_t)p->out_scales & 15u) || (uintptr_t)bias & 3u)
-    return SPCONVB_E_ARG;
+  LinearArgs a{};
+  if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)packed) & 15u || !make_output(*p, bias, out, a.o)) return SPCONVB_E_ARG;
   if (((uint64_t)launch_rows + kTileM - 1) / kTileM * (((uint64_t)p->cout + 63) / 64) > 0x7fffffffu)
     return SPCONVB_E_RANGE;  // more tiles than a 32-bit number counts
-  LinearArgs a{};
   const uint32_t cp = cpad((uint32_t)p->cin);
   a.scales = (const uint8_t*)scales;
   a.spitch = scale_pitch(p->format, (uint32_t)p->cin);
@@ -550,22 +459,8 @@ extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes
   a.cap = launch_rows;
   a.wpk = (const uint8_t*)packed;
   a.record = 128u * 128u + words_per_chunk(p->format, cp) * kAtomBytes;
-  a.bias = bias;
-  a.out = (uint8_t*)out;
-  a.out_scales = (uint8_t*)p->out_scales;
   a.status = status;
-  a.cout = (uint32_t)p->cout;
-  a.alpha = p->alpha;
-  a.act = p->act;
   a.wait_test = p->wait_test;
-  if (p->out_fp4) {
-    a.out_mode = p->out_format == SPCONVB_MXFP4 ? 1 : 2;
-    a.out_ts = p->out_tensor_scale;
-    a.out_cpitch = code_pitch(a.cout);
-    a.out_spitch = scale_pitch(p->out_format, a.cout);
-  }
-  const uint64_t bits = (uint64_t)(uintptr_t)out | 2ull * a.cout;
-  a.store = bits % 32u == 0u ? 32 : (bits % 16u == 0u ? 16 : 2);
 
   EncodeTiled encode = encode_tiled();
   if (!encode) return SPCONVB_E_UNSUPPORTED;

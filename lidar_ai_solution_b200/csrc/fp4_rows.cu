@@ -2,7 +2,12 @@
 //
 // All three only move bytes.  A thread owns a unit of 16 channels: 32 bytes of fp16 in one load, 8 bytes of codes in one store, so
 // a warp reads and writes contiguous kilobytes; the scale of an MXFP4 block belongs to two neighbouring lanes, which
-// exchange their largest magnitudes.
+// exchange their largest magnitudes.  Rows go one of three ways:
+//   flat     no padding anywhere (channels a multiple of 64 or 128) and 32-byte alignment: units, codes and scales are one sequence
+//            each, and a thread keeps the loads of kAhead units in flight
+//   aligned  rows that start on 16 bytes: a unit is found by its row, 16 bytes at a time
+//   staged   all others: 256 units in a row are one contiguous piece of the fp16 / fp32 / int8 side, which passes through
+//            shared memory in 16-byte pieces
 #include "fp4.cuh"
 #include "pdl.cuh"
 
@@ -11,13 +16,14 @@ namespace fp4 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 2;
+enum Way { kFlat, kAligned, kStaged };
 
 struct Rows {
   uint32_t channels, upr;  // units of 16 channels a row, padding included
   uint64_t upr_inv;        // ceil(2^64 / upr): u / upr = hi64(u * upr_inv) for u < 2^48, upr <= 4096
   uint32_t cpitch, spitch;
-  int flat;                // no padding anywhere: units, codes and scales are one sequence
-  int aligned;             // of a row's first element: 32, 16, or 0 (that of the element)
+  Way way;
 };
 
 // Row and unit in the row of unit u.
@@ -25,31 +31,12 @@ __device__ __forceinline__ void place(const Rows& g, uint64_t u, uint64_t& row, 
   row = __umul64hi(u, g.upr_inv);
   ub = (uint32_t)(u - row * g.upr);
 }
-
-__device__ __forceinline__ void ld32(const void* p, uint32_t (&v)[8]) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-               : "l"(p)
-               : "memory");
+// Channels of a unit that exist, and its first element counted from the first row's.
+__device__ __forceinline__ uint32_t present(const Rows& g, uint32_t ub) {
+  return ub * 16u < g.channels ? min(16u, g.channels - ub * 16u) : 0u;
 }
-__device__ __forceinline__ void st32(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "l"(p)
-               : "memory");
-}
-__device__ __forceinline__ uint4 ld16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p)
-               : "memory");
-  return v;
-}
-
-__device__ __forceinline__ uint2 ld8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-  return v;
+__device__ __forceinline__ uint64_t element_at(const Rows& g, uint64_t row, uint32_t ub) {
+  return row * g.channels + min(ub * 16u, g.channels);
 }
 
 template <int KIND>
@@ -60,68 +47,90 @@ __device__ __forceinline__ constexpr uint32_t elem_size() {
 // The 16 elements of a unit as they lie in memory (channels behind the last one: zero).
 template <int KIND>
 struct Raw {
-  uint32_t w[4 * elem_size<KIND>()];
+  static constexpr int kWords = 4 * elem_size<KIND>();
+  uint32_t w[kWords];
 };
 template <int KIND>
-__device__ __forceinline__ void load_raw(const Rows& g, const uint8_t* x, uint64_t row, uint32_t ub,
-                                         Raw<KIND>& raw) {
-  constexpr uint32_t es = elem_size<KIND>();
-  const uint8_t* p = x + (row * g.channels + ub * 16u) * es;
-  const uint32_t c0 = ub * 16u;
-  const uint32_t left = c0 < g.channels ? min(16u, g.channels - c0) : 0u;
-  if (left == 16u && g.aligned == 32 && es >= 2u) {
-#pragma unroll
-    for (int i = 0; i < (int)(es / 2u); ++i) {
-      uint32_t v[8];
-      ld32(p + 32 * i, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) raw.w[8 * i + j] = v[j];
-    }
-  } else if (g.aligned != 0) {
-    // whole 16-byte pieces: rows that start on one end on one
-#pragma unroll
-    for (uint32_t i = 0; i < es; ++i) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (i * (16u / es) < left) v = ld16(p + 16u * i);
-      raw.w[4u * i] = v.x;
-      raw.w[4u * i + 1u] = v.y;
-      raw.w[4u * i + 2u] = v.z;
-      raw.w[4u * i + 3u] = v.w;
-    }
+__device__ __forceinline__ void load_flat(const uint8_t* p, Raw<KIND>& raw) {
+  if (KIND == SPCONVB_I8) {
+    const uint4 v = ld16(p);
+    raw.w[0] = v.x;
+    raw.w[1] = v.y;
+    raw.w[2] = v.z;
+    raw.w[3] = v.w;
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 4u * es; ++i) raw.w[i] = 0u;
-#pragma unroll
-    for (uint32_t i = 0; i < 16u; ++i) {
-      if (i < left) {
-        if (KIND == SPCONVB_F32) raw.w[i] = load_in_order((const uint32_t*)p + i);
-        else if (KIND == SPCONVB_F16)
-          raw.w[i / 2u] |= (uint32_t)load_in_order((const uint16_t*)p + i) << (16u * (i % 2u));
-        else
-          raw.w[i / 4u] |= ((uint32_t)load_in_order((const int8_t*)p + i) & 255u) << (8u * (i % 4u));
-      }
-    }
+    for (int i = 0; i < Raw<KIND>::kWords / 8; ++i) ld32(p + 32 * i, raw.w + 8 * i);
   }
 }
 template <int KIND>
-__device__ __forceinline__ float element(const Raw<KIND>& raw, int i, float in_scale) {
-  if (KIND == SPCONVB_F32) return __uint_as_float(raw.w[i]);
-  if (KIND == SPCONVB_F16)
-    return __half2float(__ushort_as_half((uint16_t)(raw.w[i / 2] >> (16 * (i % 2)))));
-  return __fmul_rn((float)(int8_t)(raw.w[i / 4] >> (8 * (i % 4))), in_scale);
+__device__ __forceinline__ void load_aligned(const uint8_t* p, uint32_t left, Raw<KIND>& raw) {
+#pragma unroll
+  for (int i = 0; i < (int)elem_size<KIND>(); ++i) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if ((int)left > i * 16 / (int)elem_size<KIND>()) v = ld16(p + 16 * i);
+    raw.w[4 * i] = v.x;
+    raw.w[4 * i + 1] = v.y;
+    raw.w[4 * i + 2] = v.z;
+    raw.w[4 * i + 3] = v.w;
+  }
+}
+// From `at` bytes into shared memory on: whole words, moved into place, and what does not exist cut off.
+template <int KIND>
+__device__ __forceinline__ void load_staged(const uint32_t* buf, uint32_t at, uint32_t left, Raw<KIND>& raw) {
+  const uint32_t sh = (at & 3u) * 8u;
+  const uint32_t* p = buf + (at >> 2);
+  uint32_t w[Raw<KIND>::kWords + 1];
+#pragma unroll
+  for (int i = 0; i <= Raw<KIND>::kWords; ++i) w[i] = p[i];
+  const uint32_t bytes = left * elem_size<KIND>();
+#pragma unroll
+  for (int i = 0; i < Raw<KIND>::kWords; ++i) {
+    const uint32_t v = __funnelshift_r(w[i], w[i + 1], sh);
+    raw.w[i] = bytes >= 4u * i + 4u ? v : (bytes <= 4u * i ? 0u : v & ((1u << (8u * (bytes - 4u * i))) - 1u));
+  }
 }
 
-template <int FMT, int KIND>
-__device__ __forceinline__ void store_unit(const Rows& g, uint64_t row, uint32_t ub, uint64_t u, const Raw<KIND>& raw,
-                                           float in_scale, float tensor_scale, uint8_t* codes,
-                                           uint8_t* scales, bool live) {
-  float x[16];
-  uint32_t amax = 0u;
+// Elements to fp32, and the bits of the largest magnitude (infinities and NaN are the largest).
+template <int KIND>
+__device__ __forceinline__ uint32_t elements(const Raw<KIND>& raw, float in_scale, float (&x)[16]) {
+  if (KIND == SPCONVB_F32) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = __uint_as_float(raw.w[i]);
+      m = max(m, raw.w[i] & 0x7fffffffu);
+    }
+    return m;
+  }
+  if (KIND == SPCONVB_F16) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __half22float2(*(const __half2*)&raw.w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+      m = __vmaxu2(m, raw.w[i] & 0x7fff7fffu);
+    }
+    m = max(m & 0xffffu, m >> 16);
+    return __float_as_uint(__half2float(__ushort_as_half((uint16_t)m)));
+  }
+  // int8: byte b goes into the mantissa of 2^23 + (b + 128); a conversion instruction has an eighth of the rate
+  float m = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    x[i] = element<KIND>(raw, i, in_scale);
-    amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
+    const uint32_t b = __byte_perm(raw.w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7650u | (uint32_t)(i % 4));
+    x[i] = __fmul_rn(__fadd_rn(__uint_as_float(b), -8388736.f), in_scale);
+    m = fmaxf(m, fabsf(x[i]));
   }
+  return __float_as_uint(m);
+}
+
+template <int FMT, int KIND, Way WAY>
+__device__ __forceinline__ void store_unit(const Rows& g, uint64_t u, uint64_t row, uint32_t ub, const Raw<KIND>& raw,
+                                           float in_scale, float tensor_scale, uint8_t* codes, uint8_t* scales, bool live) {
+  float x[16];
+  uint32_t amax = elements<KIND>(raw, in_scale, x);
   if (FMT == SPCONVB_MXFP4) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   if (!live) return;
   float s;
@@ -136,104 +145,221 @@ __device__ __forceinline__ void store_unit(const Rows& g, uint64_t row, uint32_t
     for (int i = 0; i < 8; ++i) q[i] = divide(d, x[8 * h + i]);
     c[h] = none ? 0u : codes8(q);
   }
-  uint8_t* co = g.flat ? codes + u * 8u : codes + row * g.cpitch + ub * 8u;
+  uint8_t* co = WAY == kFlat ? codes + u * 8u : codes + row * g.cpitch + ub * 8u;
   *(uint2*)co = make_uint2(c[0], c[1]);
   if (FMT == SPCONVB_NVFP4) {
-    scales[g.flat ? u : row * g.spitch + ub] = (uint8_t)byte;
+    scales[WAY == kFlat ? u : row * g.spitch + ub] = (uint8_t)byte;
   } else if (!(ub & 1u)) {
-    uint8_t* so = g.flat ? scales + (u >> 1) : scales + row * g.spitch + (ub >> 1);
+    uint8_t* so = WAY == kFlat ? scales + (u >> 1) : scales + row * g.spitch + (ub >> 1);
     *so = (uint8_t)byte;
     // the two bytes behind the last block of rows of an odd number of 64 channels
-    if (!g.flat && (g.upr & 4u) && ub + 2u == g.upr) so[1] = so[2] = 0;
+    if (WAY != kFlat && (g.upr & 4u) && ub + 2u == g.upr) so[1] = so[2] = 0;
   }
 }
 
-template <int FMT, int KIND>
-__global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const uint8_t* __restrict__ x, Rows g, float in_scale,
+// The contiguous piece of rows that units [u0, u1) cover: first element, and one past the last.
+__device__ __forceinline__ void piece_of(const Rows& g, uint64_t u0, uint64_t u1, uint64_t& e0, uint64_t& e1) {
+  uint64_t row;
+  uint32_t ub;
+  place(g, u0, row, ub);
+  e0 = element_at(g, row, ub);
+  place(g, u1 - 1u, row, ub);
+  e1 = element_at(g, row, ub) + present(g, ub);
+}
+
+template <int FMT, int KIND, Way WAY>
+__global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const uint8_t* __restrict__ x, const Rows g, float in_scale,
                                                                 float tensor_scale, const uint32_t* n_ptr, uint32_t cap,
                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  constexpr uint32_t es = elem_size<KIND>();
+  __shared__ uint4 buf[WAY == kStaged ? kThreads * es + 2 : 1];  // 16 bytes of slack at either end
   pdl_wait_and_trigger();
   const uint64_t units = (uint64_t)min(load_in_order(n_ptr), cap) * g.upr;
-  const uint64_t step = (uint64_t)gridDim.x * kThreads;
-  // the bound is the same for all lanes of a warp: they exchange magnitudes
-  for (uint64_t first = (uint64_t)blockIdx.x * kThreads + (threadIdx.x & ~31u); first < units; first += step) {
-    const uint64_t u = first + (threadIdx.x & 31u);
-    const bool live = u < units;
-    uint64_t row = 0;
-    uint32_t ub = 0;
-    if (live) {
-      if (g.flat) ub = (uint32_t)(u & 1u);
-      else place(g, u, row, ub);
-    }
-    Raw<KIND> raw;
-    if (g.flat && live) {
-      Rows one = g;
-      one.channels = 16u;
-      load_raw<KIND>(one, x, u, 0u, raw);
-    } else if (live) {
-      load_raw<KIND>(g, x, row, ub, raw);
-    } else {
+  // loops go by the block: the lanes of a warp exchange magnitudes
+  if (WAY == kFlat) {
+    constexpr uint64_t kBlock = kThreads * kAhead;
+    for (uint64_t u0 = (uint64_t)blockIdx.x * kBlock; u0 < units; u0 += (uint64_t)gridDim.x * kBlock) {
+      Raw<KIND> raw[kAhead];
 #pragma unroll
-      for (uint32_t i = 0; i < 4u * elem_size<KIND>(); ++i) raw.w[i] = 0u;
+      for (int i = 0; i < kAhead; ++i) {
+        const uint64_t u = u0 + i * kThreads + threadIdx.x;
+        if (u < units) {
+          load_flat<KIND>(x + u * (16u * es), raw[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < Raw<KIND>::kWords; ++j) raw[i].w[j] = 0u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const uint64_t u = u0 + i * kThreads + threadIdx.x;
+        store_unit<FMT, KIND, WAY>(g, u, 0u, (uint32_t)u & 1u, raw[i], in_scale, tensor_scale, codes, scales, u < units);
+      }
     }
-    store_unit<FMT, KIND>(g, row, ub, u, raw, in_scale, tensor_scale, codes, scales, live);
+  } else {
+    for (uint64_t u0 = (uint64_t)blockIdx.x * kThreads; u0 < units; u0 += (uint64_t)gridDim.x * kThreads) {
+      const uint64_t u = u0 + threadIdx.x;
+      const bool live = u < units;
+      uint64_t row = 0, e0 = 0, e1 = 0;
+      uint32_t ub = 0;
+      if (live) place(g, u, row, ub);
+      const uint32_t left = live ? present(g, ub) : 0u;
+      uint64_t from = 0;
+      if (WAY == kStaged) {
+        piece_of(g, u0, min(u0 + kThreads, units), e0, e1);
+        // 16-byte pieces from the last boundary before e0 on; at the ends of x only what lies inside
+        const uint64_t a0 = (uint64_t)(uintptr_t)x + e0 * es, a1 = (uint64_t)(uintptr_t)x + e1 * es;
+        from = a0 & ~15ull;
+        __syncthreads();  // the units before are read
+        for (uint64_t p = from + threadIdx.x * 16u; p < a1; p += kThreads * 16u) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (p >= a0 && p + 16u <= a1) {
+            v = ld16((const void*)(uintptr_t)p);
+          } else {
+            uint8_t* b = (uint8_t*)&v;
+#pragma unroll
+            for (uint32_t i = 0; i < 16u; i += es) {
+              if (p + i >= a0 && p + i < a1) {
+                if (es == 1u) b[i] = *(const volatile uint8_t*)(uintptr_t)(p + i);
+                else if (es == 2u) *(uint16_t*)(b + i) = *(const volatile uint16_t*)(uintptr_t)(p + i);
+                else *(uint32_t*)(b + i) = *(const volatile uint32_t*)(uintptr_t)(p + i);
+              }
+            }
+          }
+          buf[(p - from) >> 4] = v;
+        }
+        __syncthreads();
+      }
+      Raw<KIND> raw;
+#pragma unroll
+      for (int j = 0; j < Raw<KIND>::kWords; ++j) raw.w[j] = 0u;
+      if (left) {
+        const uint64_t at = element_at(g, row, ub) * es;
+        if (WAY == kStaged) load_staged<KIND>((const uint32_t*)buf, (uint32_t)((uint64_t)(uintptr_t)x + at - from), left, raw);
+        else load_aligned<KIND>(x + at, left, raw);
+      }
+      store_unit<FMT, KIND, WAY>(g, u, row, ub, raw, in_scale, tensor_scale, codes, scales, live);
+    }
   }
 }
 
+// What a unit's codes stand for, as it lies in memory.
 template <int FMT, int KIND>
+__device__ __forceinline__ void values_of(uint2 c, uint32_t byte, float tensor_scale, Raw<KIND>& v) {
+  const float s = scale_value(FMT, byte, tensor_scale);
+  uint32_t h[2][4];
+  values8(c.x, h[0]);
+  values8(c.y, h[1]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __half22float2(*(const __half2*)&h[i / 4][i % 4]);
+    const float a = __fmul_rn(f.x, s), b = __fmul_rn(f.y, s);
+    if (KIND == SPCONVB_F16) {
+      const __half2 p = __floats2half2_rn(a, b);
+      v.w[i] = *(const uint32_t*)&p;
+    } else {
+      v.w[2 * i] = __float_as_uint(a);
+      v.w[2 * i + 1] = __float_as_uint(b);
+    }
+  }
+}
+
+template <int FMT, int KIND, Way WAY>
 __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                                  Rows g, float tensor_scale, const uint32_t* n_ptr,
+                                                                  const Rows g, float tensor_scale, const uint32_t* n_ptr,
                                                                   uint32_t cap, uint8_t* __restrict__ out) {
+  constexpr uint32_t es = elem_size<KIND>();
+  __shared__ uint4 buf[WAY == kStaged ? kThreads * es + 2 : 1];
   pdl_wait_and_trigger();
   const uint64_t units = (uint64_t)min(load_in_order(n_ptr), cap) * g.upr;
-  const uint64_t step = (uint64_t)gridDim.x * kThreads;
-  constexpr uint32_t es = elem_size<KIND>();
-  for (uint64_t u = (uint64_t)blockIdx.x * kThreads + threadIdx.x; u < units; u += step) {
-    uint64_t row = 0;
-    uint32_t ub = 0;
-    place(g, u, row, ub);
-    if (ub * 16u >= g.channels) continue;
-    const uint32_t left = min(16u, g.channels - ub * 16u);
-    const uint2 c = ld8(codes + row * g.cpitch + ub * 8u);
-    const uint32_t byte =
-        (uint32_t)load_in_order((const int8_t*)scales + row * g.spitch + (FMT == SPCONVB_MXFP4 ? ub >> 1 : ub)) & 255u;
-    const float s = scale_value(FMT, byte, tensor_scale);
-    uint32_t h[2][4], v[4 * es];
-    values8(c.x, h[0]);
-    values8(c.y, h[1]);
+  if (WAY == kFlat) {
+    constexpr uint64_t kBlock = kThreads * kAhead;
+    for (uint64_t u0 = (uint64_t)blockIdx.x * kBlock; u0 < units; u0 += (uint64_t)gridDim.x * kBlock) {
+      uint2 c[kAhead];
+      uint32_t byte[kAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 f = __half22float2(*(const __half2*)&h[i / 4][i % 4]);
-      const float a = __fmul_rn(f.x, s), b = __fmul_rn(f.y, s);
-      if (KIND == SPCONVB_F16) {
-        const __half2 p = __floats2half2_rn(a, b);
-        v[i] = *(const uint32_t*)&p;
-      } else {
-        v[2 * i] = __float_as_uint(a);
-        v[2 * i + 1] = __float_as_uint(b);
+      for (int i = 0; i < kAhead; ++i) {
+        const uint64_t u = u0 + i * kThreads + threadIdx.x;
+        if (u < units) {
+          c[i] = ld8(codes + u * 8u);
+          byte[i] = (uint32_t)load_in_order((const int8_t*)scales + (FMT == SPCONVB_MXFP4 ? u >> 1 : u)) & 255u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const uint64_t u = u0 + i * kThreads + threadIdx.x;
+        if (u < units) {
+          Raw<KIND> v;
+          values_of<FMT, KIND>(c[i], byte[i], tensor_scale, v);
+#pragma unroll
+          for (int j = 0; j < Raw<KIND>::kWords / 8; ++j) st32(out + u * (16u * es) + 32 * j, v.w + 8 * j);
+        }
       }
     }
-    uint8_t* o = out + (row * g.channels + ub * 16u) * es;
-    if (left == 16u && g.aligned == 32) {
-#pragma unroll
-      for (uint32_t i = 0; i < es / 2u; ++i) {
-        uint32_t t[8];
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) t[j] = v[8u * i + j];
-        st32(o + 32u * i, t);
+  } else {
+    for (uint64_t u0 = (uint64_t)blockIdx.x * kThreads; u0 < units; u0 += (uint64_t)gridDim.x * kThreads) {
+      const uint64_t u = u0 + threadIdx.x;
+      uint64_t row = 0;
+      uint32_t ub = 0, left = 0;
+      if (u < units) {
+        place(g, u, row, ub);
+        left = present(g, ub);
       }
-    } else if (g.aligned != 0) {
+      Raw<KIND> v;
+      if (left) {
+        const uint2 c = ld8(codes + row * g.cpitch + ub * 8u);
+        const uint32_t byte =
+            (uint32_t)load_in_order((const int8_t*)scales + row * g.spitch + (FMT == SPCONVB_MXFP4 ? ub >> 1 : ub)) & 255u;
+        values_of<FMT, KIND>(c, byte, tensor_scale, v);
+      }
+      uint8_t* o = out + element_at(g, row, ub) * es;
+      if (WAY == kAligned) {
 #pragma unroll
-      for (uint32_t i = 0; i < es; ++i)
-        if (i * (16u / es) < left)
-          ((uint4*)o)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
+        for (int i = 0; i < (int)es; ++i)
+          if ((int)left > i * 16 / (int)es)
+            ((uint4*)o)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
+        continue;
+      }
+      uint64_t e0, e1;
+      piece_of(g, u0, min(u0 + kThreads, units), e0, e1);
+      const uint64_t a0 = (uint64_t)(uintptr_t)out + e0 * es, a1 = (uint64_t)(uintptr_t)out + e1 * es, from = a0 & ~15ull;
+      uint8_t* b = (uint8_t*)buf + ((uint64_t)(uintptr_t)o - from);
+      __syncthreads();  // the units before are written
+      if (es == 4u) {
 #pragma unroll
-      for (uint32_t i = 0; i < 16u; ++i)
-        if (i < left) {
-          if (KIND == SPCONVB_F32) ((uint32_t*)o)[i] = v[i];
-          else ((uint16_t*)o)[i] = (uint16_t)(v[i / 2u] >> (16u * (i % 2u)));
+        for (int i = 0; i < 16; ++i)
+          if (i < (int)left) ((uint32_t*)b)[i] = v.w[i % Raw<KIND>::kWords];
+      } else if (((uint64_t)(uintptr_t)b & 3u) == 0u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (2 * i + 1 < (int)left) ((uint32_t*)b)[i] = v.w[i];
+          else if (2 * i < (int)left) ((uint16_t*)b)[2 * i] = (uint16_t)v.w[i];
         }
+      } else {
+        // from the odd half on: one half, pairs across the words, one half
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i == 0 && left) *(uint16_t*)b = (uint16_t)v.w[0];
+          const uint32_t pair = __funnelshift_r(v.w[i], i < 7 ? v.w[i < 7 ? i + 1 : 7] : 0u, 16);
+          if (2 * i + 2 < (int)left) *(uint32_t*)(b + 4 * i + 2) = pair;
+          else if (2 * i + 1 < (int)left) *(uint16_t*)(b + 4 * i + 2) = (uint16_t)pair;
+        }
+      }
+      __syncthreads();
+      for (uint64_t p = from + threadIdx.x * 16u; p < a1; p += kThreads * 16u) {
+        const uint4* src = buf + ((p - from) >> 4);
+        if (p >= a0 && p + 16u <= a1) {
+          *(uint4*)(uintptr_t)p = *src;
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < 16u; i += es) {
+            if (p + i >= a0 && p + i < a1) {
+              if (es == 2u) *(uint16_t*)(uintptr_t)(p + i) = ((const uint16_t*)src)[i / 2u];
+              else *(uint32_t*)(uintptr_t)(p + i) = ((const uint32_t*)src)[i / 4u];
+            }
+          }
+        }
+      }
     }
   }
 }
@@ -245,14 +371,15 @@ Rows rows_of(int format, int channels, const void* p, uint32_t es) {
   g.upr_inv = ~0ull / g.upr + 1ull;  // upr is at least 4
   g.cpitch = code_pitch(g.channels);
   g.spitch = scale_pitch(format, g.channels);
-  g.flat = g.channels % (format == SPCONVB_MXFP4 ? 128u : 64u) == 0u;
-  const uint64_t bits = (uint64_t)(uintptr_t)p | (uint64_t)g.channels * es;
-  g.aligned = bits % 32u == 0u ? 32 : (bits % 16u == 0u ? 16 : 0);
+  const uint64_t row = (uint64_t)g.channels * es;
+  if (((uint64_t)(uintptr_t)p | row) % 16u != 0u) g.way = kStaged;
+  else if (g.channels % (format == SPCONVB_MXFP4 ? 128u : 64u) == 0u && (uintptr_t)p % 32u == 0u) g.way = kFlat;
+  else g.way = kAligned;
   return g;
 }
 int blocks_of(const Rows& g, uint32_t rows) {
-  const uint64_t b = ((uint64_t)rows * g.upr + kThreads - 1) / kThreads;
-  return (int)(b < (uint64_t)kSmCount * 32 ? b : (uint64_t)kSmCount * 32);
+  const uint64_t per = kThreads * (g.way == kFlat ? kAhead : 1), b = ((uint64_t)rows * g.upr + per - 1) / per;
+  return (int)(b < (uint64_t)kSmCount * 16 ? b : (uint64_t)kSmCount * 16);
 }
 
 // One thread a 16-byte segment of the image or a word of scales.
@@ -278,7 +405,7 @@ __global__ void fp4_pack_kernel(int format, uint32_t cin, uint32_t cout, uint32_
       w = t / 128u;
       r = t % 128u;
     }
-    const uint32_t ch = cout <= 64u ? r % 64u : blk * 128u + r;
+    const uint32_t ch = blk * 128u + r;
     const uint64_t k = (uint64_t)j * kChunkK + (code ? seg * 32u : w * (kChunkK / words));
     const bool live = ch < cout && k < ktotal;
     const uint32_t tap = live ? (uint32_t)(k / cp) : 0u, c = live ? (uint32_t)(k % cp) : 0u;
@@ -295,23 +422,47 @@ __global__ void fp4_pack_kernel(int format, uint32_t cin, uint32_t cout, uint32_
   }
 }
 
-template <int FMT>
-cudaError_t quantize_kind(int kind, int blocks, cudaStream_t st, const uint8_t* x, const Rows& g, float in_scale, float ts,
-                          const uint32_t* n, uint32_t cap, uint8_t* codes, uint8_t* scales) {
-  const dim3 b(blocks), t(kThreads);
-  if (kind == SPCONVB_F16)
-    return launch_pdl(fp4_quantize_kernel<FMT, SPCONVB_F16>, b, t, 0, st, x, g, in_scale, ts, n, cap, codes, scales);
-  if (kind == SPCONVB_F32)
-    return launch_pdl(fp4_quantize_kernel<FMT, SPCONVB_F32>, b, t, 0, st, x, g, in_scale, ts, n, cap, codes, scales);
-  return launch_pdl(fp4_quantize_kernel<FMT, SPCONVB_I8>, b, t, 0, st, x, g, in_scale, ts, n, cap, codes, scales);
+struct Call {
+  int blocks;
+  cudaStream_t st;
+  Rows g;
+  float in_scale, tensor_scale;
+  const uint32_t* n;
+  uint32_t cap;
+};
+template <int FMT, int KIND>
+cudaError_t quantize_way(const Call& k, const uint8_t* x, uint8_t* codes, uint8_t* scales) {
+  const dim3 b(k.blocks), t(kThreads);
+  if (k.g.way == kFlat)
+    return launch_pdl(fp4_quantize_kernel<FMT, KIND, kFlat>, b, t, 0, k.st, x, k.g, k.in_scale, k.tensor_scale, k.n, k.cap,
+                      codes, scales);
+  if (k.g.way == kAligned)
+    return launch_pdl(fp4_quantize_kernel<FMT, KIND, kAligned>, b, t, 0, k.st, x, k.g, k.in_scale, k.tensor_scale, k.n, k.cap,
+                      codes, scales);
+  return launch_pdl(fp4_quantize_kernel<FMT, KIND, kStaged>, b, t, 0, k.st, x, k.g, k.in_scale, k.tensor_scale, k.n, k.cap, codes,
+                    scales);
 }
 template <int FMT>
-cudaError_t dequantize_kind(int kind, int blocks, cudaStream_t st, const uint8_t* codes, const uint8_t* scales, const Rows& g,
-                            float ts, const uint32_t* n, uint32_t cap, uint8_t* out) {
-  const dim3 b(blocks), t(kThreads);
-  if (kind == SPCONVB_F16)
-    return launch_pdl(fp4_dequantize_kernel<FMT, SPCONVB_F16>, b, t, 0, st, codes, scales, g, ts, n, cap, out);
-  return launch_pdl(fp4_dequantize_kernel<FMT, SPCONVB_F32>, b, t, 0, st, codes, scales, g, ts, n, cap, out);
+cudaError_t quantize_kind(int kind, const Call& k, const uint8_t* x, uint8_t* codes, uint8_t* scales) {
+  if (kind == SPCONVB_F16) return quantize_way<FMT, SPCONVB_F16>(k, x, codes, scales);
+  return kind == SPCONVB_F32 ? quantize_way<FMT, SPCONVB_F32>(k, x, codes, scales)
+                             : quantize_way<FMT, SPCONVB_I8>(k, x, codes, scales);
+}
+template <int FMT, int KIND>
+cudaError_t dequantize_way(const Call& k, const uint8_t* codes, const uint8_t* scales, uint8_t* out) {
+  const dim3 b(k.blocks), t(kThreads);
+  if (k.g.way == kFlat)
+    return launch_pdl(fp4_dequantize_kernel<FMT, KIND, kFlat>, b, t, 0, k.st, codes, scales, k.g, k.tensor_scale, k.n, k.cap, out);
+  if (k.g.way == kAligned)
+    return launch_pdl(fp4_dequantize_kernel<FMT, KIND, kAligned>, b, t, 0, k.st, codes, scales, k.g, k.tensor_scale, k.n, k.cap,
+                      out);
+  return launch_pdl(fp4_dequantize_kernel<FMT, KIND, kStaged>, b, t, 0, k.st, codes, scales, k.g, k.tensor_scale, k.n, k.cap, out);
+}
+
+template <int FMT>
+cudaError_t dequantize_kind(int kind, const Call& k, const uint8_t* codes, const uint8_t* scales, uint8_t* out) {
+  return kind == SPCONVB_F16 ? dequantize_way<FMT, SPCONVB_F16>(k, codes, scales, out)
+                             : dequantize_way<FMT, SPCONVB_F32>(k, codes, scales, out);
 }
 
 bool aligned16(const void* a, const void* b = nullptr, const void* c = nullptr) {
@@ -350,14 +501,12 @@ int spconvb_fp4_quantize(int32_t format, const void* x, int32_t kind, float in_s
   if (kind != SPCONVB_F16 && kind != SPCONVB_F32 && kind != SPCONVB_I8) return SPCONVB_E_ARG;
   const uint32_t es = kind == SPCONVB_F32 ? 4u : (kind == SPCONVB_I8 ? 1u : 2u);
   if (!aligned16(codes, scales) || (uintptr_t)x % es != 0u) return SPCONVB_E_ARG;
+  if (kind == SPCONVB_I8 && !(in_scale > -3.4e38f && in_scale < 3.4e38f)) return SPCONVB_E_ARG;
   const Rows g = rows_of(format, channels, x, es);
-  const int blocks = blocks_of(g, launch_rows);
-  if (format == SPCONVB_MXFP4)
-    SPCONVB_CUDA_TRY(quantize_kind<SPCONVB_MXFP4>(kind, blocks, (cudaStream_t)stream, (const uint8_t*)x, g, in_scale,
-                                                  tensor_scale, n_ptr, launch_rows, (uint8_t*)codes, (uint8_t*)scales));
-  else
-    SPCONVB_CUDA_TRY(quantize_kind<SPCONVB_NVFP4>(kind, blocks, (cudaStream_t)stream, (const uint8_t*)x, g, in_scale,
-                                                  tensor_scale, n_ptr, launch_rows, (uint8_t*)codes, (uint8_t*)scales));
+  const Call k{blocks_of(g, launch_rows), (cudaStream_t)stream, g, in_scale, tensor_scale, n_ptr, launch_rows};
+  SPCONVB_CUDA_TRY(format == SPCONVB_MXFP4
+                       ? quantize_kind<SPCONVB_MXFP4>(kind, k, (const uint8_t*)x, (uint8_t*)codes, (uint8_t*)scales)
+                       : quantize_kind<SPCONVB_NVFP4>(kind, k, (const uint8_t*)x, (uint8_t*)codes, (uint8_t*)scales));
   return SPCONVB_OK;
 }
 
@@ -370,13 +519,10 @@ int spconvb_fp4_dequantize(int32_t format, const void* codes, const void* scales
   const uint32_t es = out_kind == SPCONVB_F32 ? 4u : 2u;
   if (!aligned16(codes, scales) || (uintptr_t)out % es != 0u) return SPCONVB_E_ARG;
   const Rows g = rows_of(format, channels, out, es);
-  const int blocks = blocks_of(g, launch_rows);
-  if (format == SPCONVB_MXFP4)
-    SPCONVB_CUDA_TRY(dequantize_kind<SPCONVB_MXFP4>(out_kind, blocks, (cudaStream_t)stream, (const uint8_t*)codes,
-                                                    (const uint8_t*)scales, g, tensor_scale, n_ptr, launch_rows, (uint8_t*)out));
-  else
-    SPCONVB_CUDA_TRY(dequantize_kind<SPCONVB_NVFP4>(out_kind, blocks, (cudaStream_t)stream, (const uint8_t*)codes,
-                                                    (const uint8_t*)scales, g, tensor_scale, n_ptr, launch_rows, (uint8_t*)out));
+  const Call k{blocks_of(g, launch_rows), (cudaStream_t)stream, g, 1.f, tensor_scale, n_ptr, launch_rows};
+  const uint8_t *c = (const uint8_t*)codes, *s = (const uint8_t*)scales;
+  SPCONVB_CUDA_TRY(format == SPCONVB_MXFP4 ? dequantize_kind<SPCONVB_MXFP4>(out_kind, k, c, s, (uint8_t*)out)
+                                           : dequantize_kind<SPCONVB_NVFP4>(out_kind, k, c, s, (uint8_t*)out));
   return SPCONVB_OK;
 }
 

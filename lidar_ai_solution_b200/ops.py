@@ -278,90 +278,130 @@ def voxelize(points, params, status=None):
 
 # ------------------------------------------------------------- 4-bit floating point
 _FP4_KIND = {torch.float16: F16, torch.float32: F32, torch.int8: I8}
+_FP4_MAX_CHANNELS = 65536
+
+
+def _fp4_pitches(fmt, channels):
+    """Bytes of a row's codes and scales, as spconvb_fp4_code_pitch() and spconvb_fp4_scale_pitch()."""
+    if fmt not in (MXFP4, NVFP4) or not 1 <= channels <= _FP4_MAX_CHANNELS:
+        raise ValueError("no 4-bit rows of %s channels in format %s" % (channels, fmt))
+    k = (channels + 63) // 64
+    return 32 * k, 4 * ((k + 1) // 2 if fmt == MXFP4 else k)
+
+
+def _fp4_device(t, count, *others):
+    """The index of a tensor's device, which has to be the current one (the library enqueues there) and that of the row
+    count (int32) and of the others."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError("a tensor on %s where the current CUDA device's is wanted" % t.device)
+    if count.dtype != torch.int32 or count.get_device() != dev or not count.numel():
+        raise ValueError("a row count is an int32 on the rows' device (device_count)")
+    for o in others:
+        if o is not None and o.get_device() != dev:
+            raise ValueError("tensors of different devices")
+    return dev
+
+
+def _fp4_stream(dev):
+    return _stream() if _raw_stream is None else _raw_stream(dev)
+
+
+def _fp4_tensor(t, dtype, rows, width, what):
+    if t.dtype != dtype or t.dim() != 2 or not t.is_contiguous() or t.shape[0] != rows or t.shape[1] != width:
+        raise ValueError("%s: a contiguous %s [%d, %d] is wanted" % (what, dtype, rows, width))
 
 
 class Fp4Rows:
     """Rows in 4 bits: ``codes`` uint8 [rows, cpad / 2], ``scales`` uint8 [rows, pitch], the format
     (``MXFP4`` or ``NVFP4``), the channels, and the tensor scale (1 for ``MXFP4``)."""
 
-    __slots__ = ("codes", "scales", "channels", "fmt", "tensor_scale")
+    __slots__ = ("rows", "channels", "fmt", "tensor_scale", "device_index", "codes_ptr", "scales_ptr", "_hold",
+                 "_pitches")
 
     def __init__(self, codes, scales, channels, fmt, tensor_scale=1.0):
-        lib = cabi.lib()
-        cp, sp = lib.spconvb_fp4_code_pitch(channels), lib.spconvb_fp4_scale_pitch(fmt, channels)
-        if cp == 0 or sp == 0:
-            raise ValueError("no 4-bit rows of %d channels in format %s" % (channels, fmt))
-        for t, pitch in ((codes, cp), (scales, sp)):
-            if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != pitch or not t.is_contiguous():
-                raise ValueError("codes and scales are contiguous uint8 [rows, %d] and [rows, %d]" % (cp, sp))
-        if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
-            raise ValueError("codes and scales of different rows or devices")
-        self.codes, self.scales, self.channels = codes, scales, int(channels)
-        self.fmt, self.tensor_scale = fmt, float(tensor_scale)
+        cp, sp = self._pitches = _fp4_pitches(fmt, channels)
+        self.rows = codes.shape[0] if codes.dim() else -1
+        _fp4_tensor(codes, torch.uint8, self.rows, cp, "codes")
+        _fp4_tensor(scales, torch.uint8, self.rows, sp, "scales")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales of different devices")
+        self._hold = codes, scales
+        self._set(channels, fmt, tensor_scale, codes.get_device(), codes.data_ptr(), scales.data_ptr())
+
+    def _set(self, channels, fmt, tensor_scale, dev, codes_ptr, scales_ptr):
+        self.channels, self.fmt, self.tensor_scale = channels, fmt, float(tensor_scale)
+        self.device_index, self.codes_ptr, self.scales_ptr = dev, codes_ptr, scales_ptr
 
     @classmethod
     def empty(cls, rows, channels, fmt, tensor_scale=1.0, device="cuda"):
-        lib = cabi.lib()
-        return cls(torch.empty((rows, lib.spconvb_fp4_code_pitch(channels)), dtype=torch.uint8, device=device),
-                   torch.empty((rows, lib.spconvb_fp4_scale_pitch(fmt, channels)), dtype=torch.uint8, device=device),
-                   channels, fmt, tensor_scale)
+        """Rows with uninitialised contents."""
+        return cls._beside(torch.empty(0, dtype=torch.uint8, device=device), rows, channels, fmt, tensor_scale)
 
+    @classmethod
+    def _beside(cls, t, rows, channels, fmt, tensor_scale):
+        """Uninitialised rows on t's device: one buffer, of which ``codes`` and ``scales`` are made when asked for."""
+        q = cls.__new__(cls)
+        cp, sp = q._pitches = _fp4_pitches(fmt, channels)
+        q.rows = rows
+        q._hold = buf = t.new_empty(rows * (cp + sp), dtype=torch.uint8)
+        at = buf.data_ptr()
+        q._set(channels, fmt, tensor_scale, buf.get_device(), at, at + rows * cp)
+        return q
 
-def _on_current_device(*tensors):
-    """The library enqueues on the current device's stream: what it is given has to lie there."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != here):
-            raise ValueError("a tensor on %s where the current CUDA device's is wanted" % t.device)
+    @property
+    def codes(self):
+        cp = self._pitches[0]
+        return self._hold[0] if type(self._hold) is tuple else self._hold[:self.rows * cp].view(self.rows, cp)
 
+    @property
+    def scales(self):
+        cp, sp = self._pitches
+        return self._hold[1] if type(self._hold) is tuple else self._hold[self.rows * cp:].view(self.rows, sp)
 
-def _count_of(n_ptr):
-    if n_ptr.dtype != torch.int32 or n_ptr.numel() < 1:
-        raise ValueError("a row count is an int32 in device memory (device_count)")
+    def _buffer(self):
+        return self._hold[0] if type(self._hold) is tuple else self._hold
 
-
-def _rows_of(t, what, dtypes, rows=None, channels=None, device=None):
-    if t.dtype not in dtypes or t.dim() != 2 or not t.is_contiguous():
-        raise ValueError("%s: a contiguous [rows, channels] tensor of %s" % (what, "/".join(map(str, dtypes))))
-    if rows is not None and t.shape != (rows, channels):
-        raise ValueError("%s: %s where [%d, %d] is wanted" % (what, tuple(t.shape), rows, channels))
-    if device is not None and t.device != device:
-        raise ValueError("%s: on %s and not on %s" % (what, t.device, device))
+    def _check(self, rows, channels, fmt, tensor_scale, dev):
+        if (self.rows, self.channels, self.fmt, self.tensor_scale, self.device_index) != (
+                rows, channels, fmt, float(tensor_scale), dev):
+            raise ValueError("out: rows of another shape, format, scale or device")
+        return self
 
 
 def fp4_quantize(x, n_ptr, fmt, tensor_scale=1.0, in_scale=1.0, out=None):
     """Rows [rows, channels] fp16, fp32 or int8 (times ``in_scale``) to :class:`Fp4Rows`; ``out``:
     rows to write into, whose format and tensor scale have to be the same."""
-    _rows_of(x, "x", tuple(_FP4_KIND))
-    _count_of(n_ptr)
-    _on_current_device(x, n_ptr)
+    kind = _FP4_KIND.get(x.dtype)
+    if kind is None or x.dim() != 2 or not x.is_contiguous():
+        raise ValueError("x: a contiguous [rows, channels] tensor of fp16, fp32 or int8")
+    dev = _fp4_device(x, n_ptr)
     rows, ch = x.shape
     if out is None:
-        out = Fp4Rows.empty(rows, ch, fmt, tensor_scale, x.device)
-    elif (out.codes.shape[0], out.channels, out.fmt, out.tensor_scale, out.codes.device) != (
-            rows, ch, fmt, float(tensor_scale), x.device):
-        raise ValueError("out: rows of another shape, format, scale or device")
+        out = Fp4Rows._beside(x, rows, ch, fmt, tensor_scale)
+    else:
+        out._check(rows, ch, fmt, tensor_scale, dev)
     if rows:
-        cabi.check(cabi.lib().spconvb_fp4_quantize(fmt, _ptr(x), _FP4_KIND[x.dtype], in_scale, ch,
-                                                   tensor_scale, _ptr(n_ptr), rows, _ptr(out.codes),
-                                                   _ptr(out.scales), _stream()), "fp4_quantize")
+        cabi.check(cabi.lib().spconvb_fp4_quantize(
+            fmt, x.data_ptr(), kind, in_scale, ch, tensor_scale, n_ptr.data_ptr(), rows,
+            out.codes_ptr, out.scales_ptr, _fp4_stream(dev)), "fp4_quantize")
     return out
 
 
 def fp4_dequantize(q, n_ptr, out_kind=F16, out=None):
     """What the codes and scales of ``q`` stand for: [rows, channels] fp16 or fp32."""
-    _count_of(n_ptr)
-    _on_current_device(q.codes, n_ptr)
-    rows = q.codes.shape[0]
-    dt = torch.float32 if out_kind == F32 else torch.float16
+    rows, dt = q.rows, torch.float32 if out_kind == F32 else torch.float16
     if out is None:
-        out = torch.empty((rows, q.channels), dtype=dt, device=q.codes.device)
+        out = q._buffer().new_empty((rows, q.channels), dtype=dt)
     else:
-        _rows_of(out, "out", (dt,), rows, q.channels, q.codes.device)
+        _fp4_tensor(out, dt, rows, q.channels, "out")
+    dev = _fp4_device(out, n_ptr)
+    if q.device_index != dev:
+        raise ValueError("tensors of different devices")
     if rows:
-        cabi.check(cabi.lib().spconvb_fp4_dequantize(q.fmt, _ptr(q.codes), _ptr(q.scales), q.channels,
-                                                     q.tensor_scale, out_kind, _ptr(n_ptr), rows,
-                                                     _ptr(out), _stream()), "fp4_dequantize")
+        cabi.check(cabi.lib().spconvb_fp4_dequantize(
+            q.fmt, q.codes_ptr, q.scales_ptr, q.channels, q.tensor_scale, out_kind,
+            n_ptr.data_ptr(), rows, out.data_ptr(), _fp4_stream(dev)), "fp4_dequantize")
     return out
 
 
@@ -374,7 +414,7 @@ class Fp4Weights:
     def __init__(self, w, fmt, tensor_scale=1.0, bias=None, rows=None, device="cuda"):
         lib = cabi.lib()
         if rows is None:
-            w = torch.as_tensor(w).to(device)
+            w = torch.as_tensor(w)
             if w.dtype not in (torch.float16, torch.float32):
                 raise ValueError("weights in fp16 or fp32")
             shape = w.shape
@@ -391,55 +431,59 @@ class Fp4Weights:
             raise ValueError("no 4-bit weights [%d, %d, %d] in format %s" % (self.cout, self.kvol, self.cin, fmt))
         flat = self.cout * self.kvol
         if rows is None:
-            n = device_count(flat, w.device)
-            rows = fp4_quantize(w.reshape(flat, self.cin).contiguous(), n, fmt, tensor_scale)
-        elif (rows.codes.shape[0], rows.channels, rows.fmt, rows.tensor_scale) != (
-                flat, self.cin, fmt, self.tensor_scale):
-            raise ValueError("rows: of another shape, format or scale")
-        self.packed = torch.empty(nbytes, dtype=torch.uint8, device=rows.codes.device)
-        cabi.check(lib.spconvb_fp4_pack_weights(fmt, self.cin, self.cout, self.kvol, _ptr(rows.codes),
-                                                _ptr(rows.scales), _ptr(self.packed), _stream()), "fp4_pack")
+            w = w.to(device).reshape(flat, self.cin).contiguous()
+            rows = fp4_quantize(w, device_count(flat, w.device), fmt, tensor_scale)
+        else:
+            rows._check(flat, self.cin, fmt, tensor_scale, torch.cuda.current_device())
+        self.packed = rows._buffer().new_empty(nbytes, dtype=torch.uint8)
+        self.device_index = rows.device_index
+        cabi.check(lib.spconvb_fp4_pack_weights(fmt, self.cin, self.cout, self.kvol, rows.codes_ptr, rows.scales_ptr,
+                                                _ptr(self.packed), _stream()), "fp4_pack")
         self.bias = None
         if bias is not None:
-            self.bias = torch.as_tensor(bias).to(rows.codes.device, torch.float32).contiguous()
+            self.bias = torch.as_tensor(bias).to(self.packed.device, torch.float32).contiguous()
             if self.bias.shape != (self.cout,):
                 raise ValueError("bias is [cout]")
+        # what every call's parameters start from
+        self._params = cabi.Fp4Params(fmt, self.cin, self.cout, self.kvol, 1.0)
 
 
 def _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out):
-    if (q.fmt, q.channels) != (wts.fmt, wts.cin) or q.codes.device != wts.packed.device:
+    """Parameters, output, and the address of its codes or fp16 rows."""
+    if q.fmt != wts.fmt or q.channels != wts.cin or q.device_index != wts.device_index:
         raise ValueError("rows and weights of different formats, channels or devices")
-    p = cabi.Fp4Params()
-    p.format, p.cin, p.cout, p.kvol = q.fmt, wts.cin, wts.cout, wts.kvol
-    p.alpha, p.act = q.tensor_scale * wts.tensor_scale, act
+    p = cabi.Fp4Params.from_buffer_copy(wts._params)
+    p.alpha = q.tensor_scale * wts.tensor_scale
+    if act:
+        p.act = act
     if out_fmt is None:
         if out is None:
-            out = torch.empty((rows, wts.cout), dtype=torch.float16, device=q.codes.device)
+            out = wts.packed.new_empty((rows, wts.cout), dtype=torch.float16)
         else:
-            _rows_of(out, "out", (torch.float16,), rows, wts.cout, q.codes.device)
-        return p, out, out
+            _fp4_tensor(out, torch.float16, rows, wts.cout, "out")
+            if out.get_device() != wts.device_index:
+                raise ValueError("tensors of different devices")
+        return p, out, out.data_ptr()
     if out is None:
-        out = Fp4Rows.empty(rows, wts.cout, out_fmt, out_tensor_scale, q.codes.device)
-    elif (out.codes.shape[0], out.channels, out.fmt, out.tensor_scale, out.codes.device) != (
-            rows, wts.cout, out_fmt, float(out_tensor_scale), q.codes.device):
-        raise ValueError("out: rows of another shape, format, scale or device")
-    p.out_fp4, p.out_format, p.out_tensor_scale = 1, out_fmt, out_tensor_scale
-    p.out_scales = out.scales.data_ptr()
-    return p, out, out.codes
+        out = Fp4Rows._beside(wts.packed, rows, wts.cout, out_fmt, out_tensor_scale)
+    else:
+        out._check(rows, wts.cout, out_fmt, out_tensor_scale, wts.device_index)
+    p.out_fp4, p.out_format, p.out_tensor_scale, p.out_scales = 1, out_fmt, out_tensor_scale, out.scales_ptr
+    return p, out, out.codes_ptr
 
 
 def fp4_linear(q, n_ptr, wts: Fp4Weights, act=ACT_NONE, out_fmt=None, out_tensor_scale=1.0, out=None,
                status=None, wait_test=0):
     """act(x W^T + bias) of 4-bit rows: fp16 [rows, cout], or :class:`Fp4Rows` of ``out_fmt``."""
-    _count_of(n_ptr)
-    _on_current_device(q.codes, n_ptr, status)
-    rows = q.codes.shape[0]
-    p, out, buf = _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out)
-    p.wait_test = wait_test
+    rows = q.rows
+    dev = _fp4_device(wts.packed, n_ptr, status)
+    p, out, at = _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out)
+    if wait_test:
+        p.wait_test = wait_test
     if rows:
-        cabi.check(cabi.lib().spconvb_fp4_linear(C.byref(p), _ptr(q.codes), _ptr(q.scales), _ptr(n_ptr), rows,
-                                                 _ptr(wts.packed), _ptr(wts.bias), _ptr(buf), _ptr(status),
-                                                 _stream()), "fp4_linear")
+        cabi.check(cabi.lib().spconvb_fp4_linear(
+            C.byref(p), q.codes_ptr, q.scales_ptr, n_ptr.data_ptr(), rows, wts.packed.data_ptr(),
+            _ptr(wts.bias), at, _ptr(status), _fp4_stream(dev)), "fp4_linear")
     return out
 
 
@@ -449,16 +493,16 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     activation, fp16 residual [cap, cout]; fp16 [cap, cout] or :class:`Fp4Rows` of ``out_fmt``."""
     if m.dtype != torch.int32 or m.dim() != 2 or m.shape[0] != wts.kvol or not m.is_contiguous():
         raise ValueError("m is a contiguous int32 [kvol, cap]")
-    _count_of(n_out_ptr)
-    _on_current_device(q.codes, m, n_out_ptr, status)
     cap = m.shape[1]
-    p, out, buf = _fp4_product(q, wts, act, cap, out_fmt, out_tensor_scale, out)
+    dev = _fp4_device(wts.packed, n_out_ptr, m, res, status)
+    p, out, at = _fp4_product(q, wts, act, cap, out_fmt, out_tensor_scale, out)
     if res is not None:
-        _rows_of(res, "res", (torch.float16,), cap, wts.cout, q.codes.device)
-        p.res, p.res_relu = res.data_ptr(), int(res_relu)
-    p.wait_test = wait_test
+        _fp4_tensor(res, torch.float16, cap, wts.cout, "res")
+        p.res, p.res_relu = res.data_ptr(), res_relu
+    if wait_test:
+        p.wait_test = wait_test
     if cap:
-        cabi.check(cabi.lib().spconvb_fp4_conv(C.byref(p), _ptr(q.codes), _ptr(q.scales), _ptr(m), cap,
-                                               _ptr(n_out_ptr), launch_rows, _ptr(wts.packed), _ptr(wts.bias),
-                                               _ptr(buf), _ptr(status), _stream()), "fp4_conv")
+        cabi.check(cabi.lib().spconvb_fp4_conv(
+            C.byref(p), q.codes_ptr, q.scales_ptr, m.data_ptr(), cap, n_out_ptr.data_ptr(), launch_rows,
+            wts.packed.data_ptr(), _ptr(wts.bias), at, _ptr(status), _fp4_stream(dev)), "fp4_conv")
     return out
