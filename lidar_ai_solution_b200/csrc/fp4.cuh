@@ -65,17 +65,37 @@ __device__ __forceinline__ uint32_t scale_mx(uint32_t amax_bits, float& s) {
   s = byte == 0u ? 5.8774717541114375e-39f : __uint_as_float(byte << 23);  // 2^-127 is a subnormal number
   return byte;
 }
-__device__ __forceinline__ uint32_t scale_nv(uint32_t amax_bits, float tensor_scale, float& s) {
+// A quotient x / d, correctly rounded, from the product with the reciprocal r of d and one correction by the exact remainder
+// (Markstein 1990): where x is the product of d and a short number, as on the border between two codes, the corrected quotient is
+// that number.  d between 2^-90 and 2^90 and |x / d| below 2^100, so that nothing overflows and no remainder loses bits.
+__device__ __forceinline__ float quotient(float x, float d, float r) {
+  const float q = __fmul_rn(x, r);
+  return __fmaf_rn(__fmaf_rn(-q, d, x), r, q);
+}
+__host__ __device__ inline bool in_range(float d) { return d > 8.1e-28f && d < 1.2e27f; }
+
+// What a tensor scale g gives to all blocks: 6 g and its reciprocal, 0 where that is out of range.
+struct TensorScale {
+  float g, six, inv_six;
+};
+inline TensorScale tensor_scale_of(float g) {
+  TensorScale t{g, 6.f * g, 0.f};
+  if (in_range(t.six)) t.inv_six = 1.f / t.six;
+  return t;
+}
+__device__ __forceinline__ uint32_t scale_nv(uint32_t amax_bits, const TensorScale& t, float& s) {
+  const float amax = __uint_as_float(amax_bits);
   if (amax_bits >= 0x7f800000u) {
     s = 0.f;
     return 0x7fu;
   }
-  const float t = __fdiv_rn(__uint_as_float(amax_bits), __fmul_rn(6.f, tensor_scale));
+  const bool fast = t.inv_six != 0.f && amax < 1e30f;
+  const float ratio = fast ? quotient(amax, t.six, t.inv_six) : __fdiv_rn(amax, t.six);
   uint16_t two;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(t));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(ratio));
   uint32_t half2;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(half2) : "h"(two));
-  s = __fmul_rn(__half2float(__ushort_as_half((uint16_t)half2)), tensor_scale);
+  s = __fmul_rn(__half2float(__ushort_as_half((uint16_t)half2)), t.g);
   return two & 0xffu;
 }
 // S of a stored byte.
@@ -113,34 +133,42 @@ __device__ __forceinline__ void values8(uint32_t codes, uint32_t (&h)[4]) {
       : "r"(codes));
 }
 
-// x / S of a block.  MXFP4: times 2^-e, exact.  NVFP4: the correctly rounded quotient, so that a value on the border
-// between two codes is found there: reciprocal, product, and one correction with the exact remainder (Markstein 1990), where
-// nothing in it can overflow or lose bits; else the division itself.
-struct Divider {
-  float s, r;
-  bool exact_scale, plain;
-};
-__device__ __forceinline__ Divider divider(int format, float s, uint32_t amax_bits) {
-  Divider d;
-  d.s = s;
-  d.exact_scale = format == SPCONVB_MXFP4;
-  if (d.exact_scale) {
-    // 2^-e; e = -127 .. 125, so its exponent field lies in 2 .. 254
-    d.r = s < 1.1754944e-38f ? 1.7014118346046923e38f : __uint_as_float((254u << 23) - __float_as_uint(s));
-    d.plain = true;
-  } else {
-    d.r = __frcp_rn(s);
-    // (a block without codes takes the short way too: what it gives is not used)
-    d.plain = s == 0.f || (s > 1e-27f && s < 1e27f && __uint_as_float(amax_bits) < 1e30f &&
-                           __uint_as_float(amax_bits) * d.r < 1e30f);
+// N values of a block (a multiple of 8) to codes.  `s` and `amax_bits` are the block's.
+template <int N>
+__device__ __forceinline__ void codes_of(bool mx, const float* x, float s, uint32_t amax_bits, uint32_t* c) {
+  if (amax_bits >= 0x7f800000u || s == 0.f) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) c[i] = 0u;
+    return;
   }
-  return d;
-}
-__device__ __forceinline__ float divide(const Divider& d, float x) {
-  if (d.exact_scale) return __fmul_rn(x, d.r);
-  if (!d.plain) return __fdiv_rn(x, d.s);
-  const float q = __fmul_rn(x, d.r);
-  return __fmaf_rn(__fmaf_rn(-q, d.s, x), d.r, q);
+  const float amax = __uint_as_float(amax_bits);
+  float r;
+  bool fast;
+  if (mx) {
+    // times 2^-e, exact; e = -127 .. 125, so its exponent field lies in 2 .. 254
+    r = s < 1.1754944e-38f ? 1.7014118346046923e38f : __uint_as_float((254u << 23) - __float_as_uint(s));
+    fast = true;
+  } else {
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+    fast = in_range(s) && amax < 1e30f && amax * r < 1e30f;
+  }
+  if (fast) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) {
+      float q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = mx ? __fmul_rn(x[8 * i + j], r) : quotient(x[8 * i + j], s, r);
+      c[i] = codes8(q);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) {
+      float q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(x[8 * i + j], s);
+      c[i] = codes8(q);
+    }
+  }
 }
 
 }  // namespace fp4

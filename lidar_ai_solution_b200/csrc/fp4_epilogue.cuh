@@ -12,7 +12,8 @@ struct Output {
   uint8_t* out;
   uint8_t* out_scales;
   uint32_t cout, cpitch, spitch;
-  float alpha, tensor_scale;
+  float alpha;
+  TensorScale ts;  // of 4-bit output
   int act, res_relu;
   int mode;    // 0: fp16, 1: MXFP4, 2: NVFP4
   int access;  // bytes of an fp16 row that may be stored (and of the residual, read) at once: 32, 16 or 2
@@ -114,16 +115,8 @@ __device__ __forceinline__ void emit32(const Output& o, float (&y)[32], uint64_t
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float s;
-    byte[h] = mx ? scale_mx(amax[h], s) : scale_nv(amax[h], o.tensor_scale, s);
-    const bool none = amax[h] >= 0x7f800000u || s == 0.f;
-    const Divider d = divider(mx ? SPCONVB_MXFP4 : SPCONVB_NVFP4, s, amax[h]);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float q[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = divide(d, y[16 * h + 8 * e + i]);
-      c[2 * h + e] = none ? 0u : codes8(q);
-    }
+    byte[h] = mx ? scale_mx(amax[h], s) : scale_nv(amax[h], o.ts, s);
+    codes_of<16>(mx, y + 16 * h, s, amax[h], c + 2 * h);
   }
   *(uint4*)(o.out + row * o.cpitch + col / 2u) = make_uint4(c[0], c[1], c[2], c[3]);
   uint8_t* so = o.out_scales + row * o.spitch;
@@ -155,7 +148,7 @@ inline bool make_output(const spconvb_fp4_params& p, const float* bias, void* ou
   o.res_relu = p.res_relu;
   if (p.out_fp4) {
     o.mode = p.out_format == SPCONVB_MXFP4 ? 1 : 2;
-    o.tensor_scale = p.out_tensor_scale;
+    o.ts = tensor_scale_of(p.out_tensor_scale);
     o.cpitch = code_pitch(o.cout);
     o.spitch = scale_pitch(p.out_format, o.cout);
   }

@@ -3,8 +3,8 @@
 // All three only move bytes.  A thread owns a unit of 16 channels: 32 bytes of fp16 in one load, 8 bytes of codes in one store, so
 // a warp reads and writes contiguous kilobytes; the scale of an MXFP4 block belongs to two neighbouring lanes, which
 // exchange their largest magnitudes.  Rows go one of three ways:
-//   flat     no padding anywhere (channels a multiple of 64 or 128) and 32-byte alignment: units, codes and scales are one sequence
-//            each, and a thread keeps the loads of kAhead units in flight
+//   flat     no padding of channels (NVFP4: a multiple of 64; MXFP4: of 128, or 64) and 32-byte alignment: units, codes and
+//            scales are one sequence each
 //   aligned  rows that start on 16 bytes: a unit is found by its row, 16 bytes at a time
 //   staged   all others: 256 units in a row are one contiguous piece of the fp16 / fp32 / int8 side, which passes through
 //            shared memory in 16-byte pieces
@@ -16,8 +16,11 @@ namespace fp4 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 2;
 enum Way { kFlat, kAligned, kStaged };
+// Units whose loads a thread keeps in flight on the flat way (int8 units are half as long); on the others one: with two, rows of 72
+// channels took 4.2 us and not 3.8, for what they have to compute before the load.
+template <int KIND, Way WAY>
+constexpr int kAhead = WAY == kFlat ? (KIND == SPCONVB_I8 ? 4 : 2) : 1;
 
 struct Rows {
   uint32_t channels, upr;  // units of 16 channels a row, padding included
@@ -128,33 +131,36 @@ __device__ __forceinline__ uint32_t elements(const Raw<KIND>& raw, float in_scal
 
 template <int FMT, int KIND, Way WAY>
 __device__ __forceinline__ void store_unit(const Rows& g, uint64_t u, uint64_t row, uint32_t ub, const Raw<KIND>& raw,
-                                           float in_scale, float tensor_scale, uint8_t* codes, uint8_t* scales, bool live) {
+                                           float in_scale, const TensorScale& ts, uint8_t* codes, uint8_t* scales, bool live) {
   float x[16];
   uint32_t amax = elements<KIND>(raw, in_scale, x);
   if (FMT == SPCONVB_MXFP4) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  if (!live) return;
   float s;
-  const uint32_t byte = FMT == SPCONVB_MXFP4 ? scale_mx(amax, s) : scale_nv(amax, tensor_scale, s);
-  const bool none = amax >= 0x7f800000u || s == 0.f;
-  const Divider d = divider(FMT, s, amax);
+  uint32_t byte = FMT == SPCONVB_MXFP4 ? scale_mx(amax, s) : scale_nv(amax, ts, s);
+  const bool word = FMT == SPCONVB_MXFP4 && WAY == kFlat && g.upr == 4u;  // rows of 64 channels: two scales, two bytes of padding
+  if (word) byte |= __shfl_down_sync(0xffffffffu, byte, 2) << 8;
+  if (!live) return;
   uint32_t c[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = divide(d, x[8 * h + i]);
-    c[h] = none ? 0u : codes8(q);
-  }
+  codes_of<16>(FMT == SPCONVB_MXFP4, x, s, amax, c);
   uint8_t* co = WAY == kFlat ? codes + u * 8u : codes + row * g.cpitch + ub * 8u;
   *(uint2*)co = make_uint2(c[0], c[1]);
   if (FMT == SPCONVB_NVFP4) {
     scales[WAY == kFlat ? u : row * g.spitch + ub] = (uint8_t)byte;
+  } else if (word) {
+    if (!(u & 3u)) *(uint32_t*)(scales + u) = byte;
   } else if (!(ub & 1u)) {
     uint8_t* so = WAY == kFlat ? scales + (u >> 1) : scales + row * g.spitch + (ub >> 1);
     *so = (uint8_t)byte;
     // the two bytes behind the last block of rows of an odd number of 64 channels
     if (WAY != kFlat && (g.upr & 4u) && ub + 2u == g.upr) so[1] = so[2] = 0;
   }
+}
+
+// Place of unit u's scale on the flat way.
+template <int FMT>
+__device__ __forceinline__ uint64_t flat_scale(const Rows& g, uint64_t u) {
+  if (FMT == SPCONVB_NVFP4) return u;
+  return g.upr == 4u ? (u & ~3ull) + (u >> 1 & 1u) : u >> 1;
 }
 
 // The contiguous piece of rows that units [u0, u1) cover: first element, and one past the last.
@@ -169,76 +175,79 @@ __device__ __forceinline__ void piece_of(const Rows& g, uint64_t u0, uint64_t u1
 
 template <int FMT, int KIND, Way WAY>
 __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const uint8_t* __restrict__ x, const Rows g, float in_scale,
-                                                                float tensor_scale, const uint32_t* n_ptr, uint32_t cap,
+                                                                const TensorScale ts, const uint32_t* n_ptr, uint32_t cap,
                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr uint32_t es = elem_size<KIND>();
   __shared__ uint4 buf[WAY == kStaged ? kThreads * es + 2 : 1];  // 16 bytes of slack at either end
   pdl_wait_and_trigger();
   const uint64_t units = (uint64_t)min(load_in_order(n_ptr), cap) * g.upr;
   // loops go by the block: the lanes of a warp exchange magnitudes
-  if (WAY == kFlat) {
-    constexpr uint64_t kBlock = kThreads * kAhead;
-    for (uint64_t u0 = (uint64_t)blockIdx.x * kBlock; u0 < units; u0 += (uint64_t)gridDim.x * kBlock) {
-      Raw<KIND> raw[kAhead];
+  if (WAY != kStaged) {
+    constexpr int A = kAhead<KIND, WAY>;
+    for (uint64_t u0 = (uint64_t)blockIdx.x * (kThreads * A); u0 < units; u0 += (uint64_t)gridDim.x * (kThreads * A)) {
+      Raw<KIND> raw[A];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+      for (int i = 0; i < A; ++i) {
         const uint64_t u = u0 + i * kThreads + threadIdx.x;
-        if (u < units) {
-          load_flat<KIND>(x + u * (16u * es), raw[i]);
-        } else {
 #pragma unroll
-          for (int j = 0; j < Raw<KIND>::kWords; ++j) raw[i].w[j] = 0u;
+        for (int j = 0; j < Raw<KIND>::kWords; ++j) raw[i].w[j] = 0u;
+        if (u < units) {
+          if (WAY == kFlat) {
+            load_flat<KIND>(x + u * (16u * es), raw[i]);
+          } else {
+            uint64_t row;
+            uint32_t ub;
+            place(g, u, row, ub);
+            load_aligned<KIND>(x + element_at(g, row, ub) * es, present(g, ub), raw[i]);
+          }
         }
       }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+      for (int i = 0; i < A; ++i) {
         const uint64_t u = u0 + i * kThreads + threadIdx.x;
-        store_unit<FMT, KIND, WAY>(g, u, 0u, (uint32_t)u & 1u, raw[i], in_scale, tensor_scale, codes, scales, u < units);
+        uint64_t row = 0;
+        uint32_t ub = (uint32_t)u & 1u;
+        if (WAY == kAligned) place(g, u, row, ub);
+        store_unit<FMT, KIND, WAY>(g, u, row, ub, raw[i], in_scale, ts, codes, scales, u < units);
       }
     }
   } else {
     for (uint64_t u0 = (uint64_t)blockIdx.x * kThreads; u0 < units; u0 += (uint64_t)gridDim.x * kThreads) {
       const uint64_t u = u0 + threadIdx.x;
       const bool live = u < units;
-      uint64_t row = 0, e0 = 0, e1 = 0;
+      uint64_t row = 0, e0, e1;
       uint32_t ub = 0;
       if (live) place(g, u, row, ub);
       const uint32_t left = live ? present(g, ub) : 0u;
-      uint64_t from = 0;
-      if (WAY == kStaged) {
-        piece_of(g, u0, min(u0 + kThreads, units), e0, e1);
-        // 16-byte pieces from the last boundary before e0 on; at the ends of x only what lies inside
-        const uint64_t a0 = (uint64_t)(uintptr_t)x + e0 * es, a1 = (uint64_t)(uintptr_t)x + e1 * es;
-        from = a0 & ~15ull;
-        __syncthreads();  // the units before are read
-        for (uint64_t p = from + threadIdx.x * 16u; p < a1; p += kThreads * 16u) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (p >= a0 && p + 16u <= a1) {
-            v = ld16((const void*)(uintptr_t)p);
-          } else {
-            uint8_t* b = (uint8_t*)&v;
+      piece_of(g, u0, min(u0 + kThreads, units), e0, e1);
+      // 16-byte pieces from the last boundary before e0 on; at the ends only what lies inside
+      const uint64_t a0 = (uint64_t)(uintptr_t)x + e0 * es, a1 = (uint64_t)(uintptr_t)x + e1 * es, from = a0 & ~15ull;
+      __syncthreads();  // the units before are read
+      for (uint64_t p = from + threadIdx.x * 16u; p < a1; p += kThreads * 16u) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (p >= a0 && p + 16u <= a1) {
+          v = ld16((const void*)(uintptr_t)p);
+        } else {
+          uint8_t* b = (uint8_t*)&v;
 #pragma unroll
-            for (uint32_t i = 0; i < 16u; i += es) {
-              if (p + i >= a0 && p + i < a1) {
-                if (es == 1u) b[i] = *(const volatile uint8_t*)(uintptr_t)(p + i);
-                else if (es == 2u) *(uint16_t*)(b + i) = *(const volatile uint16_t*)(uintptr_t)(p + i);
-                else *(uint32_t*)(b + i) = *(const volatile uint32_t*)(uintptr_t)(p + i);
-              }
+          for (uint32_t i = 0; i < 16u; i += es) {
+            if (p + i >= a0 && p + i < a1) {
+              if (es == 1u) b[i] = *(const volatile uint8_t*)(uintptr_t)(p + i);
+              else if (es == 2u) *(uint16_t*)(b + i) = *(const volatile uint16_t*)(uintptr_t)(p + i);
+              else *(uint32_t*)(b + i) = *(const volatile uint32_t*)(uintptr_t)(p + i);
             }
           }
-          buf[(p - from) >> 4] = v;
         }
-        __syncthreads();
+        buf[(p - from) >> 4] = v;
       }
+      __syncthreads();
       Raw<KIND> raw;
 #pragma unroll
       for (int j = 0; j < Raw<KIND>::kWords; ++j) raw.w[j] = 0u;
-      if (left) {
-        const uint64_t at = element_at(g, row, ub) * es;
-        if (WAY == kStaged) load_staged<KIND>((const uint32_t*)buf, (uint32_t)((uint64_t)(uintptr_t)x + at - from), left, raw);
-        else load_aligned<KIND>(x + at, left, raw);
-      }
-      store_unit<FMT, KIND, WAY>(g, u, row, ub, raw, in_scale, tensor_scale, codes, scales, live);
+      if (left)
+        load_staged<KIND>((const uint32_t*)buf, (uint32_t)((uint64_t)(uintptr_t)x + element_at(g, row, ub) * es - from), left,
+                          raw);
+      store_unit<FMT, KIND, WAY>(g, u, row, ub, raw, in_scale, ts, codes, scales, live);
     }
   }
 }
@@ -272,27 +281,49 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t*
   __shared__ uint4 buf[WAY == kStaged ? kThreads * es + 2 : 1];
   pdl_wait_and_trigger();
   const uint64_t units = (uint64_t)min(load_in_order(n_ptr), cap) * g.upr;
-  if (WAY == kFlat) {
-    constexpr uint64_t kBlock = kThreads * kAhead;
-    for (uint64_t u0 = (uint64_t)blockIdx.x * kBlock; u0 < units; u0 += (uint64_t)gridDim.x * kBlock) {
-      uint2 c[kAhead];
-      uint32_t byte[kAhead];
+  if (WAY != kStaged) {
+    constexpr int A = kAhead<KIND, WAY>;
+    for (uint64_t u0 = (uint64_t)blockIdx.x * (kThreads * A); u0 < units; u0 += (uint64_t)gridDim.x * (kThreads * A)) {
+      uint2 c[A];
+      uint32_t byte[A], left[A];
+      uint8_t* o[A];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+      for (int i = 0; i < A; ++i) {
         const uint64_t u = u0 + i * kThreads + threadIdx.x;
+        left[i] = 0u;
         if (u < units) {
-          c[i] = ld8(codes + u * 8u);
-          byte[i] = (uint32_t)load_in_order((const int8_t*)scales + (FMT == SPCONVB_MXFP4 ? u >> 1 : u)) & 255u;
+          if (WAY == kFlat) {
+            left[i] = 16u;
+            c[i] = ld8(codes + u * 8u);
+            byte[i] = (uint32_t)load_in_order((const int8_t*)scales + flat_scale<FMT>(g, u)) & 255u;
+            o[i] = out + u * (16u * es);
+          } else {
+            uint64_t row;
+            uint32_t ub;
+            place(g, u, row, ub);
+            left[i] = present(g, ub);
+            if (left[i]) {
+              c[i] = ld8(codes + row * g.cpitch + ub * 8u);
+              byte[i] = (uint32_t)load_in_order((const int8_t*)scales + row * g.spitch +
+                                                (FMT == SPCONVB_MXFP4 ? ub >> 1 : ub)) & 255u;
+            }
+            o[i] = out + element_at(g, row, ub) * es;
+          }
         }
       }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const uint64_t u = u0 + i * kThreads + threadIdx.x;
-        if (u < units) {
-          Raw<KIND> v;
-          values_of<FMT, KIND>(c[i], byte[i], tensor_scale, v);
+      for (int i = 0; i < A; ++i) {
+        if (left[i] == 0u) continue;
+        Raw<KIND> v;
+        values_of<FMT, KIND>(c[i], byte[i], tensor_scale, v);
+        if (WAY == kFlat) {
 #pragma unroll
-          for (int j = 0; j < Raw<KIND>::kWords / 8; ++j) st32(out + u * (16u * es) + 32 * j, v.w + 8 * j);
+          for (int j = 0; j < Raw<KIND>::kWords / 8; ++j) st32(o[i] + 32 * j, v.w + 8 * j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < (int)es; ++j)
+            if ((int)left[i] > j * 16 / (int)es)
+              ((uint4*)o[i])[j] = make_uint4(v.w[4 * j], v.w[4 * j + 1], v.w[4 * j + 2], v.w[4 * j + 3]);
         }
       }
     }
@@ -313,13 +344,6 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t*
         values_of<FMT, KIND>(c, byte, tensor_scale, v);
       }
       uint8_t* o = out + element_at(g, row, ub) * es;
-      if (WAY == kAligned) {
-#pragma unroll
-        for (int i = 0; i < (int)es; ++i)
-          if ((int)left > i * 16 / (int)es)
-            ((uint4*)o)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
-        continue;
-      }
       uint64_t e0, e1;
       piece_of(g, u0, min(u0 + kThreads, units), e0, e1);
       const uint64_t a0 = (uint64_t)(uintptr_t)out + e0 * es, a1 = (uint64_t)(uintptr_t)out + e1 * es, from = a0 & ~15ull;
@@ -373,12 +397,14 @@ Rows rows_of(int format, int channels, const void* p, uint32_t es) {
   g.spitch = scale_pitch(format, g.channels);
   const uint64_t row = (uint64_t)g.channels * es;
   if (((uint64_t)(uintptr_t)p | row) % 16u != 0u) g.way = kStaged;
-  else if (g.channels % (format == SPCONVB_MXFP4 ? 128u : 64u) == 0u && (uintptr_t)p % 32u == 0u) g.way = kFlat;
+  else if ((g.channels == 64u || g.channels % (format == SPCONVB_MXFP4 ? 128u : 64u) == 0u) && (uintptr_t)p % 32u == 0u)
+    g.way = kFlat;
   else g.way = kAligned;
   return g;
 }
+template <int KIND>
 int blocks_of(const Rows& g, uint32_t rows) {
-  const uint64_t per = kThreads * (g.way == kFlat ? kAhead : 1), b = ((uint64_t)rows * g.upr + per - 1) / per;
+  const uint64_t per = kThreads * (g.way == kFlat ? kAhead<KIND, kFlat> : 1), b = ((uint64_t)rows * g.upr + per - 1) / per;
   return (int)(b < (uint64_t)kSmCount * 16 ? b : (uint64_t)kSmCount * 16);
 }
 
@@ -423,7 +449,6 @@ __global__ void fp4_pack_kernel(int format, uint32_t cin, uint32_t cout, uint32_
 }
 
 struct Call {
-  int blocks;
   cudaStream_t st;
   Rows g;
   float in_scale, tensor_scale;
@@ -432,14 +457,14 @@ struct Call {
 };
 template <int FMT, int KIND>
 cudaError_t quantize_way(const Call& k, const uint8_t* x, uint8_t* codes, uint8_t* scales) {
-  const dim3 b(k.blocks), t(kThreads);
+  const dim3 b(blocks_of<KIND>(k.g, k.cap)), t(kThreads);
   if (k.g.way == kFlat)
-    return launch_pdl(fp4_quantize_kernel<FMT, KIND, kFlat>, b, t, 0, k.st, x, k.g, k.in_scale, k.tensor_scale, k.n, k.cap,
+    return launch_pdl(fp4_quantize_kernel<FMT, KIND, kFlat>, b, t, 0, k.st, x, k.g, k.in_scale, tensor_scale_of(k.tensor_scale), k.n, k.cap,
                       codes, scales);
   if (k.g.way == kAligned)
-    return launch_pdl(fp4_quantize_kernel<FMT, KIND, kAligned>, b, t, 0, k.st, x, k.g, k.in_scale, k.tensor_scale, k.n, k.cap,
+    return launch_pdl(fp4_quantize_kernel<FMT, KIND, kAligned>, b, t, 0, k.st, x, k.g, k.in_scale, tensor_scale_of(k.tensor_scale), k.n, k.cap,
                       codes, scales);
-  return launch_pdl(fp4_quantize_kernel<FMT, KIND, kStaged>, b, t, 0, k.st, x, k.g, k.in_scale, k.tensor_scale, k.n, k.cap, codes,
+  return launch_pdl(fp4_quantize_kernel<FMT, KIND, kStaged>, b, t, 0, k.st, x, k.g, k.in_scale, tensor_scale_of(k.tensor_scale), k.n, k.cap, codes,
                     scales);
 }
 template <int FMT>
@@ -450,7 +475,7 @@ cudaError_t quantize_kind(int kind, const Call& k, const uint8_t* x, uint8_t* co
 }
 template <int FMT, int KIND>
 cudaError_t dequantize_way(const Call& k, const uint8_t* codes, const uint8_t* scales, uint8_t* out) {
-  const dim3 b(k.blocks), t(kThreads);
+  const dim3 b(blocks_of<KIND>(k.g, k.cap)), t(kThreads);
   if (k.g.way == kFlat)
     return launch_pdl(fp4_dequantize_kernel<FMT, KIND, kFlat>, b, t, 0, k.st, codes, scales, k.g, k.tensor_scale, k.n, k.cap, out);
   if (k.g.way == kAligned)
@@ -503,7 +528,7 @@ int spconvb_fp4_quantize(int32_t format, const void* x, int32_t kind, float in_s
   if (!aligned16(codes, scales) || (uintptr_t)x % es != 0u) return SPCONVB_E_ARG;
   if (kind == SPCONVB_I8 && !(in_scale > -3.4e38f && in_scale < 3.4e38f)) return SPCONVB_E_ARG;
   const Rows g = rows_of(format, channels, x, es);
-  const Call k{blocks_of(g, launch_rows), (cudaStream_t)stream, g, in_scale, tensor_scale, n_ptr, launch_rows};
+  const Call k{(cudaStream_t)stream, g, in_scale, tensor_scale, n_ptr, launch_rows};
   SPCONVB_CUDA_TRY(format == SPCONVB_MXFP4
                        ? quantize_kind<SPCONVB_MXFP4>(kind, k, (const uint8_t*)x, (uint8_t*)codes, (uint8_t*)scales)
                        : quantize_kind<SPCONVB_NVFP4>(kind, k, (const uint8_t*)x, (uint8_t*)codes, (uint8_t*)scales));
@@ -519,7 +544,7 @@ int spconvb_fp4_dequantize(int32_t format, const void* codes, const void* scales
   const uint32_t es = out_kind == SPCONVB_F32 ? 4u : 2u;
   if (!aligned16(codes, scales) || (uintptr_t)out % es != 0u) return SPCONVB_E_ARG;
   const Rows g = rows_of(format, channels, out, es);
-  const Call k{blocks_of(g, launch_rows), (cudaStream_t)stream, g, 1.f, tensor_scale, n_ptr, launch_rows};
+  const Call k{(cudaStream_t)stream, g, 1.f, tensor_scale, n_ptr, launch_rows};
   const uint8_t *c = (const uint8_t*)codes, *s = (const uint8_t*)scales;
   SPCONVB_CUDA_TRY(format == SPCONVB_MXFP4 ? dequantize_kind<SPCONVB_MXFP4>(out_kind, k, c, s, (uint8_t*)out)
                                            : dequantize_kind<SPCONVB_NVFP4>(out_kind, k, c, s, (uint8_t*)out));
