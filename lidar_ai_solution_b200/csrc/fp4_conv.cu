@@ -3,33 +3,34 @@
 //   out[o, :] = act(alpha * sum_k W[:, k, :] . in[map[k][o], :] + bias)  (+ residual)
 //
 // Voxel rows on the M side (a tile is up to 128 of them, one an accumulator lane), output channels on the N side, K in chunks
-// of 256 channels: 4, 2 or 1 taps of 64, 128 or 256 channels.  Roles of the warps of a CTA (one an SM, walking over tiles
-// whose height deals the rows out evenly):
+// of 256 channels: 4, 2 or 1 taps of 64, 128 or 256.  Roles of the warps of a CTA (one an SM, walking over tiles whose height
+// deals the rows out evenly):
 //
-//   0-7    epilogue: a lane owns a row; a warp its quadrant of 32 rows and half of the channels
-//   8      allocates tensor memory, copies the chunk's scales there, issues its MMAs
-//   9      one lane: the weights, a bulk copy of codes and scales a chunk, or once where all chunks fit
-//   10-..  producers, kGroups groups of four warps that take the chunks in turn; a warp owns 32 rows, a thread one 16-byte
-//          segment of 8 of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, zeros for missing
-//          neighbours, all of which arrive on the stage's barrier by themselves
+//   0-15   epilogue: a lane owns a row, a warp its quadrant of 32 and 32 channels; with 64 channels two sets of warps take the
+//          tiles in turn
+//   16     allocates tensor memory, copies the chunk's scales there, issues its MMAs
+//   17     one lane: the weights, a bulk copy of codes and scales a chunk, or once where all chunks fit
+//   18-25  producers, two groups of four that take the chunks in turn; a warp owns 32 rows, a thread one 16-byte segment of 8
+//          of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, zeros for missing neighbours, all
+//          of which arrive on the stage's barrier by themselves
 //
 // Within the 32 rows of a warp, row 8 slot + i of the tile lies at 4 i + slot of the operand: the words of scales that
 // the 32 lanes write at the same time then lie in eight groups of four banks and not in two.
 #include "fp4_epilogue.cuh"
-#include "fp4_umma.cuh"
-#include "pdl.cuh"
 
 namespace spconvb {
 namespace fp4 {
 namespace {
 
 constexpr uint32_t kTileRows = 128;
-constexpr int kEpiWarps = 8, kMmaWarp = 8, kWeightWarp = 9, kProdWarp0 = 10;
+constexpr int kEpiWarps = 16, kMmaWarp = 16, kWeightWarp = 17, kProdWarp0 = 18;
 constexpr uint32_t kGroups = 2;
 constexpr int kCtaThreads = 32 * (kProdWarp0 + 4 * (int)kGroups);
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kRingBytes = 224 * 1024;
-constexpr size_t kSmemBytes = kRingBytes + 1024 + 512;
+constexpr uint32_t kRingBytes = 191 * 1024;
+constexpr size_t kSmemBytes = kRingBytes + kEpiWarps * kStageBytes + 1024 + 512;
+
+static_assert(kSmemBytes <= 232448, "shared memory");
 
 struct ConvArgs {
   const uint8_t* codes;
@@ -59,8 +60,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   constexpr uint32_t kSteps = 4 / W;               // MMAs a word
   constexpr uint32_t kRecord = 128 * 128 + W * kAtomBytes;          // a chunk in the weights' image
   constexpr uint32_t kWeightBytes = COUT * 128 + W * kAtomBytes;     // and in shared memory
-  constexpr uint32_t kRowStage = kTileRows * 128 + W * kAtomBytes, kSfOff = kTileRows * 128;
+  constexpr uint32_t kSfOff = kTileRows * 128, kRowStage = kSfOff + W * kAtomBytes;
   constexpr uint32_t kSfCols = 8 * W;  // of a stage in tensor memory: rows, weights
+  constexpr uint32_t kDrain = COUT / 32 * 4;  // warps that drain a tile
   static_assert(2 * COUT + kMaxStages * kSfCols <= kTmemCols, "tensor memory");
 
   const int kbytes = a.kvol * RB;
@@ -70,12 +72,15 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
-  uint64_t* bars = (uint64_t*)(smem + kRingBytes);
-  uint32_t* tmem_holder = (uint32_t*)(bars + 2 * kMaxStages + 4);
+  uint64_t* bars = (uint64_t*)(smem + kRingBytes + kEpiWarps * kStageBytes);
+  uint32_t* tmem_holder = (uint32_t*)(bars + 3 * kMaxStages + 4);
   volatile uint32_t* abort_flag = tmem_holder + 1;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kMaxStages;
   const uint32_t bar_tfull = bar_empty + 8 * kMaxStages, bar_tempty = bar_tfull + 16;
-  const int warp = threadIdx.x >> 5;
+  const uint32_t bar_weights = bar_tempty + 16;  // of chunks that stay
+  // Warp index, row count and tensor-memory address are made the same for all lanes where the compiler sees it: what is computed from
+  // them, and the loops they bound, then stay in uniform registers, which is where the tensor-core instructions take their operands.
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const uint32_t lane = threadIdx.x & 31;
 
   if (warp == kMmaWarp) {
@@ -85,7 +90,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait_and_trigger();
-  const uint32_t n_out = min(load_in_order(a.n_out_ptr), a.cap);
+  const uint32_t n_out = __shfl_sync(0xffffffffu, min(load_in_order(a.n_out_ptr), a.cap), 0);
 
   // Tile height: the smallest multiple of 32 with which every CTA gets the same number of tiles.
   const uint32_t per_cta = (n_out + gridDim.x - 1) / gridDim.x;
@@ -93,20 +98,21 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   const uint32_t tile_rows = max(32u, ((per_cta + rounds - 1) / rounds + 31u) & ~31u);
   const uint32_t t32 = tile_rows >> 5;
   const uint32_t ntiles = (n_out + tile_rows - 1) / tile_rows;
-  // Two rings share the buffer, rows with their scales and weights with theirs.  Weights of which all chunks fit stay.
+  // Two rings share the buffer, rows with their scales and weights with theirs.  Weights of which all chunks fit beside four
+  // stages of rows stay, and are waited for on barriers of their own.
   constexpr uint32_t kFit = kRingBytes / (kWeightBytes + kRowStage);
-  const uint32_t fit = min((uint32_t)kMaxStages, kFit);
-  const bool resident = (uint32_t)nchunk <= fit;
-  const uint32_t nwst = resident ? (uint32_t)nchunk : fit;
+  const bool resident = nchunk <= kMaxStages && kRingBytes >= (uint32_t)nchunk * kWeightBytes + 4u * kRowStage;
+  const uint32_t nwst = resident ? (uint32_t)nchunk : kFit;
   const uint32_t nst = min((uint32_t)kMaxStages, (kRingBytes - nwst * kWeightBytes) / kRowStage);
   const uint32_t sW = smem_u32(smem), sR = sW + nwst * kWeightBytes;
 
   if (threadIdx.x < kMaxStages) {
-    mbar_init(bar_full + 8 * threadIdx.x, 32u * t32 + 1u);
+    mbar_init(bar_full + 8 * threadIdx.x, 32u * t32 + (resident ? 0u : 1u));
     mbar_init(bar_empty + 8 * threadIdx.x, 1);
+    mbar_init(bar_weights + 8 * threadIdx.x, 1);
     if (threadIdx.x < 2) {
       mbar_init(bar_tfull + 8 * threadIdx.x, 1);
-      mbar_init(bar_tempty + 8 * threadIdx.x, kEpiWarps);
+      mbar_init(bar_tempty + 8 * threadIdx.x, kDrain);
     }
     if (threadIdx.x == 0) *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,7 +121,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_holder;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
 
   if (warp == kWeightWarp) {
     // -------------------------------------------------------------- weights
@@ -124,15 +130,15 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       uint32_t os = 0, oph = 0;  // row stage and phase of the chunk `nwst` before
       uint32_t tile = blockIdx.x;
       int j = 0;
-      auto fetch = [&]() {
-        mbar_expect_tx(bar_full + 8 * s, kWeightBytes);
+      auto fetch = [&](uint32_t bar) {
+        mbar_expect_tx(bar, kWeightBytes);
         const uint8_t* src = a.wpk + (size_t)j * kRecord;
         const uint32_t dst = sW + ws * kWeightBytes;
         if (COUT == 128) {
-          bulk_g2s(dst, src, kWeightBytes, bar_full + 8 * s);
+          bulk_g2s(dst, src, kWeightBytes, bar);
         } else {
-          bulk_g2s(dst, src, COUT * 128, bar_full + 8 * s);
-          bulk_g2s(dst + COUT * 128, src + 128 * 128, W * kAtomBytes, bar_full + 8 * s);
+          bulk_g2s(dst, src, COUT * 128, bar);
+          bulk_g2s(dst + COUT * 128, src + 128 * 128, W * kAtomBytes, bar);
         }
         if (++s == nst) s = 0;
         if (++ws == nwst) ws = 0;
@@ -141,15 +147,20 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
           tile += gridDim.x;
         }
       };
+      if (resident) {
+        if (tile < ntiles)
+          for (int k = 0; k < nchunk; ++k) fetch(bar_weights + 8 * k);
+      } else {
 #pragma unroll 1
-      for (uint32_t n = 0; n < nwst && tile < ntiles; ++n) fetch();
-      while (!resident && tile < ntiles) {
-        if (!mbar_wait_spin(bar_empty + 8 * os, oph, abort_flag, a.status, 36u)) break;
-        if (++os == nst) {
-          os = 0;
-          oph ^= 1u;
+        for (uint32_t n = 0; n < nwst && tile < ntiles; ++n) fetch(bar_full + 8 * s);
+        while (tile < ntiles) {
+          if (!mbar_wait_spin(bar_empty + 8 * os, oph, abort_flag, a.status, 36u)) break;
+          if (++os == nst) {
+            os = 0;
+            oph ^= 1u;
+          }
+          fetch(bar_full + 8 * s);
         }
-        fetch();
       }
     }
     __syncwarp();
@@ -193,7 +204,6 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     uint32_t ntile = tile;
     int nj = j;
     uint32_t it = grp, s = grp % nst, ph = (grp / nst) & 1u;
-    const uint32_t first_thread = 32u * (kProdWarp0 + grp * 4u);
     auto step = [&](int32_t (&idx)[8]) -> bool {
       if (tile >= ntiles) return false;
       if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, abort_flag, a.status, 31u)) return false;
@@ -220,8 +230,6 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
         cp_async4(stage + sf_dst + (kParts * i + part) * 64u, src + (int64_t)sr * kPitch, sr < 0 ? 0u : 4u);
       }
       if (!(a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) cp_async_arrive_noinc(bar_full + 8 * s);
-      // the weights' arrival, where they are there already
-      if (resident && tile != blockIdx.x && threadIdx.x == first_thread) mbar_arrive(bar_full + 8 * s);
       load_idx(ntile, nj, idx);
       advance(ntile, nj, kGroups);
       advance(tile, j, kGroups);
@@ -259,6 +267,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       uint32_t accumulate = 0u;
 #pragma unroll 1
       for (int j = 0; j < nchunk; ++j) {
+        if (resident && tl == 0u)
+          alive = alive && mbar_wait_spin(bar_weights + 8 * j, 0u, abort_flag, a.status, 37u);
         alive = alive && (mbar_test_wait(bar_full + 8 * s, ph) ||
                           mbar_wait_spin(bar_full + 8 * s, ph, abort_flag, a.status, 33u));
         __syncwarp();
@@ -295,46 +305,38 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     __syncwarp();
   } else {
     // ------------------------------------------------------------- epilogue
-    const uint32_t q = (uint32_t)warp & 3u, half = (uint32_t)warp >> 2;
+    const uint32_t q = (uint32_t)warp & 3u, set = (uint32_t)warp >> 2;
+    constexpr uint32_t kTurns = kEpiWarps / kDrain;  // sets of warps that take the tiles in turn
+    const uint32_t turn = set / (COUT / 32u);
+    Patch p;
     // lane 4 i + slot of a quadrant is row 8 slot + i of its 32
-    const uint32_t row_in_tile = 32u * q + (lane & 3u) * 8u + (lane >> 2);
-    constexpr uint32_t kSets = COUT / 64;  // sets of 32 channels of a warp
-    const uint32_t col0 = half * (COUT / 2u), most = (a.o.cout + 63u) & ~63u;
-    uint32_t tl = 0;
-    for (uint32_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++tl) {
+    p.own = (lane & 3u) * 8u + (lane >> 2);
+    p.col = set % (COUT / 32u) * 32u;
+    p.lane = lane;
+    p.stage = sW + kRingBytes + (uint32_t)warp * kStageBytes;
+    const bool cols = p.col < ((a.o.cout + 63u) & ~63u);
+    stage_bias(p, load_bias(a.o, p));
+    uint32_t tl = turn;
+    for (uint32_t tile = blockIdx.x + turn * gridDim.x; tile < ntiles; tile += kTurns * gridDim.x, tl += kTurns) {
       const uint32_t buf = tl & 1u;
-      const uint64_t row = (uint64_t)tile * tile_rows + row_in_tile;
-      const bool live = row_in_tile < tile_rows && row < n_out;
-      uint32_t res[kSets][16];
-      if (RES) {
-#pragma unroll
-        for (uint32_t g = 0; g < kSets; ++g)
-          if (live) load_residual(a.o, row, col0 + 32u * g, res[g]);
-      }
+      p.row0 = (uint64_t)tile * tile_rows + 32u * q;
+      p.rows = min((uint64_t)n_out, (uint64_t)tile * tile_rows + tile_rows);  // rows of the tile end here
+      const bool any = p.row0 < p.rows && cols;
+      if (RES && any) prefetch_residual(a.o, p);
       uint32_t ok = 1u;
       if (lane == 0) ok = mbar_wait(bar_tfull + 8 * buf, (tl >> 1) & 1u, abort_flag, a.status, 34u) ? 1u : 0u;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((32u * q) << 16) + buf * COUT + col0;
-#pragma unroll
-      for (uint32_t g = 0; g < kSets; ++g) {
-        uint32_t v[32];
-        tmem_ld32(taddr + 32u * g, v);
-        tmem_ld_wait();
-        if (g + 1u == kSets) {  // no more reads of this accumulator by this warp
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
-        }
-        if (live && col0 + 32u * g < most) {
-          float y[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(v[i]);
-          emit32<RES>(a.o, y, row, col0 + 32u * g, res[g]);
-        }
-      }
+      uint32_t v[32];
+      tmem_ld32(tmem_base + ((32u * q) << 16) + buf * COUT + p.col, v);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+      if (any) emit32<RES>(a.o, v, p);
     }
+    if (RES) cp_async_wait_all();  // nothing of this thread may still be writing when the CTA exits
   }
 
   // ---------------------------------------------------------------- teardown

@@ -1,6 +1,6 @@
 // What both products do with their sums: a lane owns a row, 32 channels at a time.
 #pragma once
-#include "fp4.cuh"
+#include "fp4_umma.cuh"
 #include "pdl.cuh"
 
 namespace spconvb {
@@ -16,116 +16,157 @@ struct Output {
   TensorScale ts;  // of 4-bit output
   int act, res_relu;
   int mode;    // 0: fp16, 1: MXFP4, 2: NVFP4
-  int access;  // bytes of an fp16 row that may be stored (and of the residual, read) at once: 32, 16 or 2
+  int access;  // bytes of an fp16 row that may be stored (and of the residual, read) at once: 16 or 2
 };
 
-// The residual's 32 channels from `col` on, as pairs (channels that do not exist: 0).  Read in program order: it may be what the
-// launch before wrote.
-__device__ __forceinline__ void load_residual(const Output& o, uint64_t row, uint32_t col, uint32_t (&r)[16]) {
-  const __half* p = o.res + row * o.cout + col;
-  if (o.access == 32) {
+// A warp's 32 rows x 32 channels of fp16 between its lanes and memory by way of 2 KB of shared memory: a lane has a row
+// there, and a quarter of a row on the way to memory, where eight rows go at a time (a lane's own 32 bytes of 32 rows touch 32
+// lines an instruction and not 8).  Piece c (16 bytes) of row r lies at piece c ^ (r / 2 + r / 8) % 4 of its 64 bytes: free of bank conflicts
+// for lanes that have rows 0, 1, 2, ... and for lanes that have rows 0, 8, 16, 24, 1, 9, ...
+constexpr uint32_t kStageBytes = 2048 + 128;  // and behind it the patch's bias
+__device__ __forceinline__ uint32_t staged_at(uint32_t r, uint32_t c) {
+  return r * 64u + ((c ^ ((r >> 1 ^ r >> 3) & 3u)) << 4);
+}
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// Where a warp's 32 rows x 32 channels are: rows row0 .. (those below `rows` exist; this lane has row0 + own), channels col ..
+struct Patch {
+  uint64_t row0, rows;
+  uint32_t col, own, lane, stage;
+};
+
+// The patch's bias on its way into shared memory (zeros where there is none): a load that the epilogue would wait for is made long
+// before it.  (Read where it is used, 14 000 rows 64 -> 64 took 8.8 us and not 6.5.)
+__device__ __forceinline__ float load_bias(const Output& o, const Patch& p) {
+  return o.bias && p.col + p.lane < o.cout ? __ldg(o.bias + p.col + p.lane) : 0.f;
+}
+__device__ __forceinline__ void stage_bias(const Patch& p, float b) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(p.stage + 2048u + 4u * p.lane), "f"(b) : "memory");
+}
+
+// The residual on its way into the patch's shared memory (with 16-byte access; else it is read where it is used).  Copies in
+// program order: it may be what the launch before wrote.
+__device__ __forceinline__ void prefetch_residual(const Output& o, const Patch& p) {
+  if (o.access < 16) return;
+  __syncwarp();  // what was there is read
+  const uint32_t c = p.col + 8u * (p.lane % 4u);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (col + 16u * i < o.cout) {
-        ld32(p + 16 * i, r + 8 * i);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[8 * i + j] = 0u;
-      }
-    }
-  } else if (o.access == 16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (col + 8u * i < o.cout) v = ld16(p + 8 * i);
-      r[4 * i] = v.x;
-      r[4 * i + 1] = v.y;
-      r[4 * i + 2] = v.z;
-      r[4 * i + 3] = v.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      r[i] = 0u;
-      if (col + 2u * i < o.cout) r[i] = (uint32_t)load_in_order((const uint16_t*)p + 2 * i);
-      if (col + 2u * i + 1u < o.cout) r[i] |= (uint32_t)load_in_order((const uint16_t*)p + 2 * i + 1) << 16;
-    }
+  for (uint32_t k = 0; k < 4; ++k) {
+    const uint32_t r = 8u * k + p.lane / 4u;
+    const bool there = p.row0 + r < p.rows && c < o.cout;
+    cp_async16(p.stage + staged_at(r, p.lane % 4u), o.res + (there ? (p.row0 + r) * o.cout + c : 0u), there ? 16u : 0u);
   }
 }
 
-// 32 channels of one row, from fp32 sums to memory.  `col` is a multiple of 32 below cout rounded up to 64; the row exists.
-// A NaN passes through ReLU (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays one
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// Sums of 32 channels of this lane's row to results in memory: alpha, bias, activation, residual, fp16 or 4 bits.
+// `col` is a multiple of 32 below cout rounded up to 64.
 template <bool RES>
-__device__ __forceinline__ void emit32(const Output& o, float (&y)[32], uint64_t row, uint32_t col,
-                                       const uint32_t (&res)[16]) {
-  const float lo = o.act == SPCONVB_ACT_RELU ? 0.f : -INFINITY;
-  auto above = [](float v, float least) { return v < least ? least : v; };
-  if (o.bias && col + 32u <= o.cout && ((uintptr_t)o.bias & 15u) == 0u) {
+__device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const Patch& p) {
+  const uint64_t row = p.row0 + p.own;
+  const bool live = row < p.rows, wide = o.access >= 16;
+  const float lo = o.act == SPCONVB_ACT_RELU ? 0.f : -INFINITY, lo2 = o.res_relu ? 0.f : -INFINITY;
+  if (RES && wide) cp_async_wait_all();
+  __syncwarp();  // residual and bias are there, and what was there is read
+  // step by step over all 32 channels, so that the loads of a step are in flight together
+  {
+    uint4 b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 b = __ldg((const float4*)(o.bias + col) + i);
-      y[4 * i] = above(fmaf(y[4 * i], o.alpha, b.x), lo);
-      y[4 * i + 1] = above(fmaf(y[4 * i + 1], o.alpha, b.y), lo);
-      y[4 * i + 2] = above(fmaf(y[4 * i + 2], o.alpha, b.z), lo);
-      y[4 * i + 3] = above(fmaf(y[4 * i + 3], o.alpha, b.w), lo);
+    for (int i = 0; i < 8; ++i) b[i] = ld_shared16(p.stage + 2048u + 16u * i);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint32_t w = i % 4 == 0 ? b[i / 4].x : (i % 4 == 1 ? b[i / 4].y : (i % 4 == 2 ? b[i / 4].z : b[i / 4].w));
+      v[i] = __float_as_uint(max_nan(fmaf(__uint_as_float(v[i]), o.alpha, __uint_as_float(w)), lo));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      y[i] = col + i < o.cout ? above(fmaf(y[i], o.alpha, o.bias ? __ldg(o.bias + col + i) : 0.f), lo) : 0.f;
   }
   if (RES) {
-    const float lo2 = o.res_relu ? 0.f : -INFINITY;
+    uint32_t r[16];
+    if (wide) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint4 t = ld_shared16(p.stage + staged_at(p.own, c));
+        r[4 * c] = t.x; r[4 * c + 1] = t.y; r[4 * c + 2] = t.z; r[4 * c + 3] = t.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t at = p.col + 2 * i;
+        const uint16_t* q = (const uint16_t*)o.res + row * o.cout + at;
+        r[i] = live && at < o.cout ? (uint32_t)load_in_order(q) : 0u;
+        if (live && at + 1u < o.cout) r[i] |= (uint32_t)load_in_order(q + 1) << 16;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float2 r = __half22float2(*(const __half2*)&res[i]);
-      y[2 * i] = above(__fadd_rn(__half2float(__float2half_rn(y[2 * i])), r.x), lo2);
-      y[2 * i + 1] = above(__fadd_rn(__half2float(__float2half_rn(y[2 * i + 1])), r.y), lo2);
+      const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));  // as it would have been stored
+      const float2 x = __half22float2(h), y = __half22float2(*(const __half2*)&r[i]);
+      v[2 * i] = __float_as_uint(max_nan(__fadd_rn(x.x, y.x), lo2));
+      v[2 * i + 1] = __float_as_uint(max_nan(__fadd_rn(x.y, y.y), lo2));
     }
   }
   if (o.mode == 0) {
-    __half* p = (__half*)o.out + row * o.cout + col;
     uint32_t h[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const __half2 two = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+      const __half2 two = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
       h[i] = *(const uint32_t*)&two;
     }
-    if (o.access == 32) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (col + 16u * i < o.cout) st32(p + 16 * i, h + 8 * i);
-    } else if (o.access == 16) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col + 8u * i < o.cout)
-          ((uint4*)p)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-    } else {
+    if (!wide) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (col + i < o.cout) ((uint16_t*)p)[i] = (uint16_t)(h[i / 2] >> (16 * (i % 2)));
+        if (live && p.col + i < o.cout) ((uint16_t*)o.out)[row * o.cout + p.col + i] = (uint16_t)(h[i / 2] >> (16 * (i % 2)));
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) st_shared16(p.stage + staged_at(p.own, c), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+    __syncwarp();
+    uint4 t[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) t[k] = ld_shared16(p.stage + staged_at(8u * k + p.lane / 4u, p.lane % 4u));
+    const uint32_t c = p.col + 8u * (p.lane % 4u);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint64_t at = p.row0 + 8u * k + p.lane / 4u;
+      if (at < p.rows && c < o.cout) *(uint4*)((__half*)o.out + at * o.cout + c) = t[k];
     }
     return;
   }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = p.col + i < o.cout ? v[i] : 0u;
+  if (!live) return;
   uint32_t amax[2] = {0u, 0u}, c[4], byte[2];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) amax[i / 16] = max(amax[i / 16], __float_as_uint(y[i]) & 0x7fffffffu);
+  for (int i = 0; i < 32; ++i) amax[i / 16] = max(amax[i / 16], v[i] & 0x7fffffffu);
   const bool mx = o.mode == 1;
   if (mx) amax[0] = amax[1] = max(amax[0], amax[1]);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float s;
+    float s, y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(v[16 * h + i]);
     byte[h] = mx ? scale_mx(amax[h], s) : scale_nv(amax[h], o.ts, s);
-    codes_of<16>(mx, y + 16 * h, s, amax[h], c + 2 * h);
+    codes_of<16>(mx, y, s, amax[h], c + 2 * h);
   }
-  *(uint4*)(o.out + row * o.cpitch + col / 2u) = make_uint4(c[0], c[1], c[2], c[3]);
+  *(uint4*)(o.out + row * o.cpitch + p.col / 2u) = make_uint4(c[0], c[1], c[2], c[3]);
   uint8_t* so = o.out_scales + row * o.spitch;
   if (mx) {
-    so[col / 32u] = (uint8_t)byte[0];
+    so[p.col / 32u] = (uint8_t)byte[0];
     // the bytes behind the last block of rows of an odd number of 64 channels
-    if (col / 2u + 16u == o.cpitch && (o.cpitch & 32u)) so[col / 32u + 1u] = so[col / 32u + 2u] = 0;
+    if (p.col / 2u + 16u == o.cpitch && (o.cpitch & 32u)) so[p.col / 32u + 1u] = so[p.col / 32u + 2u] = 0;
   } else {
-    *(uint16_t*)(so + col / 16u) = (uint16_t)(byte[0] | byte[1] << 8);
+    *(uint16_t*)(so + p.col / 16u) = (uint16_t)(byte[0] | byte[1] << 8);
   }
 }
 
@@ -153,7 +194,7 @@ inline bool make_output(const spconvb_fp4_params& p, const float* bias, void* ou
     o.spitch = scale_pitch(p.out_format, o.cout);
   }
   const uint64_t bits = (uint64_t)(uintptr_t)p.res | 2ull * o.cout | (p.out_fp4 ? 0ull : (uint64_t)(uintptr_t)out);
-  o.access = bits % 32u == 0u ? 32 : (bits % 16u == 0u ? 16 : 2);
+  o.access = bits % 16u == 0u ? 16 : 2;
   return true;
 }
 

@@ -4,10 +4,11 @@
 // 256 channels: 128 bytes of codes a row, which is one swizzle atom, and four MMAs of 64 channels.  Roles of the
 // warps of a CTA (one an SM, walking over tiles):
 //
-//   0-7    epilogue: a lane owns a row; a warp its quadrant of 32 rows and half of the tile's channels
-//   8      allocates tensor memory; copies the chunk's scales there and issues its MMAs
-//   9      one lane: TMA of the rows' codes, bulk copies of the weights' image (codes and scales lie ready in it)
-//   10-13  the rows' scales, a row a lane: four chunks ahead in registers, then as words into the order that the
+//   0-15   epilogue: a lane owns a row, a warp its quadrant of 32 and 32 or 64 channels (with TN = 64 two sets of warps take the
+//          tiles in turn)
+//   16     allocates tensor memory; copies the chunk's scales there and issues its MMAs
+//   17     one lane: TMA of the rows' codes, bulk copies of the weights' image (codes and scales lie ready in it)
+//   18-21  the rows' scales, a row a lane: four chunks ahead in registers, then as words into the order that the
 //          copy to tensor memory wants.  (They are kept row by row in memory, so that a convolution can gather them.)
 //
 // Scales in tensor memory have a place for every stage of the ring: a stage is filled again only when the MMAs that
@@ -16,15 +17,13 @@
 // Few rows: the K axis is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
 // always in the same order.
 #include "fp4_epilogue.cuh"
-#include "fp4_umma.cuh"
-#include "pdl.cuh"
 
 namespace spconvb {
 namespace fp4 {
 namespace {
 
-constexpr int kEpiWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kScaleWarp0 = 10;
-constexpr int kCtaThreads = 32 * 14;
+constexpr int kEpiWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kScaleWarp0 = 18;
+constexpr int kCtaThreads = 32 * 22;
 constexpr uint32_t kTileM = 128;
 constexpr uint32_t kTmemCols = 512;
 
@@ -49,10 +48,13 @@ struct Shape {
   static constexpr uint32_t kA = kTileM * 128, kB = TN * 128;
   static constexpr uint32_t kOffB = kA, kOffSfb = kA + kB, kOffSfa = kOffSfb + kBlocks * kSf;
   static constexpr uint32_t kStage = kOffSfa + kSf;  // a multiple of 1024
-  static constexpr uint32_t kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);
+  static constexpr uint32_t kStages = TN == 256 ? 3 : (TN == 128 ? 5 : 6);
   static constexpr uint32_t kBuffers = TN == 256 ? 1 : 2;  // accumulators
   static constexpr uint32_t kSfCols = kWords * 4 * (1 + kBlocks);
-  static constexpr uint32_t kSmem = kStages * kStage + 1024 + 512;
+  static constexpr uint32_t kPatches = TN == 256 ? 2 : 1;            // of 32 channels a warp
+  static constexpr uint32_t kDrain = TN == 64 ? 8 : 16;             // warps that drain a tile
+  static constexpr uint32_t kRing = kStages * kStage;
+  static constexpr uint32_t kSmem = kRing + kEpiWarps * kStageBytes + 1024 + 512;
   static_assert(kStage % 1024 == 0, "stages start on swizzle atoms");
   static_assert(kBuffers * TN + kStages * kSfCols <= kTmemCols, "tensor memory");
   static_assert(kSmem <= 232448, "shared memory");
@@ -77,12 +79,14 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   const uint32_t s0 = smem_u32(smem);
-  uint64_t* bars = (uint64_t*)(smem + S::kStages * S::kStage);
+  uint64_t* bars = (uint64_t*)(smem + S::kRing + kEpiWarps * kStageBytes);
   uint32_t* tmem_holder = (uint32_t*)(bars + 2 * S::kStages + 4);
   volatile uint32_t* abort_flag = tmem_holder + 1;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::kStages;
   const uint32_t bar_tfull = bar_empty + 8 * S::kStages, bar_tempty = bar_tfull + 16;
-  const int warp = threadIdx.x >> 5;
+  // Warp index, row count and tensor-memory address are made the same for all lanes where the compiler sees it: what is computed from
+  // them, and the loops they bound, then stay in uniform registers, which is where the tensor-core instructions take their operands.
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const uint32_t lane = threadIdx.x & 31;
 
   if (threadIdx.x < S::kStages) {
@@ -90,7 +94,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     mbar_init(bar_empty + 8 * threadIdx.x, 1);
     if (threadIdx.x < 2) {
       mbar_init(bar_tfull + 8 * threadIdx.x, 1);
-      mbar_init(bar_tempty + 8 * threadIdx.x, kEpiWarps);
+      mbar_init(bar_tempty + 8 * threadIdx.x, S::kDrain);
     }
     if (threadIdx.x == 0) *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -103,11 +107,11 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait_and_trigger();
-  const uint32_t n = min(load_in_order(a.n_ptr), a.cap);
+  const uint32_t n = __shfl_sync(0xffffffffu, min(load_in_order(a.n_ptr), a.cap), 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
 
   const uint32_t tiles_n = (a.o.cout + TN - 1) / TN;
   const uint32_t tiles = ((n + kTileM - 1) / kTileM) * tiles_n;
@@ -116,8 +120,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   const uint32_t tile0 = a.split > 1u ? blockIdx.x / a.split : blockIdx.x;
   const uint32_t tile_step = a.split > 1u ? gridDim.x / a.split : gridDim.x;
   const uint32_t c0 = a.nchunk * rank / a.split, c1 = a.nchunk * (rank + 1u) / a.split;
-  const uint32_t no_res[16] = {};
-  float part[TN / 2];  // with a split: this thread's sums, over the cluster's barrier
+  uint32_t part[32];  // with a split: this thread's sums, over the cluster's barrier
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -283,37 +286,48 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     }
     __syncwarp();
   } else {
-    const uint32_t q = (uint32_t)warp & 3u, half = (uint32_t)warp >> 2;
-    const uint32_t lane_row = 32u * q + lane;
-    uint32_t tl = 0;
-    for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++tl) {
+    const uint32_t q = (uint32_t)warp & 3u, set = (uint32_t)warp >> 2;
+    constexpr uint32_t kTurns = kEpiWarps / S::kDrain;  // sets of warps that take the tiles in turn
+    const uint32_t turn = kTurns == 2 ? set >> 1 : 0u;
+    const uint32_t first = (kTurns == 2 ? set & 1u : set) * (32u * S::kPatches);  // channel of the tile
+    Patch p;
+    p.own = p.lane = lane;
+    p.stage = s0 + S::kRing + (uint32_t)warp * kStageBytes;
+    p.rows = n;
+    uint32_t tl = turn;
+    for (uint32_t tile = tile0 + turn * tile_step; tile < tiles; tile += kTurns * tile_step, tl += kTurns) {
       const uint32_t buf = S::kBuffers == 1 ? 0u : tl & 1u, use = S::kBuffers == 1 ? tl : tl >> 1;
+      p.row0 = (uint64_t)(tile / tiles_n) * kTileM + 32u * q;
+      const uint32_t col = (tile % tiles_n) * TN + first;
+      float bias[S::kPatches];
+#pragma unroll
+      for (uint32_t g = 0; g < S::kPatches; ++g) {
+        p.col = col + 32u * g;
+        bias[g] = load_bias(a.o, p);
+      }
       uint32_t ok = 1u;
       if (lane == 0) ok = mbar_wait(bar_tfull + 8 * buf, use & 1u, abort_flag, a.status, 25u) ? 1u : 0u;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
-      const uint64_t row = (uint64_t)(tile / tiles_n) * kTileM + lane_row;
-      const uint32_t col0 = (tile % tiles_n) * TN + half * (TN / 2u);
-      const uint32_t taddr = tmem + ((32u * q) << 16) + buf * TN + half * (TN / 2u);
+      uint32_t v[S::kPatches][32];
 #pragma unroll
-      for (uint32_t g = 0; g < TN / 64u; ++g) {
-        uint32_t v[32];
-        tmem_ld32(taddr + 32u * g, v);
-        tmem_ld_wait();
-        if (g + 1u == TN / 64u) {  // no more reads of this accumulator by this warp
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
-        }
-        if (TN == 64 && a.split > 1u) {
+      for (uint32_t g = 0; g < S::kPatches; ++g)
+        tmem_ld32(tmem + ((32u * q) << 16) + buf * TN + first + 32u * g, v[g]);
+      tmem_ld_wait();
+      tc_fence_before();  // no more reads of this accumulator by this warp
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+      if (TN == 64 && a.split > 1u) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) part[i] = __uint_as_float(v[i]);
-        } else if (row < n && col0 + 32u * g < ((a.o.cout + 63u) & ~63u)) {
-          float y[32];
+        for (int i = 0; i < 32; ++i) part[i] = v[0][i];
+      } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(v[i]);
-          emit32<false>(a.o, y, row, col0 + 32u * g, no_res);
+        for (uint32_t g = 0; g < S::kPatches; ++g) {
+          p.col = col + 32u * g;
+          __syncwarp();  // the bias before is read
+          stage_bias(p, bias[g]);
+          if (p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false>(a.o, v[g], p);
         }
       }
     }
@@ -322,26 +336,33 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   // A split's sums: every CTA but the first leaves its part in its own shared memory (no copy into it is in flight:
   // the MMAs have read all there was), the first adds them up in the order of the ranks.
   if (TN == 64 && a.split > 1u) {
-    const bool epi = warp < kEpiWarps && tile0 < tiles;
+    const bool epi = warp < (int)S::kDrain && tile0 < tiles;
     const uint32_t q = (uint32_t)warp & 3u, half = (uint32_t)warp >> 2, lane_row = 32u * q + lane;
-    const uint64_t row = (uint64_t)(tile0 / tiles_n) * kTileM + lane_row;
-    if (epi && rank != 0u && row < n) {
+    Patch p;
+    p.row0 = (uint64_t)(tile0 / tiles_n) * kTileM + 32u * q;
+    p.rows = n;
+    p.col = (tile0 % tiles_n) * TN + half * 32u;
+    p.own = p.lane = lane;
+    p.stage = s0 + S::kRing + (uint32_t)warp * kStageBytes;
+    const bool live = epi && p.row0 + lane < n;
+    if (epi && rank == 0u) stage_bias(p, load_bias(a.o, p));
+    if (live && rank != 0u) {
 #pragma unroll
-      for (uint32_t i = 0; i < 32u; ++i)
-        ((float*)smem)[(half * 32u + i) * kTileM + lane_row] = part[i];
+      for (uint32_t i = 0; i < 32u; ++i) ((uint32_t*)smem)[(half * 32u + i) * kTileM + lane_row] = part[i];
     }
     __syncwarp();
     cluster_sync();
-    if (epi && rank == 0u && row < n) {
-      for (uint32_t p = 1; p < a.split; ++p) {
+    if (rank == 0u) {
+      if (live) {
+        for (uint32_t r = 1; r < a.split; ++r) {
 #pragma unroll
-        for (uint32_t i = 0; i < 32u; ++i)
-          part[i] += ld_peer(s0 + ((half * 32u + i) * kTileM + lane_row) * 4u, p);
+          for (uint32_t i = 0; i < 32u; ++i)
+            part[i] = __float_as_uint(__uint_as_float(part[i]) +
+                                      ld_peer(s0 + ((half * 32u + i) * kTileM + lane_row) * 4u, r));
+        }
       }
-      float y[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) y[i] = part[i];
-      emit32<false>(a.o, y, row, (tile0 % tiles_n) * TN + half * 32u, no_res);
+      __syncwarp();
+      if (epi && p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false>(a.o, part, p);
     }
     __syncwarp();
     cluster_sync();  // nobody leaves while its part is read
