@@ -71,13 +71,29 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays one
   return m;
 }
 
+// Two sums at a time: a * b + c, each rounded once.
+__device__ __forceinline__ void fma2(uint32_t& x, uint32_t& y, float b, uint32_t c0, uint32_t c1) {
+  asm("{\n\t.reg .b64 v, w, u;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %2};\n\tmov.b64 u, {%3, %4};\n\t"
+      "fma.rn.f32x2 v, v, w, u;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+r"(x), "+r"(y)
+      : "f"(b), "r"(c0), "r"(c1));
+}
+__device__ __forceinline__ uint32_t halves_of(uint32_t x, uint32_t y) {
+  const __half2 h = __floats2half2_rn(__uint_as_float(x), __uint_as_float(y));
+  return *(const uint32_t*)&h;
+}
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+
 // Sums of 32 channels of this lane's row to results in memory: alpha, bias, activation, residual, fp16 or 4 bits.
 // `col` is a multiple of 32 below cout rounded up to 64.
 template <bool RES>
 __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const Patch& p) {
   const uint64_t row = p.row0 + p.own;
   const bool live = row < p.rows, wide = o.access >= 16;
-  const float lo = o.act == SPCONVB_ACT_RELU ? 0.f : -INFINITY, lo2 = o.res_relu ? 0.f : -INFINITY;
   if (RES && wide) cp_async_wait_all();
   __syncwarp();  // residual and bias are there, and what was there is read
   // step by step over all 32 channels, so that the loads of a step are in flight together
@@ -86,62 +102,78 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
 #pragma unroll
     for (int i = 0; i < 8; ++i) b[i] = ld_shared16(p.stage + 2048u + 16u * i);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const uint32_t w = i % 4 == 0 ? b[i / 4].x : (i % 4 == 1 ? b[i / 4].y : (i % 4 == 2 ? b[i / 4].z : b[i / 4].w));
-      v[i] = __float_as_uint(max_nan(fmaf(__uint_as_float(v[i]), o.alpha, __uint_as_float(w)), lo));
+    for (int i = 0; i < 8; ++i) {
+      fma2(v[4 * i], v[4 * i + 1], o.alpha, b[i].x, b[i].y);
+      fma2(v[4 * i + 2], v[4 * i + 3], o.alpha, b[i].z, b[i].w);
     }
   }
-  if (RES) {
-    uint32_t r[16];
-    if (wide) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint4 t = ld_shared16(p.stage + staged_at(p.own, c));
-        r[4 * c] = t.x; r[4 * c + 1] = t.y; r[4 * c + 2] = t.z; r[4 * c + 3] = t.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t at = p.col + 2 * i;
-        const uint16_t* q = (const uint16_t*)o.res + row * o.cout + at;
-        r[i] = live && at < o.cout ? (uint32_t)load_in_order(q) : 0u;
-        if (live && at + 1u < o.cout) r[i] |= (uint32_t)load_in_order(q + 1) << 16;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));  // as it would have been stored
-      const float2 x = __half22float2(h), y = __half22float2(*(const __half2*)&r[i]);
-      v[2 * i] = __float_as_uint(max_nan(__fadd_rn(x.x, y.x), lo2));
-      v[2 * i + 1] = __float_as_uint(max_nan(__fadd_rn(x.y, y.y), lo2));
-    }
-  }
-  if (o.mode == 0) {
+  const bool relu = o.act == SPCONVB_ACT_RELU;
+  if (RES || o.mode == 0) {
+    // fp16 from here on (the sum with a residual is rounded as if it had been stored); ReLU before or after a rounding is the same
     uint32_t h[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const __half2 two = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-      h[i] = *(const uint32_t*)&two;
-    }
-    if (!wide) {
+    for (int i = 0; i < 16; ++i) h[i] = halves_of(v[2 * i], v[2 * i + 1]);
+    if (relu) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (live && p.col + i < o.cout) ((uint16_t*)o.out)[row * o.cout + p.col + i] = (uint16_t)(h[i / 2] >> (16 * (i % 2)));
+      for (int i = 0; i < 16; ++i) h[i] = max_nan2(h[i], 0u);
+    }
+    if (RES) {
+      uint32_t r[16];
+      if (wide) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint4 t = ld_shared16(p.stage + staged_at(p.own, c));
+          r[4 * c] = t.x; r[4 * c + 1] = t.y; r[4 * c + 2] = t.z; r[4 * c + 3] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t at = p.col + 2 * i;
+          const uint16_t* q = (const uint16_t*)o.res + row * o.cout + at;
+          r[i] = live && at < o.cout ? (uint32_t)load_in_order(q) : 0u;
+          if (live && at + 1u < o.cout) r[i] |= (uint32_t)load_in_order(q + 1) << 16;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 x = __half22float2(*(const __half2*)&h[i]), y = __half22float2(*(const __half2*)&r[i]);
+        v[2 * i] = __float_as_uint(__fadd_rn(x.x, y.x));
+        v[2 * i + 1] = __float_as_uint(__fadd_rn(x.y, y.y));
+        if (o.mode == 0) h[i] = halves_of(v[2 * i], v[2 * i + 1]);
+      }
+      if (o.res_relu && o.mode == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) h[i] = max_nan2(h[i], 0u);
+      }
+    }
+    if (o.mode == 0) {
+      if (!wide) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (live && p.col + i < o.cout)
+            ((uint16_t*)o.out)[row * o.cout + p.col + i] = (uint16_t)(h[i / 2] >> (16 * (i % 2)));
+        return;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        st_shared16(p.stage + staged_at(p.own, c), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+      __syncwarp();
+      uint4 t[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) t[k] = ld_shared16(p.stage + staged_at(8u * k + p.lane / 4u, p.lane % 4u));
+      const uint32_t c = p.col + 8u * (p.lane % 4u);
+      const uint64_t at = p.row0 + p.lane / 4u;
+      const uint32_t left = c < o.cout && at < p.rows ? (uint32_t)min(p.rows - at, (uint64_t)32u) : 0u;
+      __half* to = (__half*)o.out + at * o.cout + c;
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        if (8u * k < left) *(uint4*)(to + 8u * k * o.cout) = t[k];
       return;
     }
+  }
+  if (RES ? o.res_relu != 0 : relu) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) st_shared16(p.stage + staged_at(p.own, c), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
-    __syncwarp();
-    uint4 t[4];
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) t[k] = ld_shared16(p.stage + staged_at(8u * k + p.lane / 4u, p.lane % 4u));
-    const uint32_t c = p.col + 8u * (p.lane % 4u);
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-      const uint64_t at = p.row0 + 8u * k + p.lane / 4u;
-      if (at < p.rows && c < o.cout) *(uint4*)((__half*)o.out + at * o.cout + c) = t[k];
-    }
-    return;
+    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(max_nan(__uint_as_float(v[i]), 0.f));
   }
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = p.col + i < o.cout ? v[i] : 0u;

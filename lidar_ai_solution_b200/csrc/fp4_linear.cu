@@ -438,8 +438,10 @@ int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream
   const uint64_t tm = (rows + kTileM - 1) / kTileM;
   auto tiles = [&](uint32_t tn) { return tm * ((a.o.cout + tn - 1) / tn); };
   a.split = 1;
-  // the widest tile that still gives every SM one
-  if (a.o.cout > 128u && tiles(256) >= (uint64_t)kSmCount)
+  // The widest tile that still gives every SM one; the widest of all, whose single accumulator is drained with no MMA beside it,
+  // only where the K axis is long enough to make up for that: us, TN 256 / 128: 32 400 x 256 -> 512 14.7 / 13.1,
+  // x 512 15.8 / 14.6, x 1 024 19.0 / 20.0, 8 192 x 4 096 -> 4 096 66.2 / 90.8.
+  if (a.o.cout > 128u && a.nchunk >= 4u && tiles(256) >= (uint64_t)kSmCount)
     return launch_linear<FMT, 256>(a, map, (uint32_t)tiles(256), st);
   if (a.o.cout > 64u && tiles(128) >= (uint64_t)kSmCount)
     return launch_linear<FMT, 128>(a, map, (uint32_t)tiles(128), st);
