@@ -4,8 +4,7 @@
 // 256 channels: 128 bytes of codes a row, which is one swizzle atom, and four MMAs of 64 channels.  Roles of the
 // warps of a CTA (one an SM, walking over tiles):
 //
-//   0-15   epilogue: a lane owns a row, a warp its quadrant of 32 and 32 or 64 channels (with TN = 64 two sets of warps take the
-//          tiles in turn)
+//   0-15   epilogue: a lane owns a row, a warp its quadrant of 32 and 32 or 64 channels
 //   16     allocates tensor memory; copies the chunk's scales there and issues its MMAs
 //   17     one lane: TMA of the rows' codes, bulk copies of the weights' image (codes and scales lie ready in it)
 //   18-21  the rows' scales, a row a lane: four chunks ahead in registers, then as words into the order that the
@@ -14,14 +13,28 @@
 // Scales in tensor memory have a place for every stage of the ring: a stage is filled again only when the MMAs that
 // read its scales are complete, so no copy overwrites scales that are in use.
 //
-// Few rows: the K axis is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
-// always in the same order.
+// TN is 256 or 128.  A tile of 64 channels was slower also for 64 channels (1 row x 256 -> 64 4.3 us, with half of a tile
+// of 128 empty 3.6): it takes as many instructions.  The widest, whose single accumulator is drained with no MMA beside it, is taken
+// where K is long enough to make up for that and every SM has a tile: us, TN 256 / 128: 32 400 x 256 -> 512 14.7 / 13.1, x 512
+// 15.8 / 14.6, x 1 024 19.0 / 20.0, 8 192 x 4 096 -> 4 096 66.2 / 90.8; 200 x 8 192 -> 8 192 28.5 / 17.2.
+//
+// Few tiles and a long K: K is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
+// always in the same order.  That costs 5 us and a chunk takes 0.32, so it begins at 32 chunks (64 rows -> 64 channels, us, split / not:
+// x 4 096 11.3 / 8.6, x 16 384 13.3 / 24.6).
 #include "fp4_epilogue.cuh"
 
 namespace spconvb {
 namespace fp4 {
+
+int linear_few(int format, const void* codes, const void* scales, uint32_t cin, const uint32_t* n_ptr, uint32_t cap,
+               const void* packed, const Output& o, cudaStream_t st);
+
 namespace {
 
+// What goes to the CUDA cores: up to 8 rows, as long as the products are few (us there / here: 1 x 4 096 -> 4 096 5.2 / 8.8, 4 x
+// 4 096 -> 4 096 8.9 / 8.8, 8 x 4 096 -> 512 5.8 / 8.6, 8 x 4 096 -> 4 096 13.9 / 8.8, 1 x 8 192 -> 8 192 12.2 / 15.5).
+constexpr uint32_t kFewRows = 8;
+constexpr uint64_t kFewProducts = 1ull << 26;
 constexpr int kEpiWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kScaleWarp0 = 18;
 constexpr int kCtaThreads = 32 * 22;
 constexpr uint32_t kTileM = 128;
@@ -48,11 +61,10 @@ struct Shape {
   static constexpr uint32_t kA = kTileM * 128, kB = TN * 128;
   static constexpr uint32_t kOffB = kA, kOffSfb = kA + kB, kOffSfa = kOffSfb + kBlocks * kSf;
   static constexpr uint32_t kStage = kOffSfa + kSf;  // a multiple of 1024
-  static constexpr uint32_t kStages = TN == 256 ? 3 : (TN == 128 ? 5 : 6);
+  static constexpr uint32_t kStages = TN == 256 ? 3 : 5;
   static constexpr uint32_t kBuffers = TN == 256 ? 1 : 2;  // accumulators
   static constexpr uint32_t kSfCols = kWords * 4 * (1 + kBlocks);
   static constexpr uint32_t kPatches = TN == 256 ? 2 : 1;            // of 32 channels a warp
-  static constexpr uint32_t kDrain = TN == 64 ? 8 : 16;             // warps that drain a tile
   static constexpr uint32_t kRing = kStages * kStage;
   static constexpr uint32_t kSmem = kRing + kEpiWarps * kStageBytes + 1024 + 512;
   static_assert(kStage % 1024 == 0, "stages start on swizzle atoms");
@@ -71,7 +83,8 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <int FMT, int TN>
+// SPLIT: the CTAs of a cluster share a tile's K (a kernel of its own: the sums kept for it would be spilled in the other).
+template <int FMT, int TN, bool SPLIT>
 __global__ void __launch_bounds__(kCtaThreads, 1)
 fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_map) {
   using S = Shape<FMT, TN>;
@@ -94,7 +107,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     mbar_init(bar_empty + 8 * threadIdx.x, 1);
     if (threadIdx.x < 2) {
       mbar_init(bar_tfull + 8 * threadIdx.x, 1);
-      mbar_init(bar_tempty + 8 * threadIdx.x, S::kDrain);
+      mbar_init(bar_tempty + 8 * threadIdx.x, kEpiWarps);
     }
     if (threadIdx.x == 0) *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -116,10 +129,11 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   const uint32_t tiles_n = (a.o.cout + TN - 1) / TN;
   const uint32_t tiles = ((n + kTileM - 1) / kTileM) * tiles_n;
   // this CTA's tiles and its part of K
-  const uint32_t rank = a.split > 1u ? blockIdx.x % a.split : 0u;
-  const uint32_t tile0 = a.split > 1u ? blockIdx.x / a.split : blockIdx.x;
-  const uint32_t tile_step = a.split > 1u ? gridDim.x / a.split : gridDim.x;
-  const uint32_t c0 = a.nchunk * rank / a.split, c1 = a.nchunk * (rank + 1u) / a.split;
+  const uint32_t split = SPLIT ? a.split : 1u;
+  const uint32_t rank = SPLIT ? blockIdx.x % split : 0u;
+  const uint32_t tile0 = SPLIT ? blockIdx.x / split : blockIdx.x;
+  const uint32_t tile_step = SPLIT ? gridDim.x / split : gridDim.x;
+  const uint32_t c0 = a.nchunk * rank / split, c1 = a.nchunk * (rank + 1u) / split;
   uint32_t part[32];  // with a split: this thread's sums, over the cluster's barrier
 
   if (warp == kLoadWarp) {
@@ -148,15 +162,10 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
               bulk_g2s(st + S::kOffB + 128u * 128u, w2, 128u * 128u, bar);
               bulk_g2s(st + S::kOffSfb + S::kSf, w2 + 128u * 128u, S::kSf, bar);
             }
-          } else if (TN == 128) {
-            mbar_expect_tx(bar, S::kA + S::kB + S::kSf);
-            tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
-            bulk_g2s(st + S::kOffB, w, S::kB + S::kSf, bar);
           } else {
             mbar_expect_tx(bar, S::kA + S::kB + S::kSf);
             tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
-            bulk_g2s(st + S::kOffB, w + (tn * TN % 128u) * 128u, S::kB, bar);
-            bulk_g2s(st + S::kOffSfb, w + 128u * 128u, S::kSf, bar);
+            bulk_g2s(st + S::kOffB, w, S::kB + S::kSf, bar);
           }
           if (++s == S::kStages) {
             s = 0;
@@ -245,8 +254,6 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
       __syncwarp();
       tc_fence_after();
       const uint32_t d_tmem = tmem + buf * TN;
-      // TN = 64: the tile's channels are the lower or the upper half of the block's
-      const uint32_t sfb_off = TN == 64 ? (tile % tiles_n % 2u) * 2u : 0u;
       uint32_t accumulate = 0u;
       for (uint32_t c = c0; c < c1; ++c) {
         alive = alive && (mbar_test_wait(bar_full + 8 * s, ph) ||
@@ -273,7 +280,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
           const uint32_t w = k / kPer;
           umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, a_lo + 2u * k, b_lo + 2u * k, desc_hi,
                               idesc_of<FMT>(TN, (k % kPer) * 2u), sfa + 4u * w,
-                              sfb + 4u * w * S::kBlocks + sfb_off, k == 0 ? accumulate : 1u);
+                              sfb + 4u * w * S::kBlocks, k == 0 ? accumulate : 1u);
         }
         accumulate = 1u;
         tc_commit_if(issue, bar_empty + 8 * s);
@@ -287,15 +294,13 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     __syncwarp();
   } else {
     const uint32_t q = (uint32_t)warp & 3u, set = (uint32_t)warp >> 2;
-    constexpr uint32_t kTurns = kEpiWarps / S::kDrain;  // sets of warps that take the tiles in turn
-    const uint32_t turn = kTurns == 2 ? set >> 1 : 0u;
-    const uint32_t first = (kTurns == 2 ? set & 1u : set) * (32u * S::kPatches);  // channel of the tile
+    const uint32_t first = set * (32u * S::kPatches);  // channel of the tile
     Patch p;
     p.own = p.lane = lane;
     p.stage = s0 + S::kRing + (uint32_t)warp * kStageBytes;
     p.rows = n;
-    uint32_t tl = turn;
-    for (uint32_t tile = tile0 + turn * tile_step; tile < tiles; tile += kTurns * tile_step, tl += kTurns) {
+    uint32_t tl = 0;
+    for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++tl) {
       const uint32_t buf = S::kBuffers == 1 ? 0u : tl & 1u, use = S::kBuffers == 1 ? tl : tl >> 1;
       p.row0 = (uint64_t)(tile / tiles_n) * kTileM + 32u * q;
       const uint32_t col = (tile % tiles_n) * TN + first;
@@ -318,7 +323,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
       tc_fence_before();  // no more reads of this accumulator by this warp
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
-      if (TN == 64 && a.split > 1u) {
+      if (SPLIT) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) part[i] = v[0][i];
       } else {
@@ -335,30 +340,30 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
 
   // A split's sums: every CTA but the first leaves its part in its own shared memory (no copy into it is in flight:
   // the MMAs have read all there was), the first adds them up in the order of the ranks.
-  if (TN == 64 && a.split > 1u) {
-    const bool epi = warp < (int)S::kDrain && tile0 < tiles;
-    const uint32_t q = (uint32_t)warp & 3u, half = (uint32_t)warp >> 2, lane_row = 32u * q + lane;
+  if (SPLIT) {
+    const bool epi = warp < kEpiWarps && tile0 < tiles;
+    const uint32_t q = (uint32_t)warp & 3u, set = (uint32_t)warp >> 2, lane_row = 32u * q + lane;
     Patch p;
     p.row0 = (uint64_t)(tile0 / tiles_n) * kTileM + 32u * q;
     p.rows = n;
-    p.col = (tile0 % tiles_n) * TN + half * 32u;
+    p.col = (tile0 % tiles_n) * TN + set * 32u;
     p.own = p.lane = lane;
     p.stage = s0 + S::kRing + (uint32_t)warp * kStageBytes;
     const bool live = epi && p.row0 + lane < n;
     if (epi && rank == 0u) stage_bias(p, load_bias(a.o, p));
     if (live && rank != 0u) {
 #pragma unroll
-      for (uint32_t i = 0; i < 32u; ++i) ((uint32_t*)smem)[(half * 32u + i) * kTileM + lane_row] = part[i];
+      for (uint32_t i = 0; i < 32u; ++i) ((uint32_t*)smem)[(set * 32u + i) * kTileM + lane_row] = part[i];
     }
     __syncwarp();
     cluster_sync();
     if (rank == 0u) {
       if (live) {
-        for (uint32_t r = 1; r < a.split; ++r) {
+        for (uint32_t r = 1; r < split; ++r) {
 #pragma unroll
           for (uint32_t i = 0; i < 32u; ++i)
             part[i] = __float_as_uint(__uint_as_float(part[i]) +
-                                      ld_peer(s0 + ((half * 32u + i) * kTileM + lane_row) * 4u, r));
+                                      ld_peer(s0 + ((set * 32u + i) * kTileM + lane_row) * 4u, r));
         }
       }
       __syncwarp();
@@ -400,18 +405,18 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-template <int FMT, int TN>
+template <int FMT, int TN, bool SPLIT>
 int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, cudaStream_t st) {
   using S = Shape<FMT, TN>;
   static bool attr_done[64] = {};
   int dev = 0;
   SPCONVB_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    SPCONVB_CUDA_TRY(cudaFuncSetAttribute(fp4_linear_kernel<FMT, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    SPCONVB_CUDA_TRY(cudaFuncSetAttribute(fp4_linear_kernel<FMT, TN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)S::kSmem));
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
-  if (a.split > 1u) {
+  if (SPLIT) {
     cudaLaunchAttribute at[2] = {};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -425,11 +430,11 @@ int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, c
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    SPCONVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_linear_kernel<FMT, TN>, a, map));
+    SPCONVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_linear_kernel<FMT, TN, SPLIT>, a, map));
     return SPCONVB_OK;
   }
   const uint32_t grid = tiles < (uint32_t)kSmCount ? tiles : (uint32_t)kSmCount;
-  SPCONVB_CUDA_TRY(launch_pdl(fp4_linear_kernel<FMT, TN>, dim3(grid), dim3(kCtaThreads), S::kSmem, st, a, map));
+  SPCONVB_CUDA_TRY(launch_pdl(fp4_linear_kernel<FMT, TN, SPLIT>, dim3(grid), dim3(kCtaThreads), S::kSmem, st, a, map));
   return SPCONVB_OK;
 }
 
@@ -438,21 +443,13 @@ int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream
   const uint64_t tm = (rows + kTileM - 1) / kTileM;
   auto tiles = [&](uint32_t tn) { return tm * ((a.o.cout + tn - 1) / tn); };
   a.split = 1;
-  // The widest tile that still gives every SM one; the widest of all, whose single accumulator is drained with no MMA beside it,
-  // only where the K axis is long enough to make up for that: us, TN 256 / 128: 32 400 x 256 -> 512 14.7 / 13.1,
-  // x 512 15.8 / 14.6, x 1 024 19.0 / 20.0, 8 192 x 4 096 -> 4 096 66.2 / 90.8.
   if (a.o.cout > 128u && a.nchunk >= 4u && tiles(256) >= (uint64_t)kSmCount)
-    return launch_linear<FMT, 256>(a, map, (uint32_t)tiles(256), st);
-  if (a.o.cout > 64u && tiles(128) >= (uint64_t)kSmCount)
-    return launch_linear<FMT, 128>(a, map, (uint32_t)tiles(128), st);
-  const uint64_t t = tiles(64);
-  if (t < (uint64_t)kSmCount) {
-    uint32_t split = (uint32_t)((uint64_t)kSmCount / t);
-    if (split > 8u) split = 8u;
-    if (split > a.nchunk) split = a.nchunk;
-    a.split = split;
-  }
-  return launch_linear<FMT, 64>(a, map, (uint32_t)t, st);
+    return launch_linear<FMT, 256, false>(a, map, (uint32_t)tiles(256), st);
+  const uint64_t t = tiles(128);
+  if (a.nchunk >= 32u)
+    while (a.split < 8u && 2u * a.split * t <= (uint64_t)kSmCount && a.nchunk >= 8u * a.split) a.split *= 2u;
+  return a.split > 1u ? launch_linear<FMT, 128, true>(a, map, (uint32_t)t, st)
+                      : launch_linear<FMT, 128, false>(a, map, (uint32_t)t, st);
 }
 
 }  // namespace
@@ -471,8 +468,10 @@ extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes
     return SPCONVB_E_ARG;
   LinearArgs a{};
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)packed) & 15u || !make_output(*p, bias, out, a.o)) return SPCONVB_E_ARG;
-  if (((uint64_t)launch_rows + kTileM - 1) / kTileM * (((uint64_t)p->cout + 63) / 64) > 0x7fffffffu)
+  if (((uint64_t)launch_rows + kTileM - 1) / kTileM * (((uint64_t)p->cout + 127) / 128) > 0x7fffffffu)
     return SPCONVB_E_RANGE;  // more tiles than a 32-bit number counts
+  if (launch_rows <= kFewRows && (uint64_t)launch_rows * (uint32_t)p->cin * (uint32_t)p->cout <= kFewProducts && !p->out_fp4 && p->wait_test == 0)
+    return linear_few(p->format, codes, scales, (uint32_t)p->cin, n_ptr, launch_rows, packed, a.o, (cudaStream_t)stream);
   const uint32_t cp = cpad((uint32_t)p->cin);
   a.scales = (const uint8_t*)scales;
   a.spitch = scale_pitch(p->format, (uint32_t)p->cin);

@@ -173,7 +173,7 @@ def test_rows_at_any_element(fmt, offset, channels):
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("rows,cin,cout", [
     (1, 64, 64), (1, 1, 1), (3, 16, 8), (128, 64, 64), (127, 256, 64), (129, 320, 65), (50, 200, 136), (300, 72, 130),
-    (1, 4096, 512), (5, 4100, 100), (130, 2048, 256), (1000, 512, 300), (20000, 64, 64), (19000, 192, 128),
+    (1, 4096, 512), (5, 4100, 100), (2, 200, 9), (4, 64, 130), (8, 1000, 264), (9, 300, 72), (64, 16384, 64), (130, 9000, 300), (7, 8200, 1000), (130, 2048, 256), (1000, 512, 300), (20000, 64, 64), (19000, 192, 128),
     (19100, 128, 200), (40000, 256, 256), (5000, 448, 1000)])
 def test_linear(fmt, rows, cin, cout):
     ops = _ops()
