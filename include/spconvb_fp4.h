@@ -13,7 +13,7 @@
  *   SPCONVB_NVFP4  blocks of 16 channels; scale byte e4m3 = amax / (6 * tensor_scale), rounded to nearest even and
  *                  saturated at 448; tensor_scale is one positive fp32 number a tensor.
  *   A block's scale is S = 2^e, or e4m3 * tensor_scale rounded to fp32; its codes are x / S (one fp32 division) rounded
- *   to nearest even and saturated at 6, all 0 where S is 0.  A block that holds an infinity or a NaN gets the NaN scale
+ *   to nearest even and saturated at 6, all 0 where S is 0 (the sign of a zero is not specified).  A block that holds an infinity or a NaN gets the NaN scale
  *   (0xff, 0x7f) and codes 0, so that it stays visible: it reads as NaN, and so does every product with it.
  *
  * Layout of rows (all pointers 16-byte aligned)
@@ -78,6 +78,7 @@ typedef struct spconvb_fp4_params {
   const void* res;
   int32_t res_relu;
   int32_t wait_test;      /* 0 in normal use; as in spconvb_conv_params */
+  uint32_t in_rows;       /* rows of `codes` and `scales` (spconvb_fp4_conv only): what the map says beyond them is missing */
 } spconvb_fp4_params;
 
 /* out[r] = act(alpha * W . x[r] + bias), kvol = 1, any cin and cout up to SPCONVB_FP4_MAX_CHANNELS.  bias: fp32 [cout]
@@ -92,7 +93,7 @@ SPCONVB_API int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* code
 SPCONVB_API int spconvb_fp4_conv_supported(int32_t cin, int32_t cout, int32_t kvol);
 
 /* out[o] = act(alpha * sum_k W[:, k, :] . in[map[k * cap + o]] + bias), then the residual.  map, cap, n_out_ptr and
- * launch_rows as in spconvb_conv_forward. */
+ * launch_rows as in spconvb_conv_forward; an entry of the map that is not below in_rows is a missing neighbour. */
 SPCONVB_API int spconvb_fp4_conv(const spconvb_fp4_params* p, const void* codes, const void* scales,
                                  const int32_t* map, uint32_t cap, const uint32_t* n_out_ptr,
                                  uint32_t launch_rows, const void* packed, const float* bias,

@@ -42,7 +42,7 @@ class Fp4Params(C.Structure):
         ("format", C.c_int32), ("cin", C.c_int32), ("cout", C.c_int32), ("kvol", C.c_int32),
         ("alpha", C.c_float), ("act", C.c_int32), ("out_fp4", C.c_int32), ("out_format", C.c_int32),
         ("out_tensor_scale", C.c_float), ("out_scales", C.c_void_p), ("res", C.c_void_p),
-        ("res_relu", C.c_int32), ("wait_test", C.c_int32),
+        ("res_relu", C.c_int32), ("wait_test", C.c_int32), ("in_rows", C.c_uint32),
     ]
 
 

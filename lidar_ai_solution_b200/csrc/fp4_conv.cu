@@ -36,7 +36,7 @@ struct ConvArgs {
   const uint8_t* codes;
   const uint8_t* scales;
   const int32_t* map;
-  uint32_t cap;
+  uint32_t cap, in_rows;
   const uint32_t* n_out_ptr;
   const uint8_t* wpk;
   uint32_t* status;
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
           const int32_t sr = idx[i];
           const uint32_t r = 4u * (i & 1u) + slot;  // row of its group of 8
           cp_async16(stage + (pw * 4u + (i >> 1)) * 1024u + r * 128u + ((seg ^ r) << 4), src + (int64_t)sr * RB,
-                     sr < 0 ? 0u : 16u);
+                     (uint32_t)sr < a.in_rows ? 16u : 0u);
         }
       }
       // (taps past the last one have indices -1, and zeros for scales)
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
         int32_t sr = idx[kParts * i];
 #pragma unroll
         for (uint32_t p = 1; p < kParts; ++p) sr = part == p ? idx[kParts * i + p] : sr;
-        cp_async4(stage + sf_dst + (kParts * i + part) * 64u, src + (int64_t)sr * kPitch, sr < 0 ? 0u : 4u);
+        cp_async4(stage + sf_dst + (kParts * i + part) * 64u, src + (int64_t)sr * kPitch, (uint32_t)sr < a.in_rows ? 4u : 0u);
       }
       if (!(a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) cp_async_arrive_noinc(bar_full + 8 * s);
       load_idx(ntile, nj, idx);
@@ -401,7 +401,8 @@ int spconvb_fp4_conv_supported(int32_t cin, int32_t cout, int32_t kvol) {
 int spconvb_fp4_conv(const spconvb_fp4_params* p, const void* codes, const void* scales, const int32_t* map, uint32_t cap,
                      const uint32_t* n_out_ptr, uint32_t launch_rows, const void* packed, const float* bias, void* out,
                      uint32_t* status, void* stream) {
-  if (!p || !codes || !scales || !map || !n_out_ptr || !packed || !out || cap < 1 || cap > 0x7fffff00u)
+  if (!p || !codes || !scales || !map || !n_out_ptr || !packed || !out || cap < 1 || cap > 0x7fffff00u || p->in_rows < 1 ||
+      p->in_rows > 0x80000000u)
     return SPCONVB_E_ARG;
   if (!format_ok(p->format) || !channels_ok(p->cin) || !channels_ok(p->cout) || p->kvol < 1) return SPCONVB_E_ARG;
   ConvArgs a{};
@@ -413,6 +414,7 @@ int spconvb_fp4_conv(const spconvb_fp4_params* p, const void* codes, const void*
   a.scales = (const uint8_t*)scales;
   a.map = map;
   a.cap = cap;
+  a.in_rows = p->in_rows;
   a.n_out_ptr = n_out_ptr;
   a.wpk = (const uint8_t*)packed;
   a.status = status;

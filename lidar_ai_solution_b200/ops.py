@@ -17,6 +17,7 @@ from .cabi import ACT_NONE, ACT_RELU, F16, F32, I8, MXFP4, NVFP4  # noqa: F401
 
 # torch's own way to the current stream's handle, a microsecond cheaper a call; not a public one
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream():
@@ -293,7 +294,7 @@ def _fp4_device(t, count, *others):
     """The index of a tensor's device, which has to be the current one (the library enqueues there) and that of the row
     count (int32) and of the others."""
     dev = t.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != _current_device():
         raise ValueError("a tensor on %s where the current CUDA device's is wanted" % t.device)
     if count.dtype != torch.int32 or count.get_device() != dev or not count.numel():
         raise ValueError("a row count is an int32 on the rows' device (device_count)")
@@ -327,11 +328,8 @@ class Fp4Rows:
         if codes.device != scales.device:
             raise ValueError("codes and scales of different devices")
         self._hold = codes, scales
-        self._set(channels, fmt, tensor_scale, codes.get_device(), codes.data_ptr(), scales.data_ptr())
-
-    def _set(self, channels, fmt, tensor_scale, dev, codes_ptr, scales_ptr):
         self.channels, self.fmt, self.tensor_scale = channels, fmt, float(tensor_scale)
-        self.device_index, self.codes_ptr, self.scales_ptr = dev, codes_ptr, scales_ptr
+        self.device_index, self.codes_ptr, self.scales_ptr = codes.get_device(), codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def empty(cls, rows, channels, fmt, tensor_scale=1.0, device="cuda"):
@@ -343,10 +341,10 @@ class Fp4Rows:
         """Uninitialised rows on t's device: one buffer, of which ``codes`` and ``scales`` are made when asked for."""
         q = cls.__new__(cls)
         cp, sp = q._pitches = _fp4_pitches(fmt, channels)
-        q.rows = rows
         q._hold = buf = t.new_empty(rows * (cp + sp), dtype=torch.uint8)
-        at = buf.data_ptr()
-        q._set(channels, fmt, tensor_scale, buf.get_device(), at, at + rows * cp)
+        q.codes_ptr = at = buf.data_ptr()
+        q.scales_ptr = at + rows * cp
+        q.rows, q.channels, q.fmt, q.tensor_scale, q.device_index = rows, channels, fmt, float(tensor_scale), buf.get_device()
         return q
 
     @property
@@ -499,6 +497,7 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     if res is not None:
         _fp4_tensor(res, torch.float16, cap, wts.cout, "res")
         p.res, p.res_relu = res.data_ptr(), res_relu
+    p.in_rows = q.rows
     if wait_test:
         p.wait_test = wait_test
     if cap:

@@ -81,7 +81,7 @@ def test_refusals_of_products():
 
     def params(**kw):
         p = cabi.Fp4Params()
-        p.format, p.cin, p.cout, p.kvol, p.alpha = 0, 64, 64, 1, 1.0
+        p.format, p.cin, p.cout, p.kvol, p.alpha, p.in_rows = 0, 64, 64, 1, 1.0, 10
         for k, v in kw.items():
             setattr(p, k, v)
         return C.byref(p)
@@ -102,7 +102,7 @@ def test_refusals_of_products():
         assert f(out_fp4=1, out_scales=FAKE, out_format=1, out_tensor_scale=1.0, out=FAKE + 8) == -1
     assert linear(kvol=2) == linear(rows=0) == linear(rows=0x7fffffff) == linear(res=FAKE) == -1
     assert linear(cout=65536, rows=0x7fffff00) == -2                               # more tiles than a grid has
-    assert conv(m=None) == conv(m=FAKE + 2) == conv(cap=0) == conv(cap=0x80000000) == conv(res=FAKE + 1) == -1
+    assert conv(m=None) == conv(m=FAKE + 2) == conv(cap=0) == conv(cap=0x80000000) == conv(res=FAKE + 1) == conv(in_rows=0) == -1
     assert conv(cin=192) == conv(cout=129) == conv(kvol=28) == -5
 
 

@@ -358,3 +358,263 @@ def test_strided_conv_reads_other_rows_than_it_writes(fmt):
     got = ops.fp4_conv(q, m, n_out, wq)[:count].cpu().numpy().astype(np.float64)
     y, off = ref.product(_gather(xv, m.cpu().numpy()[:, :count]), wv, alpha, bias, False)
     assert (np.abs(got - y) <= off).all() and count > 100
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_conv_takes_rows_beyond_the_input_as_missing(fmt):
+    """Entries of the map that no row of the input has: nothing is read for them."""
+    ops = _ops()
+    n_in, n = 300, 900
+    q, xv, wq, wv, alpha, bias = _conv_problem(fmt, n_in, 64, 64, 27)
+    m = _map(n, 27, 5, n_in=n_in)
+    rng = np.random.default_rng(1)
+    bad = m.copy()
+    bad[rng.random(m.shape) < 0.2] = rng.choice([n_in, n_in + 1, 2 ** 31 - 1, -2, -2 ** 31])
+    bad[0, :4] = (n_in, 2 ** 31 - 1, -2 ** 31, -7)
+    clean = np.where((bad < 0) | (bad >= n_in), -1, bad)
+    y, off = ref.product(_gather(xv, clean), wv, alpha, bias, False)
+    got = ops.fp4_conv(q, _dev(bad), ops.device_count(n), wq).cpu().numpy().astype(np.float64)
+    assert (np.abs(got - y) <= off).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_residual_may_be_the_output(fmt):
+    ops = _ops()
+    n = 3001
+    q, xv, wq, wv, alpha, bias = _conv_problem(fmt, n, 64, 104, 27)
+    m, n_ptr = _dev(_map(n, 27, 5)), ops.device_count(n)
+    res = torch.randn(n, 104, device="cuda").half()
+    want = ops.fp4_conv(q, m, n_ptr, wq, res=res, res_relu=True)
+    ops.fp4_conv(q, m, n_ptr, wq, res=res, res_relu=True, out=res)
+    assert torch.equal(res, want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_weights_quantised_elsewhere(fmt):
+    """Codes and scales of the weights that the caller has, and arrays in fp16."""
+    ops = _ops()
+    cout, kvol, cin = 72, 27, 100
+    w = (_features(cout * kvol, cin, 1, 0.3) / 50).astype(np.float16)
+    g = _scale(w.astype(np.float32), fmt)
+    codes, scales = ref.quantize(w.astype(np.float32), fmt, g)
+    rows = ops.Fp4Rows(_dev(codes), _dev(scales), cin, fmt, g)
+    given = ops.Fp4Weights((cout, kvol, cin), fmt, g, rows=rows)
+    made = ops.Fp4Weights(w.reshape(cout, kvol, cin), fmt, g)
+    q, _ = _quantized(_features(500, cin, 2), fmt, 1.0)
+    m, n = _dev(_map(500, kvol, 3)), ops.device_count(500)
+    assert torch.equal(ops.fp4_conv(q, m, n, given), ops.fp4_conv(q, m, n, made))
+    with pytest.raises(ValueError):
+        ops.Fp4Weights((cout, kvol, cin + 1), fmt, g, rows=rows)
+    with pytest.raises(ValueError):
+        ops.Fp4Weights(w.reshape(cout, kvol, cin), fmt, g, bias=np.zeros(cout + 1))
+
+
+def test_products_refuse_what_does_not_fit():
+    ops = _ops()
+    q, _ = _quantized(_features(8, 64, 1), ref.NV, 0.01)
+    n = ops.device_count(8)
+    wq = ops.Fp4Weights(_features(24, 64, 2), ref.NV, 0.01)
+    other = ops.Fp4Weights(_features(24, 64, 2), ref.MX)
+    wide = ops.Fp4Weights(_features(24, 128, 2), ref.NV, 0.01)
+    m = torch.zeros((1, 8), dtype=torch.int32, device="cuda")
+    for bad in (other, wide):
+        with pytest.raises(ValueError):
+            ops.fp4_linear(q, n, bad)
+    for kw in (dict(out=torch.empty(8, 25, dtype=torch.float16, device="cuda")),
+               dict(out=torch.empty(8, 24, device="cuda")), dict(out=torch.empty(8, 24, dtype=torch.float16)),
+               dict(out_fmt=ref.MX, out=ops.Fp4Rows.empty(8, 24, ref.NV)), dict(status=torch.zeros(4, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            ops.fp4_linear(q, n, wq, **kw)
+    with pytest.raises(ValueError):
+        ops.fp4_linear(q, torch.tensor([8], dtype=torch.int32), wq)
+    with pytest.raises(ValueError):
+        ops.fp4_conv(q, m.long(), n, wq)
+    with pytest.raises(ValueError):
+        ops.fp4_conv(q, m, n, wq, res=torch.zeros(8, 25, dtype=torch.float16, device="cuda"))
+    with pytest.raises(RuntimeError):        # a tensor scale for MXFP4
+        ops.fp4_quantize(torch.zeros(4, 64, device="cuda"), n, ref.MX, 2.0)
+    w192 = ops.Fp4Weights(_features(24, 192, 2), ref.NV, 0.01)
+    q192, _ = _quantized(_features(8, 192, 1), ref.NV, 0.01)
+    with pytest.raises(RuntimeError):        # rows of 96 bytes: the convolution does not take them
+        ops.fp4_conv(q192, m, n, w192)
+    assert ops.fp4_quantize(torch.zeros(0, 64, device="cuda"), n, ref.NV).codes.shape == (0, 32)
+
+
+def _chain(ops, x, n, m, ws, fmt, g):
+    """How they are used together: rows to 4 bits, a residual block, a pointwise layer, back to fp16."""
+    q = ops.fp4_quantize(x, n, fmt, g[0])
+    h = ops.fp4_conv(q, m, n, ws[0], act=ops.ACT_RELU, out_fmt=fmt, out_tensor_scale=g[1])
+    y = ops.fp4_conv(h, m, n, ws[1], res=x, res_relu=True)
+    p = ops.fp4_linear(ops.fp4_quantize(y, n, fmt, g[2]), n, ws[2], out_fmt=fmt, out_tensor_scale=g[3])
+    return h, y, ops.fp4_dequantize(p, n)
+
+
+def _chain_problem(fmt, n, c, seed):
+    ops = _ops()
+    x = _features(n, c, seed, 0.2).astype(np.float16)
+    g = [_scale(x.astype(np.float32), fmt)] + [1.0 if fmt == ref.MX else 0.004] * 3
+    w = [_features(c * 27, c, 2, 0.3).reshape(c, 27, c) / 20, _features(c * 27, c, 3, 0.3).reshape(c, 27, c) / 20,
+         _features(200, c, 4, 0.3) / 8]
+    gw = [_scale(v, fmt) for v in w]
+    rng = np.random.default_rng(5)
+    bias = [rng.standard_normal(v.shape[0]).astype(np.float32) for v in w]
+    ws = [ops.Fp4Weights(v, fmt, s, b) for v, s, b in zip(w, gw, bias)]
+    wv = [ref.values(*ref.quantize(v.reshape(-1, c), fmt, s), fmt, c).reshape(v.shape[0], -1)
+          for v, s in zip(w, gw)]
+    return x, _map(n, 27, seed + 7, 0.2), ws, wv, g, gw, bias
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("n,c", [(2500, 64), (700, 128)])
+def test_a_run_of_them_together(fmt, n, c):
+    """Each stage against 64 bits on what the stage before left (a code that lies on a border may fall either way)."""
+    ops = _ops()
+    x, m, ws, wv, g, gw, bias = _chain_problem(fmt, n, c, 0)
+    h, y, z = _chain(ops, _dev(x), ops.device_count(n), _dev(m), ws, fmt, g)
+    xq = ref.values(*ref.quantize(x.astype(np.float32), fmt, g[0]), fmt, c)
+    y1, off1 = ref.product(_gather(xq, m), wv[0], float(np.float32(g[0] * gw[0])), bias[0], True)
+    codes, scales = ref.quantize(y1.astype(np.float32), fmt, g[1])
+    assert (ref.magnitude_codes(h.codes.cpu().numpy()) != ref.magnitude_codes(codes)).mean() < 1e-3
+    assert (h.scales.cpu().numpy() != scales).mean() < 1e-3
+    hv = ref.values(h.codes.cpu().numpy(), h.scales.cpu().numpy(), fmt, c)
+    y2, off2 = ref.product(_gather(hv, m), wv[1], float(np.float32(g[1] * gw[1])), bias[1], False,
+                           x.astype(np.float64), True)
+    got = y.cpu().numpy().astype(np.float64)
+    assert (np.abs(got - y2) <= off2).all()
+    yv = ref.values(*ref.quantize(y.cpu().numpy().astype(np.float32), fmt, g[2]), fmt, c)
+    y3, _ = ref.product(yv, wv[2], float(np.float32(g[2] * gw[2])), bias[2], False)
+    codes, scales = ref.quantize(y3.astype(np.float32), fmt, g[3])
+    want = ref.values(codes, scales, fmt, 200, g[3]).astype(np.float32).astype(np.float16)
+    assert (z.cpu().numpy() != want).mean() < 2e-3
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_captured_and_replayed_on_other_inputs_and_counts(fmt):
+    """Two graphs of the same chain, on another stream, replayed beside one another's and with other rows and counts."""
+    ops = _ops()
+    n, c = 1500, 64
+    problems = [_chain_problem(fmt, n, c, s) for s in (0, 1, 2)]
+    ws, g = problems[0][2], problems[0][4]
+    side = torch.cuda.Stream()
+    graphs = []
+    with torch.cuda.stream(side):
+        for k in range(2):
+            x, m, cnt = _dev(problems[k][0]), _dev(problems[k][1]), ops.device_count(n)
+            _chain(ops, x, cnt, m, ws, fmt, g)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = _chain(ops, x, cnt, m, ws, fmt, g)
+            graphs.append((graph, x, m, cnt, out))
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for k, (graph, x, m, cnt, out) in enumerate(graphs):
+            p = problems[k + 1]
+            x.copy_(_dev(p[0]))
+            rows = n if k else 777
+            m.copy_(_dev(np.where(p[1] < rows, p[1], -1)))      # a rulebook points at rows below the count
+            cnt.fill_(rows)
+            torch.cuda.synchronize()
+            graph.replay()
+        torch.cuda.synchronize()
+        for k, (graph, x, m, cnt, out) in enumerate(graphs):
+            rows = int(cnt)
+            want = _chain(ops, x.clone(), cnt, m.clone(), ws, fmt, g)
+            for a, b in zip(out, want):
+                a, b = (v.codes if isinstance(v, ops.Fp4Rows) else v for v in (a, b))
+                assert torch.equal(a[:rows], b[:rows])
+
+
+def test_two_streams_at_once_give_what_one_gives():
+    ops = _ops()
+    problems = [_chain_problem(ref.NV, 2500, 64, s) for s in (0, 1)]
+    args = [(_dev(p[0]), ops.device_count(2500), _dev(p[1]), p[2], ref.NV, p[4]) for p in problems]
+    want = [_chain(ops, *a)[1] for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(_chain(ops, *args[k])[1])
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want[k]) for k in range(2) for v in got[k])
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_bounded_waits_run_out_and_the_context_survives(fmt):
+    """Producers that withhold a stage: the launch ends with the status bit, and the next one is right."""
+    from lidar_ai_solution_b200 import cabi
+    ops = _ops()
+    n = 2000
+    q, xv, wq, wv, alpha, bias = _conv_problem(fmt, n, 64, 64, 27)
+    m, n_ptr = _dev(_map(n, 27, 5)), ops.device_count(n)
+    good = ops.fp4_conv(q, m, n_ptr, wq)
+    lin = ops.Fp4Weights(_features(64, 64, 3), fmt, 1.0)
+    tall = ops.Fp4Weights(_features(64, 16384, 3), fmt, 1.0)
+    qt, _ = _quantized(_features(40, 16384, 4, 0.1), fmt, 1.0)
+    nt = ops.device_count(40)
+    good_lin, good_tall = ops.fp4_linear(q, n_ptr, lin), ops.fp4_linear(qt, nt, tall)
+    for call in (lambda st, w: ops.fp4_conv(q, m, n_ptr, wq, status=st, wait_test=w),
+                 lambda st, w: ops.fp4_linear(q, n_ptr, lin, status=st, wait_test=w),
+                 lambda st, w: ops.fp4_linear(qt, nt, tall, status=st, wait_test=w)):
+        st = ops.new_status()
+        call(st, 1)
+        torch.cuda.synchronize()
+        assert int(st[0]) == cabi.ST_TIMEOUT
+    st = ops.new_status()
+    assert torch.equal(ops.fp4_conv(q, m, n_ptr, wq, status=st), good)
+    assert torch.equal(ops.fp4_linear(q, n_ptr, lin, status=st), good_lin)
+    assert torch.equal(ops.fp4_linear(qt, nt, tall, status=st), good_tall)
+    assert int(st[0]) == 0
+
+
+def test_the_same_call_gives_the_same_bits():
+    ops = _ops()
+    q, xv, wq, wv, alpha, bias = _conv_problem(ref.NV, 9000, 128, 128, 27)
+    m, n_ptr = _dev(_map(9000, 27, 5)), ops.device_count(9000)
+    first = ops.fp4_conv(q, m, n_ptr, wq)
+    w = ops.Fp4Weights(_features(300, 9000, 2, 0.1), ref.MX)
+    qx, _ = _quantized(_features(100, 9000, 3, 0.1), ref.MX, 1.0)
+    n2 = ops.device_count(100)
+    second = ops.fp4_linear(qx, n2, w)
+    for _ in range(10):
+        assert torch.equal(ops.fp4_conv(q, m, n_ptr, wq), first)
+        assert torch.equal(ops.fp4_linear(qx, n2, w), second)
+
+
+def test_offsets_beyond_32_bits():
+    """140 M rows: codes, scales and fp16 rows whose last ones lie beyond 2^32 bytes."""
+    ops = _ops()
+    rows, ch = 140_000_000, 64
+    x = torch.zeros((rows, ch), dtype=torch.int8, device="cuda")
+    at = torch.tensor([0, 1, 67_108_863, 67_108_864, 134_217_728, rows - 2, rows - 1], device="cuda")
+    piece = torch.randint(-127, 128, (len(at), ch), device="cuda").to(torch.int8)
+    x[at] = piece
+    g, s = 0.0009765625, 0.0078125
+    n = ops.device_count(rows)
+    q = ops.fp4_quantize(x, n, ref.NV, g, in_scale=s)
+    want = ref.quantize(piece.cpu().numpy().astype(np.float32) * np.float32(s), ref.NV, g)
+    codes, scales = q.codes[at].cpu().numpy(), q.scales[at].cpu().numpy()
+    assert np.array_equal(scales, want[1])
+    assert np.array_equal(ref.magnitude_codes(codes), ref.magnitude_codes(want[0]))
+    del x
+    w = _features(8, ch, 2)
+    wq = ops.Fp4Weights(w, ref.NV, 0.01)
+    y = ops.fp4_linear(q, n, wq)[at].cpu().numpy().astype(np.float64)
+    wv = ref.values(*ref.quantize(w, ref.NV, 0.01), ref.NV, ch)
+    full, off = ref.product(ref.values(*want, ref.NV, ch), wv, float(np.float32(g * 0.01)), None, False)
+    assert (np.abs(y - full) <= off).all()
+    back = ops.fp4_dequantize(q, n)
+    exact = ref.values(*want, ref.NV, ch, g).astype(np.float32).astype(np.float16)
+    assert np.array_equal(back[at].cpu().numpy(), exact)
+    # a convolution that reads the far ones
+    m = at.to(torch.int32).repeat(3, 1).contiguous()
+    m[1] = -1
+    cw = ops.Fp4Weights(_features(24, ch, 4).reshape(8, 3, ch), ref.NV, 0.01)
+    got = ops.fp4_conv(q, m, ops.device_count(len(at)), cw).cpu().numpy().astype(np.float64)
+    cv = ref.values(*ref.quantize(_features(24, ch, 4), ref.NV, 0.01), ref.NV, ch).reshape(8, -1)
+    mm = np.tile(np.arange(len(at)), (3, 1))
+    mm[1] = -1
+    y, off = ref.product(_gather(ref.values(*want, ref.NV, ch), mm), cv, float(np.float32(g * 0.01)), None, False)
+    assert (np.abs(got - y) <= off).all()
