@@ -25,6 +25,7 @@ namespace {
 constexpr uint32_t kTileRows = 128;
 constexpr int kEpiWarps = 16, kMmaWarp = 16, kWeightWarp = 17, kProdWarp0 = 18;
 constexpr uint32_t kGroups = 2;
+constexpr uint32_t kPair = 2;
 constexpr int kCtaThreads = 32 * (kProdWarp0 + 4 * (int)kGroups);
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kRingBytes = 191 * 1024;
@@ -60,24 +61,27 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   constexpr uint32_t kSteps = 4 / W;               // MMAs a word
   constexpr uint32_t kRecord = 128 * 128 + W * kAtomBytes;          // a chunk in the weights' image
   constexpr uint32_t kWeightBytes = COUT * 128 + W * kAtomBytes;     // and in shared memory
-  constexpr uint32_t kSfOff = kTileRows * 128, kRowStage = kSfOff + W * kAtomBytes;
-  constexpr uint32_t kSfCols = 8 * W;  // of a stage in tensor memory: rows, weights
-  constexpr uint32_t kDrain = COUT / 32 * 4;  // warps that drain a tile
-  static_assert(2 * COUT + kMaxStages * kSfCols <= kTmemCols, "tensor memory");
+  // a stage is kPair chunks: codes, codes, scales, scales
+  constexpr uint32_t kCodes = kTileRows * 128, kSfOff = kPair * kCodes, kRowStage = kSfOff + kPair * W * kAtomBytes;
+  constexpr uint32_t kWeightStage = kPair * kWeightBytes;
+  constexpr uint32_t kSfCols = kPair * 8 * W;  // of a stage in tensor memory: rows, weights, chunk by chunk
+  constexpr uint32_t kDrain = COUT / 32 * 4;   // warps that drain a tile
+  constexpr uint32_t kDeepest = (kTmemCols - 2 * COUT) / kSfCols < kMaxStages ? (kTmemCols - 2 * COUT) / kSfCols : kMaxStages;
 
   const int kbytes = a.kvol * RB;
   const int nchunk = (kbytes + 127) / 128;
+  const int npair = (nchunk + (int)kPair - 1) / (int)kPair;
   const uint32_t last_steps = (uint32_t)((kbytes - (nchunk - 1) * 128) / 32);
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   uint64_t* bars = (uint64_t*)(smem + kRingBytes + kEpiWarps * kStageBytes);
-  uint32_t* tmem_holder = (uint32_t*)(bars + 3 * kMaxStages + 4);
+  uint32_t* tmem_holder = (uint32_t*)(bars + 4 * kMaxStages + 4);
   volatile uint32_t* abort_flag = tmem_holder + 1;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kMaxStages;
   const uint32_t bar_tfull = bar_empty + 8 * kMaxStages, bar_tempty = bar_tfull + 16;
-  const uint32_t bar_weights = bar_tempty + 16;  // of chunks that stay
+  const uint32_t bar_wfull = bar_tempty + 16, bar_wempty = bar_wfull + 8 * kMaxStages;
   // Warp index, row count and tensor-memory address are made the same for all lanes where the compiler sees it: what is computed from
   // them, and the loops they bound, then stay in uniform registers, which is where the tensor-core instructions take their operands.
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
@@ -98,18 +102,18 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   const uint32_t tile_rows = max(32u, ((per_cta + rounds - 1) / rounds + 31u) & ~31u);
   const uint32_t t32 = tile_rows >> 5;
   const uint32_t ntiles = (n_out + tile_rows - 1) / tile_rows;
-  // Two rings share the buffer, rows with their scales and weights with theirs.  Weights of which all chunks fit beside four
-  // stages of rows stay, and are waited for on barriers of their own.
-  constexpr uint32_t kFit = kRingBytes / (kWeightBytes + kRowStage);
-  const bool resident = nchunk <= kMaxStages && kRingBytes >= (uint32_t)nchunk * kWeightBytes + 4u * kRowStage;
-  const uint32_t nwst = resident ? (uint32_t)nchunk : kFit;
-  const uint32_t nst = min((uint32_t)kMaxStages, (kRingBytes - nwst * kWeightBytes) / kRowStage);
-  const uint32_t sW = smem_u32(smem), sR = sW + nwst * kWeightBytes;
+  // Two rings share the buffer, rows with their scales (three stages or more) and weights with theirs.  Weights that fit beside
+  // three stages of rows stay.
+  const bool resident = npair <= kMaxStages && kRingBytes >= (uint32_t)npair * kWeightStage + 3u * kRowStage;
+  const uint32_t nwst = resident ? (uint32_t)npair : min((uint32_t)kMaxStages, (kRingBytes - 3u * kRowStage) / kWeightStage);
+  const uint32_t nst = min(kDeepest, (kRingBytes - nwst * kWeightStage) / kRowStage);
+  const uint32_t sW = smem_u32(smem), sR = sW + nwst * kWeightStage;
 
   if (threadIdx.x < kMaxStages) {
-    mbar_init(bar_full + 8 * threadIdx.x, 32u * t32 + (resident ? 0u : 1u));
+    mbar_init(bar_full + 8 * threadIdx.x, 32u * t32);
     mbar_init(bar_empty + 8 * threadIdx.x, 1);
-    mbar_init(bar_weights + 8 * threadIdx.x, 1);
+    mbar_init(bar_wfull + 8 * threadIdx.x, 1);
+    mbar_init(bar_wempty + 8 * threadIdx.x, 1);
     if (threadIdx.x < 2) {
       mbar_init(bar_tfull + 8 * threadIdx.x, 1);
       mbar_init(bar_tempty + 8 * threadIdx.x, kDrain);
@@ -126,41 +130,31 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   if (warp == kWeightWarp) {
     // -------------------------------------------------------------- weights
     if (lane == 0) {
-      uint32_t s = 0, ws = 0;    // row stage (whose barrier the copy signs), weight stage
-      uint32_t os = 0, oph = 0;  // row stage and phase of the chunk `nwst` before
-      uint32_t tile = blockIdx.x;
-      int j = 0;
-      auto fetch = [&](uint32_t bar) {
-        mbar_expect_tx(bar, kWeightBytes);
-        const uint8_t* src = a.wpk + (size_t)j * kRecord;
-        const uint32_t dst = sW + ws * kWeightBytes;
-        if (COUT == 128) {
-          bulk_g2s(dst, src, kWeightBytes, bar);
-        } else {
-          bulk_g2s(dst, src, COUT * 128, bar);
-          bulk_g2s(dst + COUT * 128, src + 128 * 128, W * kAtomBytes, bar);
-        }
-        if (++s == nst) s = 0;
-        if (++ws == nwst) ws = 0;
-        if (++j == nchunk) {
-          j = 0;
-          tile += gridDim.x;
-        }
-      };
-      if (resident) {
-        if (tile < ntiles)
-          for (int k = 0; k < nchunk; ++k) fetch(bar_weights + 8 * k);
-      } else {
-#pragma unroll 1
-        for (uint32_t n = 0; n < nwst && tile < ntiles; ++n) fetch(bar_full + 8 * s);
-        while (tile < ntiles) {
-          if (!mbar_wait_spin(bar_empty + 8 * os, oph, abort_flag, a.status, 36u)) break;
-          if (++os == nst) {
-            os = 0;
-            oph ^= 1u;
+      uint32_t ws = 0, ph = 1;
+      for (uint32_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
+        for (int j = 0; j < nchunk; j += kPair) {
+          if (!mbar_wait_spin(bar_wempty + 8 * ws, ph, abort_flag, a.status, 36u)) {
+            tile = ntiles;  // (the loops end)
+            break;
           }
-          fetch(bar_full + 8 * s);
+          const uint32_t n = min(kPair, (uint32_t)(nchunk - j)), bar = bar_wfull + 8 * ws;
+          const uint8_t* src = a.wpk + (size_t)j * kRecord;
+          const uint32_t dst = sW + ws * kWeightStage;
+          mbar_expect_tx(bar, n * kWeightBytes);
+          if (COUT == 128) {
+            bulk_g2s(dst, src, n * kWeightBytes, bar);
+          } else {
+            for (uint32_t c = 0; c < n; ++c) {
+              bulk_g2s(dst + c * kWeightBytes, src + c * kRecord, COUT * 128, bar);
+              bulk_g2s(dst + c * kWeightBytes + COUT * 128, src + c * kRecord + 128 * 128, W * kAtomBytes, bar);
+            }
+          }
+          if (++ws == nwst) {
+            ws = 0;
+            ph ^= 1u;
+          }
         }
+        if (resident || tile >= ntiles) break;
       }
     }
     __syncwarp();
@@ -191,10 +185,11 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
         for (uint32_t i = 0; i < 8; ++i) v[i] = (live && row + i < n_out) ? __ldg(src + i) : -1;
       }
     };
+    // j counts pairs of chunks
     auto advance = [&](uint32_t& tile, int& j, int by) {
       j += by;
-      while (j >= nchunk) {
-        j -= nchunk;
+      while (j >= npair) {
+        j -= npair;
         tile += gridDim.x;
       }
     };
@@ -204,34 +199,44 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     uint32_t ntile = tile;
     int nj = j;
     uint32_t it = grp, s = grp % nst, ph = (grp / nst) & 1u;
-    auto step = [&](int32_t (&idx)[8]) -> bool {
+    auto load_pair = [&](int32_t (&idx)[kPair][8]) {
+#pragma unroll
+      for (uint32_t c = 0; c < kPair; ++c) load_idx(ntile, nj * (int)kPair + (int)c, idx[c]);
+      advance(ntile, nj, kGroups);
+    };
+    auto step = [&](int32_t (&idx)[kPair][8]) -> bool {
       if (tile >= ntiles) return false;
       if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, abort_flag, a.status, 31u)) return false;
-      const uint32_t stage = sR + s * kRowStage;
-      // what lies in K steps past the last tap is never read by an MMA
-      const bool dead_seg = j == nchunk - 1 && (seg >> 1) >= last_steps;
-      if (!dead_seg) {
-        const uint8_t* src = a.codes + seg_in * 16u;
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const int32_t sr = idx[i];
-          const uint32_t r = 4u * (i & 1u) + slot;  // row of its group of 8
-          cp_async16(stage + (pw * 4u + (i >> 1)) * 1024u + r * 128u + ((seg ^ r) << 4), src + (int64_t)sr * RB,
-                     (uint32_t)sr < a.in_rows ? 16u : 0u);
+      for (uint32_t c = 0; c < kPair; ++c) {
+        const int chunk = j * (int)kPair + (int)c;
+        if (chunk >= nchunk) break;
+        const uint32_t stage = sR + s * kRowStage + c * kCodes;
+        // what lies in K steps past the last tap is never read by an MMA
+        const bool dead_seg = chunk == nchunk - 1 && (seg >> 1) >= last_steps;
+        if (!dead_seg) {
+          const uint8_t* src = a.codes + seg_in * 16u;
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i) {
+            const int32_t sr = idx[c][i];
+            const uint32_t r = 4u * (i & 1u) + slot;  // row of its group of 8
+            cp_async16(stage + (pw * 4u + (i >> 1)) * 1024u + r * 128u + ((seg ^ r) << 4), src + (int64_t)sr * RB,
+                       (uint32_t)sr < a.in_rows ? 16u : 0u);
+          }
+        }
+        // (taps past the last one have indices -1, and zeros for scales)
+        const uint8_t* src = a.scales + word * 4u;
+        const uint32_t to = sR + s * kRowStage + sf_dst + c * W * kAtomBytes;
+#pragma unroll
+        for (uint32_t i = 0; i < 8 / kParts; ++i) {
+          int32_t sr = idx[c][kParts * i];
+#pragma unroll
+          for (uint32_t p = 1; p < kParts; ++p) sr = part == p ? idx[c][kParts * i + p] : sr;
+          cp_async4(to + (kParts * i + part) * 64u, src + (int64_t)sr * kPitch, (uint32_t)sr < a.in_rows ? 4u : 0u);
         }
       }
-      // (taps past the last one have indices -1, and zeros for scales)
-      const uint8_t* src = a.scales + word * 4u;
-#pragma unroll
-      for (uint32_t i = 0; i < 8 / kParts; ++i) {
-        int32_t sr = idx[kParts * i];
-#pragma unroll
-        for (uint32_t p = 1; p < kParts; ++p) sr = part == p ? idx[kParts * i + p] : sr;
-        cp_async4(stage + sf_dst + (kParts * i + part) * 64u, src + (int64_t)sr * kPitch, (uint32_t)sr < a.in_rows ? 4u : 0u);
-      }
       if (!(a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) cp_async_arrive_noinc(bar_full + 8 * s);
-      load_idx(ntile, nj, idx);
-      advance(ntile, nj, kGroups);
+      load_pair(idx);
       advance(tile, j, kGroups);
       it += kGroups;
       s += kGroups;
@@ -241,11 +246,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       }
       return true;
     };
-    int32_t idx_a[8], idx_b[8];
-    load_idx(ntile, nj, idx_a);
-    advance(ntile, nj, kGroups);
-    load_idx(ntile, nj, idx_b);
-    advance(ntile, nj, kGroups);
+    int32_t idx_a[kPair][8], idx_b[kPair][8];
+    load_pair(idx_a);
+    load_pair(idx_b);
     while (step(idx_a) && step(idx_b)) {
     }
     cp_async_wait_all();  // nothing of this thread may still be writing when the CTA exits
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     const uint32_t desc_hi = (uint32_t)(wdesc0 >> 32);
     const uint32_t sf_hi = (uint32_t)(scale_desc(sW) >> 32), sfw0 = (uint32_t)scale_desc(sW), sfr0 = (uint32_t)scale_desc(sR);
     bool alive = true;
-    uint32_t s = 0, ws = 0, ph = 0, tl = 0;
+    uint32_t s = 0, ws = 0, ph = 0, wph = 0, tl = 0;
     for (uint32_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++tl) {
       const uint32_t buf = tl & 1u;
       alive = alive && mbar_wait_spin(bar_tempty + 8 * buf, ((tl >> 1) & 1u) ^ 1u, abort_flag, a.status, 32u);
@@ -266,39 +269,49 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       const uint32_t d_tmem = tmem_base + buf * COUT;
       uint32_t accumulate = 0u;
 #pragma unroll 1
-      for (int j = 0; j < nchunk; ++j) {
-        if (resident && tl == 0u)
-          alive = alive && mbar_wait_spin(bar_weights + 8 * j, 0u, abort_flag, a.status, 37u);
+      for (int j = 0; j < nchunk; j += kPair) {
+        if (!resident || tl == 0u)
+          alive = alive && (mbar_test_wait(bar_wfull + 8 * ws, wph) ||
+                            mbar_wait_spin(bar_wfull + 8 * ws, wph, abort_flag, a.status, 37u));
         alive = alive && (mbar_test_wait(bar_full + 8 * s, ph) ||
                           mbar_wait_spin(bar_full + 8 * s, ph, abort_flag, a.status, 33u));
         __syncwarp();
         const uint32_t issue = leader && alive ? 1u : 0u;
         fence_proxy_async();  // rows come through the generic proxy, MMAs and copies read through the async one
         tc_fence_after();
-        const uint32_t w_at = (ws * kWeightBytes) >> 4, r_at = (s * kRowStage) >> 4;
-        // a place for every stage: it is filled again only when the MMAs that read its scales are complete
-        const uint32_t sfr = tmem_base + 2u * COUT + s * kSfCols, sfw = sfr + 4u * W;
 #pragma unroll
-        for (uint32_t w = 0; w < W; ++w) {
-          copy_scales_if(issue, sfr + 4u * w, sfr0 + r_at + ((kSfOff + w * kAtomBytes) >> 4), sf_hi);
-          copy_scales_if(issue, sfw + 4u * w, sfw0 + w_at + ((COUT * 128u + w * kAtomBytes) >> 4), sf_hi);
-        }
-        const uint32_t steps = j + 1 == nchunk ? last_steps : 4u;
-        const uint32_t wd = (uint32_t)wdesc0 + w_at, rd = (uint32_t)rdesc0 + r_at;
+        for (uint32_t c = 0; c < kPair; ++c) {
+          if (j + (int)c >= nchunk) break;
+          const uint32_t w_at = (ws * kWeightStage + c * kWeightBytes) >> 4, r_at = (s * kRowStage + c * kCodes) >> 4;
+          const uint32_t f_at = (s * kRowStage + kSfOff + c * W * kAtomBytes) >> 4;
+          // a place for every stage: it is filled again only when the MMAs that read its scales are complete
+          const uint32_t sfr = tmem_base + 2u * COUT + s * kSfCols + c * 8u * W, sfw = sfr + 4u * W;
 #pragma unroll
-        for (uint32_t k = 0; k < 4u; ++k) {
-          const uint32_t w = k / kSteps;
-          umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, rd + 2u * k, wd + 2u * k, desc_hi,
-                              idesc_of<FMT>(COUT, (k % kSteps) * 2u), sfr + 4u * w, sfw + 4u * w,
-                              k == 0 ? accumulate : 1u);
+          for (uint32_t w = 0; w < W; ++w) {
+            copy_scales_if(issue, sfr + 4u * w, sfr0 + f_at + ((w * kAtomBytes) >> 4), sf_hi);
+            copy_scales_if(issue, sfw + 4u * w, sfw0 + w_at + ((COUT * 128u + w * kAtomBytes) >> 4), sf_hi);
+          }
+          const uint32_t steps = j + (int)c + 1 == nchunk ? last_steps : 4u;
+          const uint32_t wd = (uint32_t)wdesc0 + w_at, rd = (uint32_t)rdesc0 + r_at;
+#pragma unroll
+          for (uint32_t k = 0; k < 4u; ++k) {
+            const uint32_t w = k / kSteps;
+            umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, rd + 2u * k, wd + 2u * k, desc_hi,
+                                idesc_of<FMT>(COUT, (k % kSteps) * 2u), sfr + 4u * w, sfw + 4u * w,
+                                k == 0 ? accumulate : 1u);
+          }
+          accumulate = 1u;
         }
-        accumulate = 1u;
         tc_commit_if(issue, bar_empty + 8 * s);
+        if (!resident) tc_commit_if(issue, bar_wempty + 8 * ws);
         if (++s == nst) {
           s = 0;
           ph ^= 1u;
         }
-        if (++ws == nwst) ws = 0;
+        if (++ws == nwst) {
+          ws = 0;
+          wph ^= 1u;
+        }
       }
       tc_commit_if(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
     }
