@@ -199,12 +199,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     uint32_t ntile = tile;
     int nj = j;
     uint32_t it = grp, s = grp % nst, ph = (grp / nst) & 1u;
-    auto load_pair = [&](int32_t (&idx)[kPair][8]) {
+    int32_t idx[kPair][8];
+    auto load_pair = [&]() {
 #pragma unroll
       for (uint32_t c = 0; c < kPair; ++c) load_idx(ntile, nj * (int)kPair + (int)c, idx[c]);
       advance(ntile, nj, kGroups);
     };
-    auto step = [&](int32_t (&idx)[kPair][8]) -> bool {
+    auto step = [&]() -> bool {
       if (tile >= ntiles) return false;
       if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, abort_flag, a.status, 31u)) return false;
 #pragma unroll
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
         }
       }
       if (!(a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) cp_async_arrive_noinc(bar_full + 8 * s);
-      load_pair(idx);
+      load_pair();
       advance(tile, j, kGroups);
       it += kGroups;
       s += kGroups;
@@ -246,10 +247,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       }
       return true;
     };
-    int32_t idx_a[kPair][8], idx_b[kPair][8];
-    load_pair(idx_a);
-    load_pair(idx_b);
-    while (step(idx_a) && step(idx_b)) {
+    // (a second set of indices, loaded one step further ahead, gained nothing: 120 000 rows 64 -> 64 26.0 us, with one 25.3)
+    load_pair();
+    while (step()) {
     }
     cp_async_wait_all();  // nothing of this thread may still be writing when the CTA exits
     __syncwarp();
