@@ -16,7 +16,7 @@ struct Output {
   TensorScale ts;  // of 4-bit output
   int act, res_relu;
   int mode;    // 0: fp16, 1: MXFP4, 2: NVFP4
-  int access;  // bytes of an fp16 row that may be stored (and of the residual, read) at once: 16 or 2
+  int access;  // bytes of an fp16 row that may be stored (and of the residual, read) at once: 16, 4 or 2
 };
 
 // A warp's 32 rows x 32 channels of fp16 between its lanes and memory by way of 2 KB of shared memory: a lane has a row
@@ -51,17 +51,35 @@ __device__ __forceinline__ void stage_bias(const Patch& p, float b) {
   asm volatile("st.shared.f32 [%0], %1;" ::"r"(p.stage + 2048u + 4u * p.lane), "f"(b) : "memory");
 }
 
-// The residual on its way into the patch's shared memory (with 16-byte access; else it is read where it is used).  Copies in
-// program order: it may be what the launch before wrote.
+// The residual on its way into the patch's shared memory, in program order: it may be what the launch before wrote.  (Rows that do
+// not start on 16 bytes go by pairs of channels, two rows an instruction, or by single ones.)
 __device__ __forceinline__ void prefetch_residual(const Output& o, const Patch& p) {
-  if (o.access < 16) return;
   __syncwarp();  // what was there is read
-  const uint32_t c = p.col + 8u * (p.lane % 4u);
+  if (o.access >= 16) {
+    const uint32_t c = p.col + 8u * (p.lane % 4u);
 #pragma unroll
-  for (uint32_t k = 0; k < 4; ++k) {
-    const uint32_t r = 8u * k + p.lane / 4u;
-    const bool there = p.row0 + r < p.rows && c < o.cout;
-    cp_async16(p.stage + staged_at(r, p.lane % 4u), o.res + (there ? (p.row0 + r) * o.cout + c : 0u), there ? 16u : 0u);
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint32_t r = 8u * k + p.lane / 4u;
+      const bool there = p.row0 + r < p.rows && c < o.cout;
+      cp_async16(p.stage + staged_at(r, p.lane % 4u), o.res + (there ? (p.row0 + r) * o.cout + c : 0u), there ? 16u : 0u);
+    }
+    return;
+  }
+  const uint32_t per = o.access == 4 ? 2u : 1u, lanes = 32u / per;  // channels a lane, lanes a row
+  const uint32_t at = p.lane % lanes * per;
+#pragma unroll 8
+  for (uint32_t k = 0; k < lanes; ++k) {
+    const uint32_t r = k * per + p.lane / lanes;
+    const bool there = p.row0 + r < p.rows && p.col + at < o.cout;
+    const __half* from = o.res + (p.row0 + r) * o.cout + p.col + at;
+    const uint32_t to = p.stage + staged_at(r, at / 8u) + at % 8u * 2u;
+    if (per == 2u) {
+      const uint32_t v = there ? load_in_order((const uint32_t*)from) : 0u;
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
+    } else {
+      const uint16_t v = there ? (uint16_t)load_in_order((const uint16_t*)from) : (uint16_t)0;
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+    }
   }
 }
 
@@ -93,8 +111,8 @@ __device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
 template <bool RES>
 __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const Patch& p) {
   const uint64_t row = p.row0 + p.own;
-  const bool live = row < p.rows, wide = o.access >= 16;
-  if (RES && wide) cp_async_wait_all();
+  const bool live = row < p.rows;
+  if (RES) cp_async_wait_all();
   __syncwarp();  // residual and bias are there, and what was there is read
   // step by step over all 32 channels, so that the loads of a step are in flight together
   {
@@ -119,20 +137,10 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
     }
     if (RES) {
       uint32_t r[16];
-      if (wide) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint4 t = ld_shared16(p.stage + staged_at(p.own, c));
-          r[4 * c] = t.x; r[4 * c + 1] = t.y; r[4 * c + 2] = t.z; r[4 * c + 3] = t.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t at = p.col + 2 * i;
-          const uint16_t* q = (const uint16_t*)o.res + row * o.cout + at;
-          r[i] = live && at < o.cout ? (uint32_t)load_in_order(q) : 0u;
-          if (live && at + 1u < o.cout) r[i] |= (uint32_t)load_in_order(q + 1) << 16;
-        }
+      for (int c = 0; c < 4; ++c) {
+        const uint4 t = ld_shared16(p.stage + staged_at(p.own, c));
+        r[4 * c] = t.x; r[4 * c + 1] = t.y; r[4 * c + 2] = t.z; r[4 * c + 3] = t.w;
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -147,17 +155,32 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
       }
     }
     if (o.mode == 0) {
-      if (!wide) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (live && p.col + i < o.cout)
-            ((uint16_t*)o.out)[row * o.cout + p.col + i] = (uint16_t)(h[i / 2] >> (16 * (i % 2)));
-        return;
-      }
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         st_shared16(p.stage + staged_at(p.own, c), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
       __syncwarp();
+      if (o.access < 16) {
+        const uint32_t per = o.access == 4 ? 2u : 1u, lanes = 32u / per;
+        const uint32_t at = p.lane % lanes * per;
+        if (p.col + at >= o.cout) return;
+        __half* to = (__half*)o.out + (p.row0 + p.lane / lanes) * o.cout + p.col + at;
+#pragma unroll 8
+        for (uint32_t k = 0; k < lanes; ++k, to += per * o.cout) {
+          const uint32_t r = k * per + p.lane / lanes;
+          if (p.row0 + r >= p.rows) break;
+          const uint32_t from = p.stage + staged_at(r, at / 8u) + at % 8u * 2u;
+          if (per == 2u) {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+            *(uint32_t*)to = v;
+          } else {
+            uint16_t v;
+            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+            *(uint16_t*)to = v;
+          }
+        }
+        return;
+      }
       uint4 t[4];
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) t[k] = ld_shared16(p.stage + staged_at(8u * k + p.lane / 4u, p.lane % 4u));
@@ -226,7 +249,7 @@ inline bool make_output(const spconvb_fp4_params& p, const float* bias, void* ou
     o.spitch = scale_pitch(p.out_format, o.cout);
   }
   const uint64_t bits = (uint64_t)(uintptr_t)p.res | 2ull * o.cout | (p.out_fp4 ? 0ull : (uint64_t)(uintptr_t)out);
-  o.access = bits % 16u == 0u ? 16 : 2;
+  o.access = bits % 16u == 0u ? 16 : (bits % 4u == 0u ? 4 : 2);
   return true;
 }
 

@@ -172,7 +172,7 @@ def test_rows_at_any_element(fmt, offset, channels):
 # ---------------------------------------------------------------------------- products
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("rows,cin,cout", [
-    (1, 64, 64), (1, 1, 1), (3, 16, 8), (128, 64, 64), (127, 256, 64), (129, 320, 65), (50, 200, 136), (300, 72, 130),
+    (1, 64, 64), (1, 1, 1), (3, 16, 8), (128, 64, 64), (127, 256, 64), (129, 320, 65), (50, 200, 136), (300, 72, 130), (300, 72, 131), (9000, 72, 330),
     (1, 4096, 512), (5, 4100, 100), (2, 200, 9), (4, 64, 130), (8, 1000, 264), (9, 300, 72), (64, 16384, 64), (130, 9000, 300), (7, 8200, 1000), (130, 2048, 256), (1000, 512, 300), (20000, 64, 64), (19000, 192, 128),
     (19100, 128, 200), (40000, 256, 256), (5000, 448, 1000)])
 def test_linear(fmt, rows, cin, cout):
@@ -224,7 +224,7 @@ def _conv_problem(fmt, n, cin, cout, kvol, seed=0):
 
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("n,cin,cout,kvol", [
-    (1, 64, 64, 27), (33, 64, 64, 27), (200, 128, 128, 27), (1000, 256, 128, 27), (777, 48, 24, 27), (500, 100, 100, 27),
+    (1, 64, 64, 27), (33, 64, 64, 27), (200, 128, 128, 27), (1000, 256, 128, 27), (777, 48, 24, 27), (500, 100, 100, 27), (1500, 64, 50, 27), (1500, 64, 33, 27), (1500, 128, 105, 9),
     (5000, 64, 64, 27), (9000, 64, 128, 27), (30000, 64, 32, 27), (29000, 128, 128, 27), (24000, 128, 64, 9),
     (3000, 256, 64, 3), (4000, 64, 64, 1), (2000, 33, 1, 8), (60000, 64, 64, 3)])
 def test_conv(fmt, n, cin, cout, kvol):
