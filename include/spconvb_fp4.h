@@ -12,8 +12,8 @@
  *                  exponent clamped to -127 (amax = 0 gives byte 0).  No tensor scale: pass 1.
  *   SPCONVB_NVFP4  blocks of 16 channels; scale byte e4m3 = amax / (6 * tensor_scale), rounded to nearest even and
  *                  saturated at 448; tensor_scale is one positive fp32 number a tensor.
- *   A block's scale is S = 2^e, or e4m3 * tensor_scale rounded to fp32; its codes are x / S (one fp32 division) rounded
- *   to nearest even and saturated at 6, all 0 where S is 0 (the sign of a zero is not specified).  A block that holds an infinity or a NaN gets the NaN scale
+ *   A block's scale is S = 2^e, or e4m3 * tensor_scale rounded to fp32; its codes are x / S (in fp32, to the last bit, and
+ *   exactly on the borders between codes) rounded to nearest even and saturated at 6, all 0 where S is 0 (the sign of a zero is not specified).  A block that holds an infinity or a NaN gets the NaN scale
  *   (0xff, 0x7f) and codes 0, so that it stays visible: it reads as NaN, and so does every product with it.
  *
  * Layout of rows (all pointers 16-byte aligned)

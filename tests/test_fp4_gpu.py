@@ -618,3 +618,40 @@ def test_offsets_beyond_32_bits():
     mm[1] = -1
     y, off = ref.product(_gather(ref.values(*want, ref.NV, ch), mm), cv, float(np.float32(g * 0.01)), None, False)
     assert (np.abs(got - y) <= off).all()
+
+
+@pytest.mark.parametrize("rows,cin,cout", [(1, 512, 64), (8, 300, 41), (64, 16384, 64), (300, 200, 131), (20000, 1024, 256)])
+def test_every_form_of_the_linear_layer_is_captured_and_replayed(rows, cin, cout):
+    """Few rows, a split K, odd channels, wide tiles: a graph gives what calls give, on rows that came later."""
+    ops = _ops()
+    w = ops.Fp4Weights(_features(cout, cin, 1, 0.1), ref.NV, 0.01)
+    q, _ = _quantized(_features(rows, cin, 2, 0.1), ref.NV, 0.01)
+    later, _ = _quantized(_features(rows, cin, 3, 0.1), ref.NV, 0.01)
+    n = ops.device_count(rows)
+    ops.fp4_linear(q, n, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.fp4_linear(q, n, w, act=ops.ACT_RELU)
+    want = ops.fp4_linear(later, n, w, act=ops.ACT_RELU)
+    q.codes.copy_(later.codes)
+    q.scales.copy_(later.scales)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_few_rows_of_extreme_scales():
+    """Blocks whose scales' product is beyond fp32, with and without products of codes."""
+    ops = _ops()
+    x = np.zeros((2, 64), np.float32)
+    x[0, 0], x[1, 1] = 6 * 2.0 ** 100, 3 * 2.0 ** -100
+    w = np.zeros((8, 64), np.float32)
+    w[0, 2], w[1, 0], w[2, 1] = 2.0 ** 60, 2.0 ** -100, 2.0 ** 100
+    q, _ = _quantized(x, ref.MX, 1.0)
+    for rows in (2, 9):                      # on the CUDA cores, and on the tensor cores
+        codes, scales = ref.quantize(np.concatenate([x, np.zeros((rows - 2, 64), np.float32)]), ref.MX)
+        q = ops.Fp4Rows(_dev(codes), _dev(scales), 64, ref.MX)
+        y = ops.fp4_linear(q, ops.device_count(rows), ops.Fp4Weights(w, ref.MX)).cpu().numpy()
+        assert np.array_equal(y[:2], (x.astype(np.float64) @ w.T.astype(np.float64)).astype(np.float16)), rows
+        assert not y[2:].any()
