@@ -14,9 +14,11 @@
 // read its scales are complete, so no copy overwrites scales that are in use.
 //
 // TN is 256 or 128.  A tile of 64 channels was slower also for 64 channels (1 row x 256 -> 64 4.3 us, with half of a tile
-// of 128 empty 3.6): it takes as many instructions.  The widest, whose single accumulator is drained with no MMA beside it, is taken
-// where K is long enough to make up for that and every SM has a tile: us, TN 256 / 128: 32 400 x 256 -> 512 14.7 / 13.1, x 512
-// 15.8 / 14.6, x 1 024 19.0 / 20.0, 8 192 x 4 096 -> 4 096 66.2 / 90.8; 200 x 8 192 -> 8 192 28.5 / 17.2.
+// of 128 empty 3.6): it takes as many instructions.  A tile of 256 brings 54 KB a chunk into the SM where two of 128 bring 72, but its
+// single accumulator is drained with no MMA beside it; measured, a tile takes about 4 400 cycles and 820 a chunk, one of 128 2 000 and 600, and
+// the launch takes what costs less over its rounds of tiles (us, 256 / 128: 32 400 x 256 -> 512 14.7 / 13.1, x 1 024 19.0 / 20.0; 8 192 x
+// 4 096 -> 4 096 66.2 / 90.8; 200 x 8 192 -> 8 192 28.5 / 17.2).  What bounds it: short K, the epilogue and the writing of fp16 rows (2 100
+// cycles for 32 KB a tile and SM); long K, the bytes from L2 to an SM, 45-60 a cycle (8 192 x 4 096 -> 4 096: 4.2 PFLOP/s, 52 % of the tensor pipe).
 //
 // Few tiles and a long K: K is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
 // always in the same order.  That costs 5 us and a chunk takes 0.32, so it begins at 32 chunks (64 rows -> 64 channels, us, split / not:
@@ -443,7 +445,10 @@ int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream
   const uint64_t tm = (rows + kTileM - 1) / kTileM;
   auto tiles = [&](uint32_t tn) { return tm * ((a.o.cout + tn - 1) / tn); };
   a.split = 1;
-  if (a.o.cout > 128u && a.nchunk >= 4u && tiles(256) >= (uint64_t)kSmCount)
+  auto cost = [&](uint32_t tn, uint64_t tile, uint64_t chunk) {
+    return (tiles(tn) + kSmCount - 1) / kSmCount * (tile + chunk * a.nchunk);
+  };
+  if (a.o.cout > 128u && cost(256, 4400, 820) < cost(128, 2000, 600))
     return launch_linear<FMT, 256, false>(a, map, (uint32_t)tiles(256), st);
   const uint64_t t = tiles(128);
   if (a.nchunk >= 32u)
