@@ -11,14 +11,16 @@
 //   16     allocates tensor memory, copies the chunk's scales there, issues its MMAs
 //   17     one lane: the weights, a bulk copy of codes and scales a chunk, or once where all chunks fit
 //   18-25  producers, two groups of four that take the chunks in turn; a warp owns 32 rows, a thread one 16-byte segment of 8
-//          of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, zeros for missing neighbours, all
-//          of which arrive on the stage's barrier by themselves
+//          of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, which arrive on the stage's barrier by
+//          themselves.  A missing neighbour has zeros for scales; its codes stay what they were (any sixteen values are numbers, and times
+//          an e4m3 scale of 0 they are 0), except in MXFP4, whose smallest scale is not 0
 //
 // What bounds it.  A chunk of 128 rows costs the tensor pipe 331 cycles (128 channels) or 267 (64), its 48 copies about 400 in the
 // load-store pipe, and shared memory about 600 in the wide layer (18 KB of rows and 18 of weights written, 32 read by the MMAs); in the kernel
-// it takes 740, of which half goes away without the gather and the epilogue.  120 000 rows, us: 64 -> 64 25.3, 128 -> 128 42.3
-// (MXFP4) and 45.3 (NVFP4, twice the scale words), with a residual 26.9 / 45.9 / 49.1; 14 000 rows 64 -> 64 6.9.  Stages of two chunks
-// because every wait, fence and commit is paid once a stage (one chunk a stage: 28.7, 55.9).
+// it takes 690, of which half goes away without the gather and the epilogue.  120 000 rows, us, MXFP4 / NVFP4: 64 -> 64 24.8 / 23.9,
+// 128 -> 128 41.1 / 42.4 (twice the scale words), with a residual 26.3 / 25.2 and 44.7 / 45.6; 14 000 rows 64 -> 64 6.9.  Zeros for the codes of
+// missing neighbours, too, cost NVFP4 4 % (24.8, 43.9).  Stages of two chunks because every wait, fence and commit is paid once
+// a stage (one chunk a stage: 28.7, 55.9).
 //
 // Within the 32 rows of a warp, row 8 slot + i of the tile lies at 4 i + slot of the operand: the words of scales that
 // the 32 lanes write at the same time then lie in eight groups of four banks and not in two.
@@ -54,6 +56,14 @@ struct ConvArgs {
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t src_bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+
+// A copy that is made or not made: nothing is written where it is not.
+__device__ __forceinline__ void cp_async16_if(uint32_t make, uint32_t dst, const void* src) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst),
+      "l"(src), "r"(make)
+      : "memory");
 }
 
 // CP: stored channels of an input row.  COUT: output channels, rounded up to 64 or 128.  RES: with a residual.
@@ -227,8 +237,10 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
           for (uint32_t i = 0; i < 8; ++i) {
             const int32_t sr = idx[c][i];
             const uint32_t r = 4u * (i & 1u) + slot;  // row of its group of 8
-            cp_async16(stage + (pw * 4u + (i >> 1)) * 1024u + r * 128u + ((seg ^ r) << 4), src + (int64_t)sr * RB,
-                       (uint32_t)sr < a.in_rows ? 16u : 0u);
+            const uint32_t to = stage + (pw * 4u + (i >> 1)) * 1024u + r * 128u + ((seg ^ r) << 4);
+            const bool there = (uint32_t)sr < a.in_rows;
+            if (FMT == SPCONVB_NVFP4) cp_async16_if(there, to, src + (int64_t)sr * RB);
+            else cp_async16(to, src + (int64_t)sr * RB, there ? 16u : 0u);
           }
         }
         // (taps past the last one have indices -1, and zeros for scales)

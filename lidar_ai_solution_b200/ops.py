@@ -304,6 +304,11 @@ def _fp4_device(t, count, *others):
     return dev
 
 
+def _fp4_tensor_scale(fmt, g):
+    if not (g == 1 if fmt == MXFP4 else 0 < g < math.inf):
+        raise ValueError("a tensor scale is a positive number, and 1 for MXFP4")
+
+
 def _fp4_stream(dev):
     return _stream() if _raw_stream is None else _raw_stream(dev)
 
@@ -327,6 +332,7 @@ class Fp4Rows:
         _fp4_tensor(scales, torch.uint8, self.rows, sp, "scales")
         if codes.device != scales.device:
             raise ValueError("codes and scales of different devices")
+        _fp4_tensor_scale(fmt, tensor_scale)
         self._hold = codes, scales
         self.channels, self.fmt, self.tensor_scale = channels, fmt, float(tensor_scale)
         self.device_index, self.codes_ptr, self.scales_ptr = codes.get_device(), codes.data_ptr(), scales.data_ptr()
@@ -390,7 +396,8 @@ def fp4_dequantize(q, n_ptr, out_kind=F16, out=None):
     """What the codes and scales of ``q`` stand for: [rows, channels] fp16 or fp32."""
     rows, dt = q.rows, torch.float32 if out_kind == F32 else torch.float16
     if out is None:
-        out = q._buffer().new_empty((rows, q.channels), dtype=dt)
+        buf = q._buffer()
+        out = torch.empty_strided((rows, q.channels), (q.channels, 1), dtype=dt, device=buf.device)
     else:
         _fp4_tensor(out, dt, rows, q.channels, "out")
     dev = _fp4_device(out, n_ptr)
@@ -423,6 +430,7 @@ class Fp4Weights:
         if len(shape) != 3:
             raise ValueError("weights are [cout, kvol, cin] or [cout, cin]")
         self.cout, self.kvol, self.cin = (int(v) for v in shape)
+        _fp4_tensor_scale(fmt, tensor_scale)
         self.fmt, self.tensor_scale = fmt, float(tensor_scale)
         nbytes = lib.spconvb_fp4_packed_bytes(fmt, self.cin, self.cout, self.kvol)
         if nbytes == 0:
@@ -456,7 +464,7 @@ def _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out):
         p.act = act
     if out_fmt is None:
         if out is None:
-            out = wts.packed.new_empty((rows, wts.cout), dtype=torch.float16)
+            out = torch.empty_strided((rows, wts.cout), (wts.cout, 1), dtype=torch.float16, device=wts.packed.device)
         else:
             _fp4_tensor(out, torch.float16, rows, wts.cout, "out")
             if out.get_device() != wts.device_index:

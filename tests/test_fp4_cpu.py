@@ -125,6 +125,11 @@ def test_python_calls_check_what_they_are_given():
                  (codes, scales, 0)):
         with pytest.raises(ValueError):
             ops.Fp4Rows(*args, ops.NVFP4)
+    for fmt, g in ((ops.NVFP4, 0.0), (ops.NVFP4, -1.0), (ops.NVFP4, float("nan")), (ops.NVFP4, float("inf")), (ops.MXFP4, 0.5)):
+        with pytest.raises(ValueError):
+            ops.Fp4Rows(codes, scales, 64, fmt, g)
+        with pytest.raises(ValueError):
+            ops.Fp4Weights(torch.zeros(4, 64), fmt, g, device="cpu")
     with pytest.raises(ValueError):
         ops.fp4_dequantize(q, n)
     with pytest.raises(ValueError):

@@ -378,6 +378,29 @@ def test_conv_takes_rows_beyond_the_input_as_missing(fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_missing_neighbours_add_nothing_whatever_lay_there(fmt):
+    """After rows of large values in every stage: rows with no neighbour at all, and rows whose only one is zero, give the bias;
+    the map may start at any word."""
+    ops = _ops()
+    n = 3000
+    q, xv, wq, wv, alpha, bias = _conv_problem(fmt, n, 64, 64, 27)
+    x = _features(n, 64, 9, 0.3)
+    x[::7] = 0.0
+    q0, _ = _quantized(x, fmt, _scale(x, fmt))
+    big, _ = _quantized(np.full((n, 64), 6e4, np.float32), fmt, 1.0)
+    n_ptr = ops.device_count(n)
+    every = _dev(_map(n, 27, 1, live=1.1))
+    flat = torch.full((27 * n + 1,), -1, dtype=torch.int32, device="cuda")
+    none = flat[1:].view(27, n)
+    m = np.full((27, n), -1, np.int32)
+    m[5] = np.arange(n) // 7 * 7
+    for lone in (none, _dev(m)):
+        ops.fp4_conv(big, every, n_ptr, wq)
+        y = ops.fp4_conv(q0, lone, n_ptr, wq)
+        assert torch.equal(y, torch.from_numpy(bias).half().cuda().expand(n, 64))
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 def test_residual_may_be_the_output(fmt):
     ops = _ops()
     n = 3001
