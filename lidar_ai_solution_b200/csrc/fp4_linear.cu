@@ -1,24 +1,33 @@
 // 4-bit rows times 4-bit weights:  out[r, c] = act(alpha * sum_k x[r, k] W[c, k] + bias[c]).
 //
-// A tile is 128 rows (M, accumulator lanes) by TN output channels (N, accumulator columns).  K goes by chunks of
-// 256 channels: 128 bytes of codes a row, which is one swizzle atom, and four MMAs of 64 channels.  Roles of the
-// warps of a CTA (one an SM, walking over tiles):
+// A tile is 128 rows (M, accumulator lanes) by 128 output channels (N, accumulator columns) on one SM, or 256 by 256 on two: a
+// cluster of two CTAs, each with 128 rows, whose tensor cores share the weights, half of them in either's shared memory.  K goes by
+// chunks of 256 channels: 128 bytes of codes a row, which is one swizzle atom, and four MMAs of 64 channels.  Roles of the warps of a
+// CTA (one an SM, walking over tiles):
 //
 //   0-15   epilogue: a lane owns a row, a warp its quadrant of 32 and 32 or 64 channels
-//   16     allocates tensor memory; copies the chunk's scales there and issues its MMAs
-//   17     one lane: TMA of the rows' codes, bulk copies of the weights' image (codes and scales lie ready in it)
+//   16     allocates tensor memory; copies the chunk's scales there and issues its MMAs, of a pair those of both CTAs.  In the second
+//          CTA of a pair it tells the first one that its stage is full
+//   17     one lane: TMA of the rows' codes
 //   18-21  the rows' scales, a row a lane: four chunks ahead in registers, then as words into the order that the
 //          copy to tensor memory wants.  (They are kept row by row in memory, so that a convolution can gather them.)
+//   22     one lane: bulk copies of the weights' image (codes and scales lie ready in it)
 //
 // Scales in tensor memory have a place for every stage of the ring: a stage is filled again only when the MMAs that
 // read its scales are complete, so no copy overwrites scales that are in use.
 //
-// TN is 256 or 128.  A tile of 64 channels was slower also for 64 channels (1 row x 256 -> 64 4.3 us, with half of a tile
-// of 128 empty 3.6): it takes as many instructions.  A tile of 256 brings 54 KB a chunk into the SM where two of 128 bring 72, but its
-// single accumulator is drained with no MMA beside it; measured, a tile takes about 4 400 cycles and 820 a chunk, one of 128 2 000 and 600, and
-// the launch takes what costs less over its rounds of tiles (us, 256 / 128: 32 400 x 256 -> 512 14.7 / 13.1, x 1 024 19.0 / 20.0; 8 192 x
-// 4 096 -> 4 096 66.2 / 90.8; 200 x 8 192 -> 8 192 28.5 / 17.2).  What bounds it: short K, the epilogue and the writing of fp16 rows (2 100
-// cycles for 32 KB a tile and SM); long K, the bytes from L2 to an SM, 45-60 a cycle (8 192 x 4 096 -> 4 096: 4.2 PFLOP/s, 52 % of the tensor pipe).
+// A tile of 64 channels was slower also for 64 channels (1 row x 256 -> 64 4.3 us, with half of a tile of 128 empty 3.6): it takes as
+// many instructions.  A chunk of a pair brings 38 KB into an SM and is four times the work of one of 128 x 128, which brings 36, on twice
+// the SMs.  But its accumulator is the only one (two and the scales are more than tensor memory holds), drained with no MMA beside it, and
+// its channels are twice as many to write before the next tile's: measured, a tile takes about 5 000 cycles and 580 a chunk, one of 128
+// 2 000 and 600, a launch in pairs 1 500 more, and the launch takes what costs less over its rounds of tiles (us, pairs / not: 32 400 x
+// 256 -> 512 14.9 / 12.4, x 1 024 18.3 / 19.4; 8 192 x 4 096 -> 4 096 56 / 88; 200 x 8 192 -> 8 192 18.6 / 16.5, x 16 384 -> 16 384
+// 36 / 53).  With a tile of 128 rows x 256 channels on one SM, 54 KB a chunk, 8 192 x 4 096 -> 4 096 took 65.
+//
+// What bounds it: short K, the epilogue and the writing of fp16 rows (2 100 cycles for 32 KB a tile and SM).  Long K, several things at
+// once: 8 192 x 4 096 -> 4 096 takes 57 us (4.9 PFLOP/s), 51 with no code copied at all, 52 on zeros (the power limit then lowers the
+// clock less).  Of 13 100 cycles a tile the MMAs are 8 500, 1 900 the exchange of the accumulator; shared memory takes in 38 KB a chunk
+// and gives them to the tensor core at 66 + 62 of its 128 bytes a cycle when they run at their full rate.
 //
 // Few tiles and a long K: K is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
 // always in the same order.  That costs 5 us and a chunk takes 0.32, so it begins at 32 chunks (64 rows -> 64 channels, us, split / not:
@@ -37,8 +46,8 @@ namespace {
 // 4 096 -> 4 096 8.9 / 8.8, 8 x 4 096 -> 512 5.8 / 8.6, 8 x 4 096 -> 4 096 13.9 / 8.8, 1 x 8 192 -> 8 192 12.2 / 15.5).
 constexpr uint32_t kFewRows = 8;
 constexpr uint64_t kFewProducts = 1ull << 26;
-constexpr int kEpiWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kScaleWarp0 = 18;
-constexpr int kCtaThreads = 32 * 22;
+constexpr int kEpiWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kScaleWarp0 = 18, kWeightWarp = 22;
+constexpr int kCtaThreads = 32 * 23;
 constexpr uint32_t kTileM = 128;
 constexpr uint32_t kTmemCols = 512;
 
@@ -57,13 +66,16 @@ struct LinearArgs {
 
 template <int FMT, int TN>
 struct Shape {
+  static constexpr bool kPair = TN == 256;  // two CTAs of a cluster, on two SMs, share a tile of 256 rows
+  static constexpr uint32_t kCtas = kPair ? 2 : 1;
+  static constexpr uint32_t kRows = kCtas * kTileM;                 // of a tile
   static constexpr uint32_t kWords = FMT == SPCONVB_MXFP4 ? 2 : 4;  // scale words a row and chunk
   static constexpr uint32_t kBlocks = TN > 128 ? TN / 128 : 1;      // blocks of 128 channels of the image
   static constexpr uint32_t kSf = kWords * kAtomBytes;
-  static constexpr uint32_t kA = kTileM * 128, kB = TN * 128;
+  static constexpr uint32_t kA = kTileM * 128, kB = 128 * 128;
   static constexpr uint32_t kOffB = kA, kOffSfb = kA + kB, kOffSfa = kOffSfb + kBlocks * kSf;
   static constexpr uint32_t kStage = kOffSfa + kSf;  // a multiple of 1024
-  static constexpr uint32_t kStages = TN == 256 ? 3 : 5;
+  static constexpr uint32_t kStages = 5;
   static constexpr uint32_t kBuffers = TN == 256 ? 1 : 2;  // accumulators
   static constexpr uint32_t kSfCols = kWords * 4 * (1 + kBlocks);
   static constexpr uint32_t kPatches = TN == 256 ? 2 : 1;            // of 32 channels a warp
@@ -103,72 +115,92 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   // them, and the loops they bound, then stay in uniform registers, which is where the tensor-core instructions take their operands.
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const uint32_t lane = threadIdx.x & 31;
+  const uint32_t cta = S::kPair ? blockIdx.x % 2u : 0u;  // of the pair; the first issues the MMAs of both
 
   if (threadIdx.x < S::kStages) {
-    mbar_init(bar_full + 8 * threadIdx.x, 1 + 4);  // the copies' bytes, the four scale warps
+    // two with copies, the four scale warps; of a pair, the second CTA, whose warp 16 passes on that its stage is full
+    mbar_init(bar_full + 8 * threadIdx.x, 2 + 4 + (S::kPair && cta == 0u ? 1 : 0));
     mbar_init(bar_empty + 8 * threadIdx.x, 1);
     if (threadIdx.x < 2) {
       mbar_init(bar_tfull + 8 * threadIdx.x, 1);
-      mbar_init(bar_tempty + 8 * threadIdx.x, kEpiWarps);
+      mbar_init(bar_tempty + 8 * threadIdx.x, S::kCtas * kEpiWarps);
     }
     if (threadIdx.x == 0) *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
   if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (S::kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   pdl_wait_and_trigger();
   const uint32_t n = __shfl_sync(0xffffffffu, min(load_in_order(a.n_ptr), a.cap), 0);
   tc_fence_before();
   __syncthreads();
+  __syncwarp();
+  if (S::kPair) cluster_sync();  // the other CTA's barriers are there
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
 
   const uint32_t tiles_n = (a.o.cout + TN - 1) / TN;
-  const uint32_t tiles = ((n + kTileM - 1) / kTileM) * tiles_n;
+  const uint32_t tiles = ((n + S::kRows - 1) / S::kRows) * tiles_n;
   // this CTA's tiles and its part of K
   const uint32_t split = SPLIT ? a.split : 1u;
   const uint32_t rank = SPLIT ? blockIdx.x % split : 0u;
-  const uint32_t tile0 = SPLIT ? blockIdx.x / split : blockIdx.x;
-  const uint32_t tile_step = SPLIT ? gridDim.x / split : gridDim.x;
+  const uint32_t tile0 = SPLIT ? blockIdx.x / split : blockIdx.x / S::kCtas;
+  const uint32_t tile_step = SPLIT ? gridDim.x / split : gridDim.x / S::kCtas;
   const uint32_t c0 = a.nchunk * rank / split, c1 = a.nchunk * (rank + 1u) / split;
   uint32_t part[32];  // with a split: this thread's sums, over the cluster's barrier
 
-  if (warp == kLoadWarp) {
+  if (warp == kLoadWarp || warp == kWeightWarp) {
     if (lane == 0) {
       uint32_t s = 0, ph = 1, it = 0;
       bool on = true;
       for (uint32_t tile = tile0; on && tile < tiles; tile += tile_step) {
-        const uint32_t tm = tile / tiles_n, tn = tile % tiles_n;
-        for (uint32_t c = c0; c < c1; ++c, ++it) {
+        const uint32_t blk = tile % tiles_n * S::kBlocks;
+        const int32_t row = (int32_t)(tile / tiles_n * S::kRows + cta * kTileM);
+        const uint64_t block = (uint64_t)a.nchunk * a.record;  // of 128 channels
+        const uint8_t* w = a.wpk + blk * block + (uint64_t)c0 * a.record;
+        // of a pair, the codes of this CTA's block and the scales of both (the last tile may have one only)
+        const bool two = S::kPair && blk * 128u + 128u < a.o.cout;
+        const bool own = cta == 0u || two;
+        for (uint32_t c = c0; c < c1; ++c, ++it, w += a.record) {
           if (!mbar_wait(bar_empty + 8 * s, ph, abort_flag, a.status, 21u) ||
               (a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) {
             on = false;
             break;
           }
           const uint32_t st = s0 + s * S::kStage, bar = bar_full + 8 * s;
-          const uint32_t blk = tn * TN / 128u;
-          const uint8_t* w = a.wpk + ((uint64_t)blk * a.nchunk + c) * a.record;
-          if (TN == 256) {
-            const bool two = blk * 128u + 128u < a.o.cout;
-            mbar_expect_tx(bar, S::kA + (two ? 2u : 1u) * (128u * 128u + S::kSf));
-            tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
-            bulk_g2s(st + S::kOffB, w, 128u * 128u, bar);
+          if (warp == kLoadWarp) {
+            mbar_expect_tx(bar, S::kA);
+            tma_load_2d(st, &rows_map, (int32_t)(c * 128u), row, bar);
+          } else if (S::kPair) {
+            mbar_expect_tx(bar, (own ? S::kB : 0u) + (two ? 2u : 1u) * S::kSf);
+            if (own) bulk_g2s(st + S::kOffB, cta == 0u ? w : w + block, S::kB, bar);
             bulk_g2s(st + S::kOffSfb, w + 128u * 128u, S::kSf, bar);
-            if (two) {
-              const uint8_t* w2 = w + (uint64_t)a.nchunk * a.record;
-              bulk_g2s(st + S::kOffB + 128u * 128u, w2, 128u * 128u, bar);
-              bulk_g2s(st + S::kOffSfb + S::kSf, w2 + 128u * 128u, S::kSf, bar);
-            }
+            if (two) bulk_g2s(st + S::kOffSfb + S::kSf, w + block + 128u * 128u, S::kSf, bar);
           } else {
-            mbar_expect_tx(bar, S::kA + S::kB + S::kSf);
-            tma_load_2d(st, &rows_map, (int32_t)(c * 128u), (int32_t)(tm * kTileM), bar);
+            mbar_expect_tx(bar, S::kB + S::kSf);
             bulk_g2s(st + S::kOffB, w, S::kB + S::kSf, bar);
           }
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (S::kPair) {  // the last commits of the first CTA land here before this one leaves
+        for (uint32_t i = 0; on && i < S::kStages; ++i) {
+          on = mbar_wait(bar_empty + 8 * s, ph, abort_flag, a.status, 21u);
           if (++s == S::kStages) {
             s = 0;
             ph ^= 1u;
@@ -182,31 +214,36 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     const uint32_t dst = S::kOffSfa + (r % 32u) * 16u + (r / 32u) * 4u;
     constexpr uint32_t W = S::kWords;
     const bool vec = a.spitch % (4u * W) == 0u;  // a chunk's words lie whole inside the row
-    auto load = [&](uint32_t tile, uint32_t c, uint32_t (&v)[W]) {
+    // a cursor for the loads, four chunks ahead of the one for the stages; of its tile, the row's words, or none
+    uint32_t lt = tile0, lc = c0, tile = tile0, c = c0, s = 0, ph = 1;
+    const uint8_t* words = nullptr;
+    auto find = [&] {
+      const uint64_t row = (uint64_t)(lt / tiles_n) * S::kRows + cta * kTileM + r;
+      words = lt < tiles && row < n ? a.scales + row * a.spitch : nullptr;
+    };
+    find();
+    auto load = [&](uint32_t (&v)[W]) {
 #pragma unroll
       for (uint32_t w = 0; w < W; ++w) v[w] = 0u;
-      const uint64_t row = (uint64_t)(tile / tiles_n) * kTileM + r;
-      if (tile >= tiles || row >= n) return;
-      const uint8_t* p = a.scales + row * a.spitch + c * (4u * W);
-      if (vec && W == 4) {
-        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[W - 2]), "=r"(v[W - 1])
-                     : "l"(p)
-                     : "memory");
-      } else if (vec) {
-        asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p) : "memory");
-      } else {
+      if (words) {
+        const uint8_t* p = words + lc * (4u * W);
+        if (vec && W == 4) {
+          asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[W - 2]), "=r"(v[W - 1])
+                       : "l"(p)
+                       : "memory");
+        } else if (vec) {
+          asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p) : "memory");
+        } else {
 #pragma unroll
-        for (uint32_t w = 0; w < W; ++w)
-          if (c * (4u * W) + 4u * w < a.spitch) v[w] = load_in_order((const uint32_t*)p + w);
+          for (uint32_t w = 0; w < W; ++w)
+            if (lc * (4u * W) + 4u * w < a.spitch) v[w] = load_in_order((const uint32_t*)p + w);
+        }
       }
-    };
-    // a cursor for the loads, four chunks ahead of the one for the stages
-    uint32_t lt = tile0, lc = c0, tile = tile0, c = c0, s = 0, ph = 1;
-    auto next = [&](uint32_t& t, uint32_t& k) {
-      if (++k == c1) {
-        k = c0;
-        t += tile_step;
+      if (++lc == c1) {
+        lc = c0;
+        lt += tile_step;
+        find();
       }
     };
     auto step = [&](uint32_t (&v)[W]) -> bool {
@@ -220,9 +257,11 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_full + 8 * s);
-      load(lt, lc, v);
-      next(lt, lc);
-      next(tile, c);
+      load(v);
+      if (++c == c1) {
+        c = c0;
+        tile += tile_step;
+      }
       if (++s == S::kStages) {
         s = 0;
         ph ^= 1u;
@@ -231,18 +270,40 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     };
     if (c0 < c1) {
       uint32_t v0[W], v1[W], v2[W], v3[W];
-      load(lt, lc, v0);
-      next(lt, lc);
-      load(lt, lc, v1);
-      next(lt, lc);
-      load(lt, lc, v2);
-      next(lt, lc);
-      load(lt, lc, v3);
-      next(lt, lc);
+      load(v0);
+      load(v1);
+      load(v2);
+      load(v3);
       while (step(v0) && step(v1) && step(v2) && step(v3)) {
       }
     }
+  } else if (S::kPair && warp == kMmaWarp && cta != 0u) {
+    if (lane == 0) {
+      uint32_t s = 0, ph = 0;
+      bool on = true;
+      for (uint32_t tile = tile0; on && tile < tiles; tile += tile_step) {
+        for (uint32_t c = c0; c < c1; ++c) {
+          on = mbar_wait_spin(bar_full + 8 * s, ph, abort_flag, a.status, 24u);
+          if (!on) break;
+          mbar_arrive_at(bar_full + 8 * s, 0u);
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
+    auto wait = [&](uint32_t bar, uint32_t parity, uint32_t where) {
+      return mbar_test_wait(bar, parity) || mbar_wait_spin(bar, parity, abort_flag, a.status, where);
+    };
+    auto commit = [&](uint32_t go, uint32_t bar) {
+      if (S::kPair)
+        tc_commit_pair_if(go, bar);
+      else
+        tc_commit_if(go, bar);
+    };
     const bool leader = elect_one();
     const uint64_t d0 = make_smem_desc(s0);
     const uint32_t desc_hi = (uint32_t)(d0 >> 32);
@@ -252,14 +313,13 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     uint32_t s = 0, ph = 0, tl = 0;
     for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++tl) {
       const uint32_t buf = S::kBuffers == 1 ? 0u : tl & 1u, use = S::kBuffers == 1 ? tl : tl >> 1;
-      alive = alive && mbar_wait_spin(bar_tempty + 8 * buf, (use & 1u) ^ 1u, abort_flag, a.status, 23u);
+      alive = alive && wait(bar_tempty + 8 * buf, (use & 1u) ^ 1u, 23u);
       __syncwarp();
       tc_fence_after();
       const uint32_t d_tmem = tmem + buf * TN;
       uint32_t accumulate = 0u;
       for (uint32_t c = c0; c < c1; ++c) {
-        alive = alive && (mbar_test_wait(bar_full + 8 * s, ph) ||
-                          mbar_wait_spin(bar_full + 8 * s, ph, abort_flag, a.status, 24u));
+        alive = alive && wait(bar_full + 8 * s, ph, 24u);
         __syncwarp();
         const uint32_t issue = leader && alive ? 1u : 0u;
         tc_fence_after();
@@ -268,10 +328,10 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
         const uint32_t sfa = tmem + S::kBuffers * TN + s * S::kSfCols, sfb = sfa + S::kWords * 4u;
 #pragma unroll
         for (uint32_t w = 0; w < S::kWords; ++w) {
-          copy_scales_if(issue, sfa + 4u * w, sf_lo + ((S::kOffSfa + w * kAtomBytes) >> 4), sf_hi);
+          copy_scales_if<S::kPair>(issue, sfa + 4u * w, sf_lo + ((S::kOffSfa + w * kAtomBytes) >> 4), sf_hi);
 #pragma unroll
           for (uint32_t b = 0; b < S::kBlocks; ++b)
-            copy_scales_if(issue, sfb + 4u * (w * S::kBlocks + b),
+            copy_scales_if<S::kPair>(issue, sfb + 4u * (w * S::kBlocks + b),
                            sf_lo + ((S::kOffSfb + b * S::kSf + w * kAtomBytes) >> 4), sf_hi);
         }
         const uint32_t steps = c + 1u == a.nchunk ? a.last_steps : 4u;
@@ -280,18 +340,18 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
         for (uint32_t k = 0; k < 4u; ++k) {
           constexpr uint32_t kPer = FMT == SPCONVB_MXFP4 ? 2u : 1u;
           const uint32_t w = k / kPer;
-          umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, a_lo + 2u * k, b_lo + 2u * k, desc_hi,
-                              idesc_of<FMT>(TN, (k % kPer) * 2u), sfa + 4u * w,
+          umma_scaled_if<FMT, S::kPair>(issue && k < steps ? 1u : 0u, d_tmem, a_lo + 2u * k, b_lo + 2u * k, desc_hi,
+                              idesc_of<FMT>(TN, (k % kPer) * 2u, S::kRows), sfa + 4u * w,
                               sfb + 4u * w * S::kBlocks, k == 0 ? accumulate : 1u);
         }
         accumulate = 1u;
-        tc_commit_if(issue, bar_empty + 8 * s);
+        commit(issue, bar_empty + 8 * s);
         if (++s == S::kStages) {
           s = 0;
           ph ^= 1u;
         }
       }
-      tc_commit_if(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
+      commit(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
     }
     __syncwarp();
   } else {
@@ -304,7 +364,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     uint32_t tl = 0;
     for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++tl) {
       const uint32_t buf = S::kBuffers == 1 ? 0u : tl & 1u, use = S::kBuffers == 1 ? tl : tl >> 1;
-      p.row0 = (uint64_t)(tile / tiles_n) * kTileM + 32u * q;
+      p.row0 = (uint64_t)(tile / tiles_n) * S::kRows + cta * kTileM + 32u * q;
       const uint32_t col = (tile % tiles_n) * TN + first;
       float bias[S::kPatches];
 #pragma unroll
@@ -324,7 +384,12 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
       tmem_ld_wait();
       tc_fence_before();  // no more reads of this accumulator by this warp
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+      if (lane == 0) {
+        if (S::kPair && cta != 0u)
+          mbar_arrive_at(bar_tempty + 8 * buf, 0u);
+        else
+          mbar_arrive(bar_tempty + 8 * buf);
+      }
       if (SPLIT) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) part[i] = v[0][i];
@@ -385,9 +450,14 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     }
     __syncthreads();
   }
+  __syncwarp();
+  if (S::kPair) cluster_sync();  // nobody leaves while its memory is read or its barriers are signed
   if (warp == kMmaWarp) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    if (S::kPair)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
 }
 
@@ -418,39 +488,40 @@ int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, c
                                           (int)S::kSmem));
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
-  if (SPLIT) {
-    cudaLaunchAttribute at[2] = {};
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = a.split;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles * a.split);
-    cfg.blockDim = dim3(kCtaThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
-    cfg.stream = st;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    SPCONVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_linear_kernel<FMT, TN, SPLIT>, a, map));
+  const uint32_t ctas = SPLIT ? a.split : S::kCtas;  // of a cluster
+  const uint32_t grid = SPLIT ? tiles * ctas : tiles < kSmCount / ctas ? tiles * ctas : (uint32_t)kSmCount;
+  if (ctas == 1u) {
+    SPCONVB_CUDA_TRY(launch_pdl(fp4_linear_kernel<FMT, TN, SPLIT>, dim3(grid), dim3(kCtaThreads), S::kSmem, st, a, map));
     return SPCONVB_OK;
   }
-  const uint32_t grid = tiles < (uint32_t)kSmCount ? tiles : (uint32_t)kSmCount;
-  SPCONVB_CUDA_TRY(launch_pdl(fp4_linear_kernel<FMT, TN, SPLIT>, dim3(grid), dim3(kCtaThreads), S::kSmem, st, a, map));
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = ctas;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kCtaThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  SPCONVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_linear_kernel<FMT, TN, SPLIT>, a, map));
   return SPCONVB_OK;
 }
 
 template <int FMT>
 int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream_t st) {
-  const uint64_t tm = (rows + kTileM - 1) / kTileM;
-  auto tiles = [&](uint32_t tn) { return tm * ((a.o.cout + tn - 1) / tn); };
+  auto tiles = [&](uint64_t tm, uint64_t tn) { return (rows + tm - 1) / tm * ((a.o.cout + tn - 1) / tn); };
   a.split = 1;
-  auto cost = [&](uint32_t tn, uint64_t tile, uint64_t chunk) {
-    return (tiles(tn) + kSmCount - 1) / kSmCount * (tile + chunk * a.nchunk);
+  auto cost = [&](uint64_t t, uint64_t places, uint64_t tile, uint64_t chunk) {
+    return (t + places - 1) / places * (tile + chunk * a.nchunk);
   };
-  if (a.o.cout > 128u && cost(256, 4400, 820) < cost(128, 2000, 600))
-    return launch_linear<FMT, 256, false>(a, map, (uint32_t)tiles(256), st);
-  const uint64_t t = tiles(128);
+  if (a.o.cout > 128u &&
+      cost(tiles(256, 256), kSmCount / 2, 5000, 580) + 1500u < cost(tiles(128, 128), kSmCount, 2000, 600))
+    return launch_linear<FMT, 256, false>(a, map, (uint32_t)tiles(256, 256), st);
+  const uint64_t t = tiles(128, 128);
   if (a.nchunk >= 32u)
     while (a.split < 8u && 2u * a.split * t <= (uint64_t)kSmCount && a.nchunk >= 8u * a.split) a.split *= 2u;
   return a.split > 1u ? launch_linear<FMT, 128, true>(a, map, (uint32_t)t, st)

@@ -14,48 +14,78 @@ using namespace umma_detail;
 // B format (1 = e2m1), [17,23) N >> 3, [23] scale format (0 = e4m3, 1 = e8m0), [27,29) M >> 7, [29,31) half of the scale
 // word of A; both operands K-major, K = 64.
 template <int FMT>
-__device__ __forceinline__ constexpr uint32_t idesc_of(uint32_t n, uint32_t sf_id) {
+__device__ __forceinline__ constexpr uint32_t idesc_of(uint32_t n, uint32_t sf_id, uint32_t m = 128) {
   return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) |
-         ((FMT == SPCONVB_MXFP4 ? 1u : 0u) << 23) | (1u << 27) | (sf_id << 29);
+         ((FMT == SPCONVB_MXFP4 ? 1u : 0u) << 23) | ((m >> 7) << 27) | (sf_id << 29);
 }
 
-// One MMA, M = 128, K = 64, by predicate from one lane of a converged warp.
-template <int FMT>
+// One MMA, K = 64, by predicate from one lane of a converged warp: M = 128 on this SM, or with PAIR M = 256 on the two SMs of a
+// cluster of two.  Of a pair, each SM holds its own 128 rows of A, its half of B's columns, the scales of its rows and those of all
+// columns, at the same places in both; one SM issues for both, here and in the two functions below.
+#define FP4_MMA(GROUP, KIND)                                                                                               \
+  asm volatile(                                                                                                            \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"                                               \
+      "setp.ne.b32 q, %6, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"                                          \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %4, [%7], [%8], p;\n\t}" ::"r"(d_tmem),            \
+      "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(issue), "r"(sfa), "r"(sfb)                      \
+      : "memory")
+template <int FMT, bool PAIR = false>
 __device__ __forceinline__ void umma_scaled_if(uint32_t issue, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
                                                uint32_t desc_hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                                uint32_t accumulate) {
   if (FMT == SPCONVB_MXFP4) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "setp.ne.b32 q, %6, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%7], [%8], p;\n\t}" ::"r"(
-            d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(issue), "r"(sfa), "r"(sfb)
-        : "memory");
+    if (PAIR)
+      FP4_MMA("2", "mxf4.block_scale.scale_vec::2X");
+    else
+      FP4_MMA("1", "mxf4.block_scale.scale_vec::2X");
   } else {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "setp.ne.b32 q, %6, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], da, db, %4, [%7], [%8], p;\n\t}" ::"r"(
-            d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(issue), "r"(sfa), "r"(sfb)
-        : "memory");
+    if (PAIR)
+      FP4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    else
+      FP4_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
   }
 }
+#undef FP4_MMA
 
 // 128 rows of scale words (512 bytes: row r's word at (r % 32) * 16 + (r / 32) * 4) into four columns of tensor memory, the
-// word of row r in lane r % 32 (of every quadrant of lanes) and column r / 32.
+// word of row r in lane r % 32 (of every quadrant of lanes) and column r / 32.  With PAIR each SM of the pair copies its own.
+#define FP4_COPY(GROUP)                                                            \
+  asm volatile(                                                                    \
+      "{\n\t.reg .pred q;\n\t.reg .b64 d;\n\tsetp.ne.b32 q, %3, 0;\n\tmov.b64 d, {%1, %2};\n\t" \
+      "@q tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem), \
+      "r"(desc_lo), "r"(desc_hi), "r"(issue)                                       \
+      : "memory")
+template <bool PAIR = false>
 __device__ __forceinline__ void copy_scales_if(uint32_t issue, uint32_t tmem, uint32_t desc_lo, uint32_t desc_hi) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\t.reg .b64 d;\n\tsetp.ne.b32 q, %3, 0;\n\tmov.b64 d, {%1, %2};\n\t"
-      "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem),
-      "r"(desc_lo), "r"(desc_hi), "r"(issue)
-      : "memory");
+  if (PAIR)
+    FP4_COPY("2");
+  else
+    FP4_COPY("1");
 }
+#undef FP4_COPY
 // Its shared-memory descriptor: no swizzle, groups of 8 rows of 16 bytes 128 bytes apart.
 __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) |
          ((uint64_t)1 << 46);
+}
+
+// Commits what this thread issued for the pair to the barrier at the same place in both of its CTAs.
+__device__ __forceinline__ void tc_commit_pair_if(uint32_t issue, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b16 m;\n\tsetp.ne.b32 q, %1, 0;\n\tmov.b16 m, 3;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(bar),
+      "r"(issue)
+      : "memory");
+}
+// Arrives on the barrier at the same place in CTA `rank` of the cluster.  What it tells of is tensor memory, or shared memory of the
+// arriving CTA whose writers have fenced it for the tensor core of that SM, which is what reads it; a release at the scope of the cluster
+// would wait for the thread's global stores too, and cost 1 200 cycles.
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar),
+      "r"(rank)
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {

@@ -272,6 +272,75 @@ def test_linear_to_4_bits_is_the_definition(fmt, out_fmt, rows, cin, cout):
         _check_codes(got, *ref.quantize(y.astype(np.float32), out_fmt, g))
 
 
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("rows,cin,cout,counts", [
+    (1300, 1100, 1800, (1300, 0, 1, 128, 129, 257, 1000)),  # tiles of 256 x 256: the last one of 20 rows, of 8 channels
+    (1281, 1281, 1928, (1281, 1280)),                       # the last one of 1 row, of 136 channels
+    (20000, 2304, 256, (20000, 18945)),                     # several tiles a pair of SMs
+])
+def test_large_linear_layers(fmt, rows, cin, cout, counts):
+    ops = _ops()
+    x, w = _features(rows, cin, 1, 0.3), _features(cout, cin, 2, 0.3) / np.float32(np.sqrt(cin))
+    gx, gw = _scale(x, fmt), _scale(w, fmt)
+    q, xv = _quantized(x, fmt, gx)
+    wc, ws = ref.quantize(w, fmt, gw)
+    bias = np.random.default_rng(3).standard_normal(cout).astype(np.float32)
+    wq = ops.Fp4Weights(w, fmt, gw, bias)
+    y, off = ref.product(xv, ref.values(wc, ws, fmt, cin), float(np.float32(gx * gw)), bias, True)
+    st = ops.new_status()
+    for n in counts:
+        out = torch.full((rows, cout), 7.0, dtype=torch.float16, device="cuda")
+        ops.fp4_linear(q, ops.device_count(n), wq, act=ops.ACT_RELU, out=out, status=st)
+        got = out.cpu().numpy().astype(np.float64)
+        assert (np.abs(got[:n] - y[:n]) <= off[:n]).all(), n
+        assert (got[n:] == 7.0).all(), n
+        assert int(st[0]) == 0
+
+
+@pytest.mark.parametrize("out_fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_large_linear_layers_to_4_bits(fmt, out_fmt):
+    ops = _ops()
+    rows, cin, cout = 1300, 1100, 1800
+    x, w = _exact_rows(rows, cin, 1), _exact_rows(cout, cin, 2)
+    q, xv = _quantized(x, fmt, 1.0)
+    g = 1.0 if out_fmt == ref.MX else 0.0625
+    got = ops.fp4_linear(q, ops.device_count(rows), ops.Fp4Weights(w, fmt, 1.0), out_fmt=out_fmt, out_tensor_scale=g)
+    _check_codes(got, *ref.quantize((xv @ w.T.astype(np.float64)).astype(np.float32), out_fmt, g))
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_large_linear_layers_replayed_on_two_streams(fmt):
+    """Captured, replayed with other inputs and counts while another stream runs a layer of its own: the bits of a call alone."""
+    ops = _ops()
+    rows, cin, cout = 1300, 1100, 1800
+    xs = [_features(rows, cin, i, 0.3) for i in range(3)]
+    g = max(_scale(x, fmt) for x in xs)
+    w = _features(cout, cin, 5, 0.3) / np.float32(np.sqrt(cin))
+    wq = ops.Fp4Weights(w, fmt, _scale(w, fmt))
+    qs = [_quantized(x, fmt, g)[0] for x in xs]
+    alone = [ops.fp4_linear(q, ops.device_count(rows), wq).cpu() for q in qs]
+    q, n_ptr = _quantized(xs[0], fmt, g)[0], ops.device_count(rows)
+    side = torch.cuda.Stream()
+    out = torch.empty((rows, cout), dtype=torch.float16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.fp4_linear(q, n_ptr, wq, out=out)
+    for i, n in ((1, 1300), (2, 700), (0, 1), (1, 0), (2, 1300)):
+        q.codes.copy_(qs[i].codes)
+        q.scales.copy_(qs[i].scales)
+        n_ptr.fill_(n)
+        out.fill_(3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            other = [ops.fp4_linear(qs[0], ops.device_count(rows), wq) for _ in range(4)]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.cpu()
+        assert torch.equal(got[:n], alone[i][:n]) and (got[n:] == 3.0).all()
+        assert all(torch.equal(o.cpu(), alone[0]) for o in other)
+
+
 @pytest.mark.parametrize("out_fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("n,cin,cout", [(1, 64, 64), (100, 64, 64), (3000, 64, 24), (3001, 128, 128), (30000, 64, 100),
@@ -589,6 +658,25 @@ def test_bounded_waits_run_out_and_the_context_survives(fmt):
     assert torch.equal(ops.fp4_conv(q, m, n_ptr, wq, status=st), good)
     assert torch.equal(ops.fp4_linear(q, n_ptr, lin, status=st), good_lin)
     assert torch.equal(ops.fp4_linear(qt, nt, tall, status=st), good_tall)
+    assert int(st[0]) == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_bounded_waits_of_a_large_linear_layer(fmt):
+    """Copies withheld at the first chunk, inside a tile and at a later tile: the launch ends with the status bit, the next one is right."""
+    from lidar_ai_solution_b200 import cabi
+    ops = _ops()
+    rows, cin, cout = 20000, 2304, 256
+    q, _ = _quantized(_features(rows, cin, 1, 0.1), fmt, 1.0)
+    wq, n_ptr = ops.Fp4Weights(_features(cout, cin, 2, 0.1), fmt, 1.0), ops.device_count(rows)
+    good = ops.fp4_linear(q, n_ptr, wq)
+    for at in (1, 4, 9):
+        st = ops.new_status()
+        ops.fp4_linear(q, n_ptr, wq, status=st, wait_test=at)
+        torch.cuda.synchronize()
+        assert int(st[0]) == cabi.ST_TIMEOUT
+    st = ops.new_status()
+    assert torch.equal(ops.fp4_linear(q, n_ptr, wq, status=st), good)
     assert int(st[0]) == 0
 
 
