@@ -8,19 +8,24 @@
 //
 //   0-15   epilogue: a lane owns a row, a warp its quadrant of 32 and 32 channels; with 64 channels two sets of warps take the
 //          tiles in turn
-//   16     allocates tensor memory, copies the chunk's scales there, issues its MMAs
+//   16     allocates tensor memory, copies a chunk's scales there, issues its MMAs
 //   17     one lane: the weights, a bulk copy of codes and scales a chunk, or once where all chunks fit
 //   18-25  producers, two groups of four that take the chunks in turn; a warp owns 32 rows, a thread one 16-byte segment of 8
 //          of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, which arrive on the stage's barrier by
 //          themselves.  A missing neighbour has zeros for scales; its codes stay what they were (any sixteen values are numbers, and times
 //          an e4m3 scale of 0 they are 0), except in MXFP4, whose smallest scale is not 0
+//   26     64 channels: every second stage's copies and MMAs, into accumulators of its own, which the epilogue adds to the others (a sum of
+//          two, whichever is which).  One warp's waits, fences and commits for a stage then pass beside the other's MMAs
 //
 // What bounds it.  A chunk of 128 rows costs the tensor pipe 331 cycles (128 channels) or 267 (64), its 48 copies about 400 in the
 // load-store pipe, and shared memory about 600 in the wide layer (18 KB of rows and 18 of weights written, 32 read by the MMAs); in the kernel
-// it takes 690, of which half goes away without the gather and the epilogue.  120 000 rows, us, MXFP4 / NVFP4: 64 -> 64 24.8 / 23.9,
-// 128 -> 128 41.1 / 42.4 (twice the scale words), with a residual 26.3 / 25.2 and 44.7 / 45.6; 14 000 rows 64 -> 64 6.9.  Zeros for the codes of
-// missing neighbours, too, cost NVFP4 4 % (24.8, 43.9).  Stages of two chunks because every wait, fence and commit is paid once
-// a stage (one chunk a stage: 28.7, 55.9).
+// it takes 690.  120 000 rows, us, MXFP4 / NVFP4: 64 -> 64 24.3 / 23.1 (with one warp for the MMAs 25.2 / 24.3, 4-bit rows out 24.0 / 23.7 and
+// 26.1 / 26.4), 128 -> 128 42.5 / 44.0 (twice the scale words), with a residual 25.7 / 24.1 and 46.0 / 47.8; 14 000 rows 64 -> 64 6.6.
+// Without the gather of the codes 64 -> 64 takes 19.9, without the scales' 21.0, without the output 20.7: they share the SM's issue slots and
+// its load-store pipe.  Zeros for the codes of missing neighbours, too, cost NVFP4 4 %.  Stages of two chunks because every wait,
+// fence and commit is paid once a stage (one chunk a stage: 28.7, 55.9).  128 channels with two warps for the MMAs take 45.7 / 46.5: their four
+// accumulators leave no room for scales, and a single pair is drained with no MMA beside it.  With a tile on two SMs that share the weights
+// they take 41.4 / 43.8, and 14 000 rows 10.4 / 10.9 in place of 9.4 / 10.0.
 //
 // Within the 32 rows of a warp, row 8 slot + i of the tile lies at 4 i + slot of the operand: the words of scales that
 // the 32 lanes write at the same time then lie in eight groups of four banks and not in two.
@@ -34,8 +39,8 @@ constexpr uint32_t kTileRows = 128;
 constexpr int kEpiWarps = 16, kMmaWarp = 16, kWeightWarp = 17, kProdWarp0 = 18;
 constexpr uint32_t kGroups = 2;
 constexpr uint32_t kPair = 2;
-constexpr int kCtaThreads = 32 * (kProdWarp0 + 4 * (int)kGroups);
-constexpr uint32_t kTmemCols = 512;
+constexpr int kMmaWarp2 = kProdWarp0 + 4 * (int)kGroups;
+constexpr int cta_threads(int cout) { return 32 * (kMmaWarp2 + (cout == 64 ? 1 : 0)); }
 constexpr uint32_t kRingBytes = 191 * 1024;
 constexpr size_t kSmemBytes = kRingBytes + kEpiWarps * kStageBytes + 1024 + 512;
 
@@ -68,7 +73,7 @@ __device__ __forceinline__ void cp_async16_if(uint32_t make, uint32_t dst, const
 
 // CP: stored channels of an input row.  COUT: output channels, rounded up to 64 or 128.  RES: with a residual.
 template <int FMT, int CP, int COUT, bool RES>
-__global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs a) {
+__global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const ConvArgs a) {
   constexpr int RB = CP / 2;                       // bytes of a row's codes
   constexpr int OPC = 128 / RB, SPO = RB / 16;     // taps a chunk, 16-byte segments a tap
   constexpr uint32_t W = FMT == SPCONVB_MXFP4 && CP != 64 ? 2 : 4;  // scale words a row and chunk
@@ -82,7 +87,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   constexpr uint32_t kWeightStage = kPair * kWeightBytes;
   constexpr uint32_t kSfCols = kPair * 8 * W;  // of a stage in tensor memory: rows, weights, chunk by chunk
   constexpr uint32_t kDrain = COUT / 32 * 4;   // warps that drain a tile
-  constexpr uint32_t kDeepest = (kTmemCols - 2 * COUT) / kSfCols < kMaxStages ? (kTmemCols - 2 * COUT) / kSfCols : kMaxStages;
+  constexpr uint32_t kMmas = COUT == 64 ? 2 : 1;   // warps that issue MMAs, each into an accumulator of its own
+  constexpr uint32_t kAccCols = 2 * kMmas * COUT;  // accumulators of two tiles
+  constexpr uint32_t kDeepest = (kTmemCols - kAccCols) / kSfCols < kMaxStages / kMmas ? (kTmemCols - kAccCols) / kSfCols : kMaxStages / kMmas;
 
   const int kbytes = a.kvol * RB;
   const int nchunk = (kbytes + 127) / 128;
@@ -104,10 +111,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   const uint32_t lane = threadIdx.x & 31;
 
   if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc_all<false>(smem_u32(tmem_holder));
   }
   pdl_wait_and_trigger();
   const uint32_t n_out = __shfl_sync(0xffffffffu, min(load_in_order(a.n_out_ptr), a.cap), 0);
@@ -121,8 +125,12 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   // Two rings share the buffer, rows with their scales (three stages or more) and weights with theirs.  Weights that fit beside
   // three stages of rows stay.
   const bool resident = npair <= kMaxStages && kRingBytes >= (uint32_t)npair * kWeightStage + 3u * kRowStage;
-  const uint32_t nwst = resident ? (uint32_t)npair : min((uint32_t)kMaxStages, (kRingBytes - 3u * kRowStage) / kWeightStage);
+  const uint32_t nwst = resident ? (uint32_t)npair : min((uint32_t)kMaxStages, (kRingBytes - 3u * kRowStage) / kWeightStage / kMmas * kMmas);
   const uint32_t nst = min(kDeepest, (kRingBytes - nwst * kWeightStage) / kRowStage);
+  // A stage has a pair of barriers for each of the MMA warps, used in turn.  The warps take the pairs of chunks in turn too, and so all
+  // phases of a barrier are one warp's (and one producer group's), in order: nobody can look at one two phases early, where its parity
+  // would say what it said two before.
+  const uint32_t nbar = kMmas * nst;
   const uint32_t sW = smem_u32(smem), sR = sW + nwst * kWeightStage;
 
   if (threadIdx.x < kMaxStages) {
@@ -131,7 +139,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     mbar_init(bar_wfull + 8 * threadIdx.x, 1);
     mbar_init(bar_wempty + 8 * threadIdx.x, 1);
     if (threadIdx.x < 2) {
-      mbar_init(bar_tfull + 8 * threadIdx.x, 1);
+      mbar_init(bar_tfull + 8 * threadIdx.x, kMmas);
       mbar_init(bar_tempty + 8 * threadIdx.x, kDrain);
     }
     if (threadIdx.x == 0) *abort_flag = 0u;
@@ -174,6 +182,76 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       }
     }
     __syncwarp();
+  } else if (warp == kMmaWarp || warp == kMmaWarp2) {
+    // ------------------------------------------------------------ MMA issue
+    const bool leader = elect_one();
+    const uint64_t wdesc0 = make_smem_desc(sW), rdesc0 = make_smem_desc(sR);
+    const uint32_t desc_hi = (uint32_t)(wdesc0 >> 32);
+    const uint32_t sf_hi = (uint32_t)(scale_desc(sW) >> 32), sfw0 = (uint32_t)scale_desc(sW), sfr0 = (uint32_t)scale_desc(sR);
+    bool alive = true;
+    uint32_t b = 0, ws = 0, ph = 0, wph = 0, tl = 0;
+    const uint32_t which = warp == kMmaWarp ? 0u : 1u;
+    uint32_t turn = which;  // 0: the next stage is this warp's
+    for (uint32_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++tl) {
+      const uint32_t buf = tl & 1u;
+      alive = alive && mbar_wait_spin(bar_tempty + 8 * buf, ((tl >> 1) & 1u) ^ 1u, abort_flag, a.status, 32u);
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + (kMmas * buf + which) * COUT;
+      uint32_t accumulate = 0u;
+#pragma unroll 1
+      for (int j = 0; j < nchunk; j += kPair) {
+        if (kMmas == 1u || turn == 0u) {
+          const uint32_t s = b >= nst ? b - nst : b;
+          const uint32_t wp = resident ? 0u : wph;
+          if (!resident || tl < 2u)
+            alive = alive && (mbar_test_wait(bar_wfull + 8 * ws, wp) ||
+                              mbar_wait_spin(bar_wfull + 8 * ws, wp, abort_flag, a.status, 37u));
+          alive = alive && (mbar_test_wait(bar_full + 8 * b, ph) ||
+                            mbar_wait_spin(bar_full + 8 * b, ph, abort_flag, a.status, 33u));
+          __syncwarp();
+          const uint32_t issue = leader && alive ? 1u : 0u;
+          fence_proxy_async();  // rows come through the generic proxy, MMAs and copies read through the async one
+          tc_fence_after();
+#pragma unroll
+          for (uint32_t c = 0; c < kPair; ++c) {
+            if (j + (int)c >= nchunk) break;
+            const uint32_t w_at = (ws * kWeightStage + c * kWeightBytes) >> 4, r_at = (s * kRowStage + c * kCodes) >> 4;
+            const uint32_t f_at = (s * kRowStage + kSfOff + c * W * kAtomBytes) >> 4;
+            // a place for every stage: it is filled again only when the MMAs that read its scales are complete
+            const uint32_t sfr = tmem_base + kAccCols + s * kSfCols + c * 8u * W, sfw = sfr + 4u * W;
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) {
+              copy_scales_if(issue, sfr + 4u * w, sfr0 + f_at + ((w * kAtomBytes) >> 4), sf_hi);
+              copy_scales_if(issue, sfw + 4u * w, sfw0 + w_at + ((COUT * 128u + w * kAtomBytes) >> 4), sf_hi);
+            }
+            const uint32_t steps = j + (int)c + 1 == nchunk ? last_steps : 4u;
+            const uint32_t wd = (uint32_t)wdesc0 + w_at, rd = (uint32_t)rdesc0 + r_at;
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+              const uint32_t w = k / kSteps;
+              umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, rd + 2u * k, wd + 2u * k, desc_hi,
+                                  idesc_of<FMT>(COUT, (k % kSteps) * 2u), sfr + 4u * w, sfw + 4u * w,
+                                  k == 0 ? accumulate : 1u);
+            }
+            accumulate = 1u;
+          }
+          tc_commit_if(issue, bar_empty + 8 * b);
+          if (!resident) tc_commit_if(issue, bar_wempty + 8 * ws);
+        }
+        turn ^= 1u;
+        if (++b == nbar) {
+          b = 0;
+          ph ^= 1u;
+        }
+        if (++ws == nwst) {
+          ws = 0;
+          wph ^= 1u;
+        }
+      }
+      tc_commit_if(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
+    }
+    __syncwarp();
   } else if (warp >= kProdWarp0) {
     // ------------------------------------------------------------ producers
     const uint32_t pw_all = (uint32_t)(warp - kProdWarp0);
@@ -214,7 +292,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     advance(tile, j, (int)grp);
     uint32_t ntile = tile;
     int nj = j;
-    uint32_t it = grp, s = grp % nst, ph = (grp / nst) & 1u;
+    uint32_t it = grp, b = grp, ph = 0u;
     int32_t idx[kPair][8];
     auto load_pair = [&]() {
 #pragma unroll
@@ -223,7 +301,10 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     };
     auto step = [&]() -> bool {
       if (tile >= ntiles) return false;
-      if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, abort_flag, a.status, 31u)) return false;
+      // the use of the stage before this one, nst pairs ago
+      const bool wrap = b < nst;
+      const uint32_t s = wrap ? b : b - nst;
+      if (!mbar_wait(bar_empty + 8 * (wrap ? b + nbar - nst : b - nst), ph ^ (wrap ? 1u : 0u), abort_flag, a.status, 31u)) return false;
 #pragma unroll
       for (uint32_t c = 0; c < kPair; ++c) {
         const int chunk = j * (int)kPair + (int)c;
@@ -254,13 +335,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
           cp_async4(to + (kParts * i + part) * 64u, src + (int64_t)sr * kPitch, (uint32_t)sr < a.in_rows ? 4u : 0u);
         }
       }
-      if (!(a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) cp_async_arrive_noinc(bar_full + 8 * s);
+      if (!(a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) cp_async_arrive_noinc(bar_full + 8 * b);
       load_pair();
       advance(tile, j, kGroups);
       it += kGroups;
-      s += kGroups;
-      if (s >= nst) {
-        s -= nst;
+      b += kGroups;
+      if (b >= nbar) {
+        b -= nbar;
         ph ^= 1u;
       }
       return true;
@@ -270,69 +351,6 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
     while (step()) {
     }
     cp_async_wait_all();  // nothing of this thread may still be writing when the CTA exits
-    __syncwarp();
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issue
-    const bool leader = elect_one();
-    const uint64_t wdesc0 = make_smem_desc(sW), rdesc0 = make_smem_desc(sR);
-    const uint32_t desc_hi = (uint32_t)(wdesc0 >> 32);
-    const uint32_t sf_hi = (uint32_t)(scale_desc(sW) >> 32), sfw0 = (uint32_t)scale_desc(sW), sfr0 = (uint32_t)scale_desc(sR);
-    bool alive = true;
-    uint32_t s = 0, ws = 0, ph = 0, wph = 0, tl = 0;
-    for (uint32_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++tl) {
-      const uint32_t buf = tl & 1u;
-      alive = alive && mbar_wait_spin(bar_tempty + 8 * buf, ((tl >> 1) & 1u) ^ 1u, abort_flag, a.status, 32u);
-      __syncwarp();
-      tc_fence_after();
-      const uint32_t d_tmem = tmem_base + buf * COUT;
-      uint32_t accumulate = 0u;
-#pragma unroll 1
-      for (int j = 0; j < nchunk; j += kPair) {
-        if (!resident || tl == 0u)
-          alive = alive && (mbar_test_wait(bar_wfull + 8 * ws, wph) ||
-                            mbar_wait_spin(bar_wfull + 8 * ws, wph, abort_flag, a.status, 37u));
-        alive = alive && (mbar_test_wait(bar_full + 8 * s, ph) ||
-                          mbar_wait_spin(bar_full + 8 * s, ph, abort_flag, a.status, 33u));
-        __syncwarp();
-        const uint32_t issue = leader && alive ? 1u : 0u;
-        fence_proxy_async();  // rows come through the generic proxy, MMAs and copies read through the async one
-        tc_fence_after();
-#pragma unroll
-        for (uint32_t c = 0; c < kPair; ++c) {
-          if (j + (int)c >= nchunk) break;
-          const uint32_t w_at = (ws * kWeightStage + c * kWeightBytes) >> 4, r_at = (s * kRowStage + c * kCodes) >> 4;
-          const uint32_t f_at = (s * kRowStage + kSfOff + c * W * kAtomBytes) >> 4;
-          // a place for every stage: it is filled again only when the MMAs that read its scales are complete
-          const uint32_t sfr = tmem_base + 2u * COUT + s * kSfCols + c * 8u * W, sfw = sfr + 4u * W;
-#pragma unroll
-          for (uint32_t w = 0; w < W; ++w) {
-            copy_scales_if(issue, sfr + 4u * w, sfr0 + f_at + ((w * kAtomBytes) >> 4), sf_hi);
-            copy_scales_if(issue, sfw + 4u * w, sfw0 + w_at + ((COUT * 128u + w * kAtomBytes) >> 4), sf_hi);
-          }
-          const uint32_t steps = j + (int)c + 1 == nchunk ? last_steps : 4u;
-          const uint32_t wd = (uint32_t)wdesc0 + w_at, rd = (uint32_t)rdesc0 + r_at;
-#pragma unroll
-          for (uint32_t k = 0; k < 4u; ++k) {
-            const uint32_t w = k / kSteps;
-            umma_scaled_if<FMT>(issue && k < steps ? 1u : 0u, d_tmem, rd + 2u * k, wd + 2u * k, desc_hi,
-                                idesc_of<FMT>(COUT, (k % kSteps) * 2u), sfr + 4u * w, sfw + 4u * w,
-                                k == 0 ? accumulate : 1u);
-          }
-          accumulate = 1u;
-        }
-        tc_commit_if(issue, bar_empty + 8 * s);
-        if (!resident) tc_commit_if(issue, bar_wempty + 8 * ws);
-        if (++s == nst) {
-          s = 0;
-          ph ^= 1u;
-        }
-        if (++ws == nwst) {
-          ws = 0;
-          wph ^= 1u;
-        }
-      }
-      tc_commit_if(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
-    }
     __syncwarp();
   } else {
     // ------------------------------------------------------------- epilogue
@@ -360,8 +378,21 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
       if (!ok) break;
       tc_fence_after();
       uint32_t v[32];
-      tmem_ld32(tmem_base + ((32u * q) << 16) + buf * COUT + p.col, v);
-      tmem_ld_wait();
+      const uint32_t acc = tmem_base + ((32u * q) << 16) + kMmas * buf * COUT + p.col;
+      if (kMmas == 1u || npair == 1) {
+        tmem_ld32(acc + (kMmas == 1u ? 0u : (tl & 1u) * COUT), v);
+        tmem_ld_wait();
+      } else {
+        tmem_ld32(acc, v);
+#pragma unroll
+        for (uint32_t h = 0; h < 32u; h += 16u) {
+          uint32_t u[16];
+          tmem_ld16(acc + COUT + h, u);
+          tmem_ld_wait();
+#pragma unroll
+          for (uint32_t i = 0; i < 16u; ++i) v[h + i] = __float_as_uint(__uint_as_float(v[h + i]) + __uint_as_float(u[i]));
+        }
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
@@ -382,7 +413,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1) fp4_conv_kernel(const ConvArgs
   }
   if (warp == kMmaWarp) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+    tmem_free_all<false>(tmem_base);
   }
 }
 
@@ -398,7 +429,7 @@ int launch_conv(const ConvArgs& a, uint32_t launch_rows, cudaStream_t st) {
   }
   const uint32_t tiles = (launch_rows + 31) / 32;  // the kernel picks the tile height
   const uint32_t grid = tiles < (uint32_t)kSmCount ? (tiles ? tiles : 1u) : (uint32_t)kSmCount;
-  SPCONVB_CUDA_TRY(launch_pdl(fp4_conv_kernel<FMT, CP, COUT, RES>, dim3(grid), dim3(kCtaThreads), kSmemBytes, st, a));
+  SPCONVB_CUDA_TRY(launch_pdl(fp4_conv_kernel<FMT, CP, COUT, RES>, dim3(grid), dim3(cta_threads(COUT)), kSmemBytes, st, a));
   return SPCONVB_OK;
 }
 template <int FMT, int CP, int COUT>

@@ -49,7 +49,6 @@ constexpr uint64_t kFewProducts = 1ull << 26;
 constexpr int kEpiWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kScaleWarp0 = 18, kWeightWarp = 22;
 constexpr int kCtaThreads = 32 * 23;
 constexpr uint32_t kTileM = 128;
-constexpr uint32_t kTmemCols = 512;
 
 struct LinearArgs {
   const uint8_t* scales;
@@ -93,9 +92,6 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
   return v;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 // SPLIT: the CTAs of a cluster share a tile's K (a kernel of its own: the sums kept for it would be spilled in the other).
 template <int FMT, int TN, bool SPLIT>
@@ -130,17 +126,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     fence_proxy_async();
   }
   if (warp == kMmaWarp) {
-    if (S::kPair) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                   "r"(kTmemCols)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                   "r"(kTmemCols)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    tmem_alloc_all<S::kPair>(smem_u32(tmem_holder));
   }
   pdl_wait_and_trigger();
   const uint32_t n = __shfl_sync(0xffffffffu, min(load_in_order(a.n_ptr), a.cap), 0);
@@ -298,12 +284,6 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     auto wait = [&](uint32_t bar, uint32_t parity, uint32_t where) {
       return mbar_test_wait(bar, parity) || mbar_wait_spin(bar, parity, abort_flag, a.status, where);
     };
-    auto commit = [&](uint32_t go, uint32_t bar) {
-      if (S::kPair)
-        tc_commit_pair_if(go, bar);
-      else
-        tc_commit_if(go, bar);
-    };
     const bool leader = elect_one();
     const uint64_t d0 = make_smem_desc(s0);
     const uint32_t desc_hi = (uint32_t)(d0 >> 32);
@@ -345,13 +325,13 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
                               sfb + 4u * w * S::kBlocks, k == 0 ? accumulate : 1u);
         }
         accumulate = 1u;
-        commit(issue, bar_empty + 8 * s);
+        commit_if<S::kPair>(issue, bar_empty + 8 * s);
         if (++s == S::kStages) {
           s = 0;
           ph ^= 1u;
         }
       }
-      commit(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
+      commit_if<S::kPair>(leader && alive ? 1u : 0u, bar_tfull + 8 * buf);
     }
     __syncwarp();
   } else {
@@ -454,10 +434,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   if (S::kPair) cluster_sync();  // nobody leaves while its memory is read or its barriers are signed
   if (warp == kMmaWarp) {
     tc_fence_after();
-    if (S::kPair)
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-    else
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    tmem_free_all<S::kPair>(tmem);
   }
 }
 
@@ -490,24 +467,7 @@ int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, c
   }
   const uint32_t ctas = SPLIT ? a.split : S::kCtas;  // of a cluster
   const uint32_t grid = SPLIT ? tiles * ctas : tiles < kSmCount / ctas ? tiles * ctas : (uint32_t)kSmCount;
-  if (ctas == 1u) {
-    SPCONVB_CUDA_TRY(launch_pdl(fp4_linear_kernel<FMT, TN, SPLIT>, dim3(grid), dim3(kCtaThreads), S::kSmem, st, a, map));
-    return SPCONVB_OK;
-  }
-  cudaLaunchAttribute at[2] = {};
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = ctas;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kCtaThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = st;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  SPCONVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_linear_kernel<FMT, TN, SPLIT>, a, map));
+  SPCONVB_CUDA_TRY(launch_clusters(fp4_linear_kernel<FMT, TN, SPLIT>, grid, ctas, kCtaThreads, S::kSmem, st, a, map));
   return SPCONVB_OK;
 }
 

@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <utility>
+
 #include "fp4.cuh"
 #include "umma_common.cuh"
 
@@ -77,6 +79,35 @@ __device__ __forceinline__ void tc_commit_pair_if(uint32_t issue, uint32_t bar) 
       "r"(issue)
       : "memory");
 }
+template <bool PAIR>
+__device__ __forceinline__ void commit_if(uint32_t issue, uint32_t bar) {
+  if (PAIR)
+    tc_commit_pair_if(issue, bar);
+  else
+    tc_commit_if(issue, bar);
+}
+// All of an SM's tensor memory, by one warp; of a pair, one in either CTA.  The address is left at `holder` in shared memory.
+constexpr uint32_t kTmemCols = 512;
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc_all(uint32_t holder) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(holder), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(holder), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free_all(uint32_t tmem) {
+  if (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Arrives on the barrier at the same place in CTA `rank` of the cluster.  What it tells of is tensor memory, or shared memory of the
 // arriving CTA whose writers have fenced it for the tensor core of that SM, which is what reads it; a release at the scope of the cluster
 // would wait for the thread's global stores too, and cost 1 200 cycles.
@@ -107,6 +138,26 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
           dst),
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+
+// A launch in clusters of `ctas` (1: none) that may begin while the kernel before it ends.
+template <typename... P, typename... A>
+cudaError_t launch_clusters(void (*kernel)(P...), uint32_t grid, uint32_t ctas, uint32_t threads, size_t smem, cudaStream_t st,
+                            A&&... args) {
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = ctas;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = ctas > 1u ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
 }
 
 }  // namespace fp4
