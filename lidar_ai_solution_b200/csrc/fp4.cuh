@@ -57,6 +57,35 @@ __device__ __forceinline__ uint2 ld8(const void* p) {
   return v;
 }
 
+// Two fp32 numbers in an instruction, each rounded as by itself: what these kernels spend is issue slots.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// The largest magnitude of m >= 0 and two more.
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
 // The block scale of a block whose largest magnitude is `amax` (the bits of a float >= 0, infinity or NaN): its byte,
 // and S in fp32.  x / S of MXFP4 is a multiplication by a power of two.
 __device__ __forceinline__ uint32_t scale_mx(uint32_t amax_bits, float& s) {
@@ -71,6 +100,10 @@ __device__ __forceinline__ uint32_t scale_mx(uint32_t amax_bits, float& s) {
 __device__ __forceinline__ float quotient(float x, float d, float r) {
   const float q = __fmul_rn(x, r);
   return __fmaf_rn(__fmaf_rn(-q, d, x), r, q);
+}
+__device__ __forceinline__ F2 quotient2(F2 x, F2 minus_d, F2 r) {  // (d is given with its sign turned)
+  const F2 q = mul2(x, r);
+  return fma2(fma2(q, minus_d, x), r, q);
 }
 __host__ __device__ inline bool in_range(float d) { return d > 8.1e-28f && d < 1.2e27f; }
 
@@ -153,11 +186,15 @@ __device__ __forceinline__ void codes_of(bool mx, const float* x, float s, uint3
     fast = in_range(s) && amax < 1e30f && amax * r < 1e30f;
   }
   if (fast) {
+    const F2 r2(r, r), d2(-s, -s);
 #pragma unroll
     for (int i = 0; i < N / 8; ++i) {
       float q[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = mx ? __fmul_rn(x[8 * i + j], r) : quotient(x[8 * i + j], s, r);
+      for (int j = 0; j < 8; j += 2) {
+        const F2 x2(x[8 * i + j], x[8 * i + j + 1]);
+        (mx ? mul2(x2, r2) : quotient2(x2, d2, r2)).get(q[j], q[j + 1]);
+      }
       c[i] = codes8(q);
     }
   } else {

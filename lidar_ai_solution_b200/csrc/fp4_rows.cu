@@ -125,10 +125,12 @@ __device__ __forceinline__ uint32_t elements(const Raw<KIND>& raw, float in_scal
   // int8: byte b goes into the mantissa of 2^23 + (b + 128); a conversion instruction has an eighth of the rate
   float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t b = __byte_perm(raw.w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7650u | (uint32_t)(i % 4));
-    x[i] = __fmul_rn(__fadd_rn(__uint_as_float(b), -8388736.f), in_scale);
-    m = fmaxf(m, fabsf(x[i]));
+  for (int i = 0; i < 16; i += 2) {
+    const uint32_t w = raw.w[i / 4] ^ 0x80808080u;
+    const F2 b(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650u | (uint32_t)(i % 4))),
+               __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650u | (uint32_t)(i % 4 + 1))));
+    mul2(add2(b, F2(-8388736.f, -8388736.f)), F2(in_scale, in_scale)).get(x[i], x[i + 1]);
+    m = max_abs(m, x[i], x[i + 1]);
   }
   return __float_as_uint(m);
 }
@@ -266,7 +268,8 @@ __device__ __forceinline__ void values_of(uint2 c, uint32_t byte, float tensor_s
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 f = __half22float2(*(const __half2*)&h[i / 4][i % 4]);
-    const float a = __fmul_rn(f.x, s), b = __fmul_rn(f.y, s);
+    float a, b;
+    mul2(F2(f.x, f.y), F2(s, s)).get(a, b);
     if (KIND == SPCONVB_F16) {
       const __half2 p = __floats2half2_rn(a, b);
       v.w[i] = *(const uint32_t*)&p;
