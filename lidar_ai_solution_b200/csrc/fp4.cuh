@@ -79,10 +79,16 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-// The largest magnitude of m >= 0 and two more.
+// The largest magnitude of m >= 0 and two more; and the same where a NaN counts as the largest.
 __device__ __forceinline__ float max_abs(float m, float a, float b) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
+__device__ __forceinline__ float max_abs_nan(float m, float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
   return r;
 }
 

@@ -198,12 +198,19 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(max_nan(__uint_as_float(v[i]), 0.f));
   }
+  if (p.col + 32u > o.cout) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = p.col + i < o.cout ? v[i] : 0u;
+    for (int i = 0; i < 32; ++i) v[i] = p.col + i < o.cout ? v[i] : 0u;
+  }
   if (!live) return;
-  uint32_t amax[2] = {0u, 0u}, c[4], byte[2];
+  uint32_t amax[2], c[4], byte[2];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) amax[i / 16] = max(amax[i / 16], v[i] & 0x7fffffffu);
+  for (int h = 0; h < 2; ++h) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) m = max_abs_nan(m, __uint_as_float(v[16 * h + i]), __uint_as_float(v[16 * h + i + 1]));
+    amax[h] = __float_as_uint(m);
+  }
   const bool mx = o.mode == 1;
   if (mx) amax[0] = amax[1] = max(amax[0], amax[1]);
 #pragma unroll

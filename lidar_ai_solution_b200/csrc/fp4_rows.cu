@@ -102,13 +102,14 @@ __device__ __forceinline__ void load_staged(const uint32_t* buf, uint32_t at, ui
 template <int KIND>
 __device__ __forceinline__ uint32_t elements(const Raw<KIND>& raw, float in_scale, float (&x)[16]) {
   if (KIND == SPCONVB_F32) {
-    uint32_t m = 0u;
+    float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 16; i += 2) {
       x[i] = __uint_as_float(raw.w[i]);
-      m = max(m, raw.w[i] & 0x7fffffffu);
+      x[i + 1] = __uint_as_float(raw.w[i + 1]);
+      m = max_abs_nan(m, x[i], x[i + 1]);
     }
-    return m;
+    return __float_as_uint(m);
   }
   if (KIND == SPCONVB_F16) {
     uint32_t m = 0u;
