@@ -188,8 +188,8 @@ __device__ __forceinline__ void codes_of(bool mx, const float* x, float s, uint3
     r = s < 1.1754944e-38f ? 1.7014118346046923e38f : __uint_as_float((254u << 23) - __float_as_uint(s));
     fast = true;
   } else {
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
-    fast = in_range(s) && amax < 1e30f && amax * r < 1e30f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));  // (subnormal scales are out of range)
+    fast = in_range(s) && amax * r < 1e30f;
   }
   if (fast) {
     const F2 r2(r, r), d2(-s, -s);

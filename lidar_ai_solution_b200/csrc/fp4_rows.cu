@@ -9,9 +9,10 @@
 //   staged   all others: 256 units in a row are one contiguous piece of the fp16 / fp32 / int8 side, which passes through
 //            shared memory in 16-byte pieces
 //
-// Measured: 480 000 x 128 fp16 -> NVFP4 27.3 us (5.8 TB/s, 87 % of a copy's rate; 158 instructions a unit and warp, 68 % of the issue slots), 120 000 x
-// 128 -> MXFP4 5.6 us (out of L2); 960 000 x 64 int8 -> NVFP4 26.5 us (3.6 TB/s: three quarters of the issue slots); back to fp16
-// 27.3 us (5.8 TB/s); 200 000 rows of 100 channels, staged, 22.3 us and back 15.9.
+// Measured: 480 000 x 128 fp16 -> NVFP4 25.4 us (6.2 TB/s, 96 % of a copy's rate), 120 000 x 128 -> MXFP4 5.5 us (out of L2); 960 000 x 64
+// int8 -> NVFP4 21.7 us (4.4 TB/s: two thirds of the issue slots and of the integer pipe, whatever the occupancy); back to fp16 25.8 us
+// (6.1 TB/s); 200 000 rows of 100 channels, staged, 20.6 us and back 15.4.  A grid of 32 blocks an SM: with 16, a block had one turn or
+// two, and the last ones ran alone (back to fp16 27.5; with 6 33.5, with as many as there are turns 25.8).
 #include "fp4.cuh"
 #include "pdl.cuh"
 
@@ -193,6 +194,15 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const uint8_t* _
     constexpr int A = kAhead<KIND, WAY>;
     for (uint64_t u0 = (uint64_t)blockIdx.x * (kThreads * A); u0 < units; u0 += (uint64_t)gridDim.x * (kThreads * A)) {
       Raw<KIND> raw[A];
+      if (WAY == kFlat && u0 + kThreads * A <= units) {  // all of the block's units are there: nothing to ask (int8 -> NVFP4 23.7 -> 21.7 us)
+        const uint64_t u = u0 + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < A; ++i) load_flat<KIND>(x + (u + i * kThreads) * (16u * es), raw[i]);
+#pragma unroll
+        for (int i = 0; i < A; ++i)
+          store_unit<FMT, KIND, WAY>(g, u + i * kThreads, 0, (uint32_t)u & 1u, raw[i], in_scale, ts, codes, scales, true);
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < A; ++i) {
         const uint64_t u = u0 + i * kThreads + threadIdx.x;
@@ -413,7 +423,7 @@ Rows rows_of(int format, int channels, const void* p, uint32_t es) {
 template <int KIND>
 int blocks_of(const Rows& g, uint32_t rows) {
   const uint64_t per = kThreads * (g.way == kFlat ? kAhead<KIND, kFlat> : 1), b = ((uint64_t)rows * g.upr + per - 1) / per;
-  return (int)(b < (uint64_t)kSmCount * 16 ? b : (uint64_t)kSmCount * 16);
+  return (int)(b < (uint64_t)kSmCount * 32 ? b : (uint64_t)kSmCount * 32);
 }
 
 // One thread a 16-byte segment of the image or a word of scales.
