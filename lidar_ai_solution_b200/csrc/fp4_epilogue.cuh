@@ -16,6 +16,7 @@ struct Output {
   TensorScale ts;  // of 4-bit output
   int act, res_relu;
   int mode;    // 0: fp16, 1: MXFP4, 2: NVFP4
+  int bulk;    // fp16: whole patches go out as tensor copies
   int access;  // bytes of an fp16 row that may be stored (and of the residual, read) at once: 16, 4 or 2
 };
 
@@ -23,7 +24,7 @@ struct Output {
 // there, and a quarter of a row on the way to memory, where eight rows go at a time (a lane's own 32 bytes of 32 rows touch 32
 // lines an instruction and not 8).  Piece c (16 bytes) of row r lies at piece c ^ (r / 2 + r / 8) % 4 of its 64 bytes: free of bank conflicts
 // for lanes that have rows 0, 1, 2, ... and for lanes that have rows 0, 8, 16, 24, 1, 9, ...
-constexpr uint32_t kStageBytes = 2048 + 128;  // and behind it the patch's bias
+constexpr uint32_t kPatchBytes = 2048, kBiasBytes = 128;
 __device__ __forceinline__ uint32_t staged_at(uint32_t r, uint32_t c) {
   return r * 64u + ((c ^ ((r >> 1 ^ r >> 3) & 3u)) << 4);
 }
@@ -39,8 +40,28 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
 // Where a warp's 32 rows x 32 channels are: rows row0 .. (those below `rows` exist; this lane has row0 + own), channels col ..
 struct Patch {
   uint64_t row0, rows;
-  uint32_t col, own, lane, stage;
+  uint32_t col, own, lane, stage, bias;  // (the last two: where in shared memory)
 };
+
+// Of fp16 results, a patch all of whose rows exist leaves as one tensor copy of 32 x 32, which the next patch waits for before it writes
+// there: the lanes' four loads and stores and the wait between them are out of the way of the next tile (32 400 x 256 -> 512 12.3 us, this way
+// 9.8; 120 000 x 256 -> 256 19.9 and 15.6; 100 x 256 -> 128 3.8 and 3.6).  Its pieces lie as that copy wants them: piece c of row r at c ^ (r / 2) % 4.
+__device__ __forceinline__ uint32_t copied_at(uint32_t r, uint32_t c) { return r * 64u + ((c ^ (r >> 1 & 3u)) << 4); }
+__device__ __forceinline__ void store_patch(const CUtensorMap* map, const Patch& p) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"((int32_t)p.col),
+               "r"((int32_t)p.row0), "r"(p.stage)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// By all lanes: what this warp has stored has left shared memory; and, before the CTA ends, has been written.
+template <bool BULK>
+__device__ __forceinline__ void patch_free(const Output& o, const Patch& p) {
+  if (BULK && o.bulk && p.lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
+__device__ __forceinline__ void stores_done(const Output& o, const Patch& p) {
+  if (o.bulk && p.lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
 
 // The patch's bias on its way into shared memory (zeros where there is none): a load that the epilogue would wait for is made long
 // before it.  (Read where it is used, 14 000 rows 64 -> 64 took 8.8 us and not 6.5.)
@@ -48,13 +69,14 @@ __device__ __forceinline__ float load_bias(const Output& o, const Patch& p) {
   return o.bias && p.col + p.lane < o.cout ? __uint_as_float(load_in_order((const uint32_t*)o.bias + p.col + p.lane)) : 0.f;
 }
 __device__ __forceinline__ void stage_bias(const Patch& p, float b) {
-  asm volatile("st.shared.f32 [%0], %1;" ::"r"(p.stage + 2048u + 4u * p.lane), "f"(b) : "memory");
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(p.bias + 4u * p.lane), "f"(b) : "memory");
 }
 
 // The residual on its way into the patch's shared memory, in program order: it may be what the launch before wrote.  (Rows that do
 // not start on 16 bytes go by pairs of channels, two rows an instruction, or by single ones.)
+template <bool BULK>
 __device__ __forceinline__ void prefetch_residual(const Output& o, const Patch& p) {
-  __syncwarp();  // what was there is read
+  patch_free<BULK>(o, p);  // what was there is read
   if (o.access >= 16) {
     const uint32_t c = p.col + 8u * (p.lane % 4u);
 #pragma unroll
@@ -108,17 +130,17 @@ __device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
 
 // Sums of 32 channels of this lane's row to results in memory: alpha, bias, activation, residual, fp16 or 4 bits.
 // `col` is a multiple of 32 below cout rounded up to 64.
-template <bool RES>
-__device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const Patch& p) {
+template <bool RES, bool BULK>
+__device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const Patch& p, const CUtensorMap* out_map) {
   const uint64_t row = p.row0 + p.own;
   const bool live = row < p.rows;
   if (RES) cp_async_wait_all();
-  __syncwarp();  // residual and bias are there, and what was there is read
+  patch_free<BULK>(o, p);  // residual and bias are there, and what was there is read
   // step by step over all 32 channels, so that the loads of a step are in flight together
   {
     uint4 b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = ld_shared16(p.stage + 2048u + 16u * i);
+    for (int i = 0; i < 8; ++i) b[i] = ld_shared16(p.bias + 16u * i);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       fma2(v[4 * i], v[4 * i + 1], o.alpha, b[i].x, b[i].y);
@@ -155,6 +177,15 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
       }
     }
     if (o.mode == 0) {
+      if (BULK && o.bulk && p.row0 + 32u <= p.rows) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          st_shared16(p.stage + copied_at(p.own, c), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+        fence_proxy_async();
+        __syncwarp();
+        if (p.lane == 0 && p.col < o.cout) store_patch(out_map, p);
+        return;
+      }
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         st_shared16(p.stage + staged_at(p.own, c), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
@@ -258,6 +289,12 @@ inline bool make_output(const spconvb_fp4_params& p, const float* bias, void* ou
   const uint64_t bits = (uint64_t)(uintptr_t)p.res | 2ull * o.cout | (p.out_fp4 ? 0ull : (uint64_t)(uintptr_t)out);
   o.access = bits % 16u == 0u ? 16 : (bits % 4u == 0u ? 4 : 2);
   return true;
+}
+
+// Host: the map of fp16 results, where their rows can be copied so.
+inline bool encode_out(CUtensorMap& map, const Output& o, uint32_t rows) {
+  return o.mode == 0 && o.access == 16 && o.cout >= 32u &&
+         encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.out, o.cout, rows, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 }  // namespace fp4

@@ -21,13 +21,14 @@
 // the SMs.  But its accumulator is the only one (two and the scales are more than tensor memory holds), drained with no MMA beside it, and
 // its channels are twice as many to write before the next tile's: measured, a tile takes about 5 000 cycles and 580 a chunk, one of 128
 // 2 000 and 600, a launch in pairs 1 500 more, and the launch takes what costs less over its rounds of tiles (us, pairs / not: 32 400 x
-// 256 -> 512 14.9 / 12.4, x 1 024 18.3 / 19.4; 8 192 x 4 096 -> 4 096 56 / 88; 200 x 8 192 -> 8 192 18.6 / 16.5, x 16 384 -> 16 384
-// 36 / 53).  With a tile of 128 rows x 256 channels on one SM, 54 KB a chunk, 8 192 x 4 096 -> 4 096 took 65.
+// 256 -> 512 11.8 / 9.8, x 1 024 15.5 / 16.6; 8 192 x 4 096 -> 4 096 56 / 88; 200 x 8 192 -> 8 192 18.9 / 16.6, x 16 384 -> 16 384
+// 37 / 53).  With a tile of 128 rows x 256 channels on one SM, 54 KB a chunk, 8 192 x 4 096 -> 4 096 took 65.
 //
-// What bounds it: short K, the epilogue and the writing of fp16 rows (2 100 cycles for 32 KB a tile and SM).  Long K, several things at
-// once: 8 192 x 4 096 -> 4 096 takes 57 us (4.9 PFLOP/s), 51 with no code copied at all, 52 on zeros (the power limit then lowers the
-// clock less).  Of 13 100 cycles a tile the MMAs are 8 500, 1 900 the exchange of the accumulator; shared memory takes in 38 KB a chunk
-// and gives them to the tensor core at 66 + 62 of its 128 bytes a cycle when they run at their full rate.
+// What bounds it: short K, the epilogue and the writing of fp16 rows (1 900 cycles for 32 KB a tile and SM; 32 400 x 256 -> 512 takes 9.8
+// us, and 6.7 without results).  Long K, several things at once: 8 192 x 4 096 -> 4 096 takes 55 us (5.0 PFLOP/s), 5 less with no code
+// copied at all, 5 less on zeros (the power limit then lowers the clock less).  Of 13 100 cycles a tile the MMAs are 8 500, 1 900 the
+// exchange of the accumulator; shared memory takes in 38 KB a chunk and gives them to the tensor core, at 66 + 62 of its 128 bytes a
+// cycle when the MMAs run at their full rate.
 //
 // Few tiles and a long K: K is split over the CTAs of a cluster, whose sums the first one collects through distributed shared memory,
 // always in the same order.  That costs 5 us and a chunk takes 0.32, so it begins at 32 chunks (64 rows -> 64 channels, us, split / not:
@@ -79,7 +80,7 @@ struct Shape {
   static constexpr uint32_t kSfCols = kWords * 4 * (1 + kBlocks);
   static constexpr uint32_t kPatches = TN == 256 ? 2 : 1;            // of 32 channels a warp
   static constexpr uint32_t kRing = kStages * kStage;
-  static constexpr uint32_t kSmem = kRing + kEpiWarps * kStageBytes + 1024 + 512;
+  static constexpr uint32_t kSmem = kRing + kEpiWarps * (kPatchBytes + kBiasBytes) + 1024 + 512;
   static_assert(kStage % 1024 == 0, "stages start on swizzle atoms");
   static_assert(kBuffers * TN + kStages * kSfCols <= kTmemCols, "tensor memory");
   static_assert(kSmem <= 232448, "shared memory");
@@ -96,13 +97,13 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
 // SPLIT: the CTAs of a cluster share a tile's K (a kernel of its own: the sums kept for it would be spilled in the other).
 template <int FMT, int TN, bool SPLIT>
 __global__ void __launch_bounds__(kCtaThreads, 1)
-fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_map) {
+fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_map, const __grid_constant__ CUtensorMap out_map) {
   using S = Shape<FMT, TN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   const uint32_t s0 = smem_u32(smem);
-  uint64_t* bars = (uint64_t*)(smem + S::kRing + kEpiWarps * kStageBytes);
+  uint64_t* bars = (uint64_t*)(smem + S::kRing + kEpiWarps * (kPatchBytes + kBiasBytes));
   uint32_t* tmem_holder = (uint32_t*)(bars + 2 * S::kStages + 4);
   volatile uint32_t* abort_flag = tmem_holder + 1;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::kStages;
@@ -339,7 +340,8 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     const uint32_t first = set * (32u * S::kPatches);  // channel of the tile
     Patch p;
     p.own = p.lane = lane;
-    p.stage = s0 + S::kRing + (uint32_t)warp * kStageBytes;
+    p.stage = s0 + S::kRing + (uint32_t)warp * kPatchBytes;
+    p.bias = s0 + S::kRing + kEpiWarps * kPatchBytes + (uint32_t)warp * kBiasBytes;
     p.rows = n;
     uint32_t tl = 0;
     for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++tl) {
@@ -379,10 +381,11 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
           p.col = col + 32u * g;
           __syncwarp();  // the bias before is read
           stage_bias(p, bias[g]);
-          if (p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false>(a.o, v[g], p);
+          if (p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false, !SPLIT>(a.o, v[g], p, &out_map);
         }
       }
     }
+    if (!SPLIT) stores_done(a.o, p);
   }
 
   // A split's sums: every CTA but the first leaves its part in its own shared memory (no copy into it is in flight:
@@ -395,7 +398,8 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
     p.rows = n;
     p.col = (tile0 % tiles_n) * TN + set * 32u;
     p.own = p.lane = lane;
-    p.stage = s0 + S::kRing + (uint32_t)warp * kStageBytes;
+    p.stage = s0 + S::kRing + (uint32_t)warp * kPatchBytes;
+    p.bias = s0 + S::kRing + kEpiWarps * kPatchBytes + (uint32_t)warp * kBiasBytes;
     const bool live = epi && p.row0 + lane < n;
     if (epi && rank == 0u) stage_bias(p, load_bias(a.o, p));
     if (live && rank != 0u) {
@@ -414,7 +418,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
         }
       }
       __syncwarp();
-      if (epi && p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false>(a.o, part, p);
+      if (epi && p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false, !SPLIT>(a.o, part, p, &out_map);
     }
     __syncwarp();
     cluster_sync();  // nobody leaves while its part is read
@@ -438,24 +442,8 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
   }
 }
 
-typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled() {
-  static EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return (EncodeTiled)p;
-  }();
-  return fn;
-}
-
 template <int FMT, int TN, bool SPLIT>
-int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, cudaStream_t st) {
+int launch_linear(const LinearArgs& a, const CUtensorMap& map, const CUtensorMap& out_map, uint32_t tiles, cudaStream_t st) {
   using S = Shape<FMT, TN>;
   static bool attr_done[64] = {};
   int dev = 0;
@@ -467,12 +455,13 @@ int launch_linear(const LinearArgs& a, const CUtensorMap& map, uint32_t tiles, c
   }
   const uint32_t ctas = SPLIT ? a.split : S::kCtas;  // of a cluster
   const uint32_t grid = SPLIT ? tiles * ctas : tiles < kSmCount / ctas ? tiles * ctas : (uint32_t)kSmCount;
-  SPCONVB_CUDA_TRY(launch_clusters(fp4_linear_kernel<FMT, TN, SPLIT>, grid, ctas, kCtaThreads, S::kSmem, st, a, map));
+  SPCONVB_CUDA_TRY(launch_clusters(fp4_linear_kernel<FMT, TN, SPLIT>, grid, ctas, kCtaThreads, S::kSmem, st, a, map,
+                                   out_map));
   return SPCONVB_OK;
 }
 
 template <int FMT>
-int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream_t st) {
+int launch_shape(LinearArgs a, const CUtensorMap& map, const CUtensorMap& out_map, uint32_t rows, cudaStream_t st) {
   auto tiles = [&](uint64_t tm, uint64_t tn) { return (rows + tm - 1) / tm * ((a.o.cout + tn - 1) / tn); };
   a.split = 1;
   auto cost = [&](uint64_t t, uint64_t places, uint64_t tile, uint64_t chunk) {
@@ -480,12 +469,12 @@ int launch_shape(LinearArgs a, const CUtensorMap& map, uint32_t rows, cudaStream
   };
   if (a.o.cout > 128u &&
       cost(tiles(256, 256), kSmCount / 2, 5000, 580) + 1500u < cost(tiles(128, 128), kSmCount, 2000, 600))
-    return launch_linear<FMT, 256, false>(a, map, (uint32_t)tiles(256, 256), st);
+    return launch_linear<FMT, 256, false>(a, map, out_map, (uint32_t)tiles(256, 256), st);
   const uint64_t t = tiles(128, 128);
   if (a.nchunk >= 32u)
     while (a.split < 8u && 2u * a.split * t <= (uint64_t)kSmCount && a.nchunk >= 8u * a.split) a.split *= 2u;
-  return a.split > 1u ? launch_linear<FMT, 128, true>(a, map, (uint32_t)t, st)
-                      : launch_linear<FMT, 128, false>(a, map, (uint32_t)t, st);
+  return a.split > 1u ? launch_linear<FMT, 128, true>(a, map, out_map, (uint32_t)t, st)
+                      : launch_linear<FMT, 128, false>(a, map, out_map, (uint32_t)t, st);
 }
 
 }  // namespace
@@ -520,15 +509,11 @@ extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes
   a.status = status;
   a.wait_test = p->wait_test;
 
-  EncodeTiled encode = encode_tiled();
-  if (!encode) return SPCONVB_E_UNSUPPORTED;
   CUtensorMap map;
-  const cuuint64_t dims[2] = {cp / 2u, launch_rows}, strides[1] = {cp / 2u};
-  const cuuint32_t box[2] = {128, kTileM}, ones[2] = {1, 1};
-  if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, ones,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return SPCONVB_E_ARG;
-  return p->format == SPCONVB_MXFP4 ? launch_shape<SPCONVB_MXFP4>(a, map, launch_rows, (cudaStream_t)stream)
-                                    : launch_shape<SPCONVB_NVFP4>(a, map, launch_rows, (cudaStream_t)stream);
+  if (!encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, cp / 2u, launch_rows, 128, kTileM, CU_TENSOR_MAP_SWIZZLE_128B))
+    return encode_tiled() ? SPCONVB_E_ARG : SPCONVB_E_UNSUPPORTED;
+  CUtensorMap out_map{};
+  a.o.bulk = encode_out(out_map, a.o, launch_rows);
+  return p->format == SPCONVB_MXFP4 ? launch_shape<SPCONVB_MXFP4>(a, map, out_map, launch_rows, (cudaStream_t)stream)
+                                    : launch_shape<SPCONVB_NVFP4>(a, map, out_map, launch_rows, (cudaStream_t)stream);
 }

@@ -140,6 +140,32 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeTiled)p;
+  }();
+  return fn;
+}
+
+// A map of a matrix that is copied in boxes; false where there is none to be had.
+inline bool encode_map(CUtensorMap& map, CUtensorMapDataType type, uint32_t size, const void* at, uint64_t columns, uint64_t rows,
+                       uint32_t box_columns, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  const EncodeTiled encode = encode_tiled();
+  const cuuint64_t dims[2] = {columns, rows}, strides[1] = {columns * size};
+  const cuuint32_t box[2] = {box_columns, box_rows}, ones[2] = {1, 1};
+  return encode && encode(&map, type, 2, const_cast<void*>(at), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // A launch in clusters of `ctas` (1: none) that may begin while the kernel before it ends.
 template <typename... P, typename... A>
 cudaError_t launch_clusters(void (*kernel)(P...), uint32_t grid, uint32_t ctas, uint32_t threads, size_t smem, cudaStream_t st,
