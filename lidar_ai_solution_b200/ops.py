@@ -290,13 +290,12 @@ def _fp4_pitches(fmt, channels):
     return 32 * k, 4 * ((k + 1) // 2 if fmt == MXFP4 else k)
 
 
-def _fp4_device(t, count, *others):
+def _fp4_device(dev, count, *others):
     """The index of a tensor's device, which has to be the current one (the library enqueues there) and that of the row
     count (int32) and of the others."""
-    dev = t.get_device()
     if dev < 0 or dev != _current_device():
-        raise ValueError("a tensor on %s where the current CUDA device's is wanted" % t.device)
-    if count.dtype != torch.int32 or count.get_device() != dev or not count.numel():
+        raise ValueError("a tensor on device %d where the current CUDA device's is wanted" % dev)
+    if count.dtype is not torch.int32 or count.get_device() != dev or not count.numel():
         raise ValueError("a row count is an int32 on the rows' device (device_count)")
     for o in others:
         if o is not None and o.get_device() != dev:
@@ -379,7 +378,7 @@ def fp4_quantize(x, n_ptr, fmt, tensor_scale=1.0, in_scale=1.0, out=None):
     kind = _FP4_KIND.get(x.dtype)
     if kind is None or x.dim() != 2 or not x.is_contiguous():
         raise ValueError("x: a contiguous [rows, channels] tensor of fp16, fp32 or int8")
-    dev = _fp4_device(x, n_ptr)
+    dev = _fp4_device(x.get_device(), n_ptr)
     rows, ch = x.shape
     if out is None:
         out = Fp4Rows._beside(x, rows, ch, fmt, tensor_scale)
@@ -400,7 +399,7 @@ def fp4_dequantize(q, n_ptr, out_kind=F16, out=None):
         out = torch.empty_strided((rows, q.channels), (q.channels, 1), dtype=dt, device=buf.device)
     else:
         _fp4_tensor(out, dt, rows, q.channels, "out")
-    dev = _fp4_device(out, n_ptr)
+    dev = _fp4_device(out.get_device(), n_ptr)
     if q.device_index != dev:
         raise ValueError("tensors of different devices")
     if rows:
@@ -482,7 +481,7 @@ def fp4_linear(q, n_ptr, wts: Fp4Weights, act=ACT_NONE, out_fmt=None, out_tensor
                status=None, wait_test=0):
     """act(x W^T + bias) of 4-bit rows: fp16 [rows, cout], or :class:`Fp4Rows` of ``out_fmt``."""
     rows = q.rows
-    dev = _fp4_device(wts.packed, n_ptr, status)
+    dev = _fp4_device(wts.device_index, n_ptr, status)
     p, out, at = _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out)
     if wait_test:
         p.wait_test = wait_test
@@ -500,7 +499,7 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     if m.dtype != torch.int32 or m.dim() != 2 or m.shape[0] != wts.kvol or not m.is_contiguous():
         raise ValueError("m is a contiguous int32 [kvol, cap]")
     cap = m.shape[1]
-    dev = _fp4_device(wts.packed, n_out_ptr, m, res, status)
+    dev = _fp4_device(wts.device_index, n_out_ptr, m, res, status)
     p, out, at = _fp4_product(q, wts, act, cap, out_fmt, out_tensor_scale, out)
     if res is not None:
         _fp4_tensor(res, torch.float16, cap, wts.cout, "res")
