@@ -253,6 +253,40 @@ def _exact_rows(rows, channels, seed):
     return v[:, :channels].astype(np.float32)
 
 
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("n,cin,cout,kvol", [
+    (60000, 64, 64, 1), (60000, 64, 40, 8),    # one stage a tile, four tiles a CTA
+    (60000, 64, 64, 9), (40000, 128, 64, 5),   # two
+    (40000, 64, 64, 17), (40000, 256, 24, 5),  # three
+    (20001, 128, 64, 27), (20001, 256, 64, 11),  # seven and six, weights that do not stay
+    (40000, 128, 128, 1), (20001, 128, 104, 5),
+])
+def test_conv_of_few_and_many_stages(fmt, n, cin, cout, kvol):
+    """Tiles of one stage, of even and of odd numbers of them, several to a CTA: sums that are exact, so every bit counts.  A launch's
+    stages may be ready in any order; ten launches have to agree."""
+    ops = _ops()
+    x, w = _exact_rows(n, cin, 1), _exact_rows(cout * kvol, cin, 2).reshape(cout, kvol, cin)
+    q, xv = _quantized(x, fmt, 1.0)
+    m = _map(n, kvol, 4, 0.3)
+    rng = np.random.default_rng(5)
+    bias = rng.integers(-64, 64, cout).astype(np.float32) / 4
+    wq, n_ptr, dm = ops.Fp4Weights(w, fmt, 1.0, bias), ops.device_count(n), _dev(m)
+    # on the device, in 64 bits, tap by tap
+    xd, wd = _dev(xv), _dev(w.astype(np.float64))
+    y = _dev(bias.astype(np.float64)).expand(n, cout).clone()
+    for k in range(kvol):
+        there = torch.nonzero(dm[k] >= 0).flatten()
+        y[there] += xd[dm[k][there].long()] @ wd[:, k].T
+    want = y.to(torch.float16)
+    res = _dev((rng.integers(-512, 512, (n, cout)) / 4).astype(np.float16))
+    want_res = (want.float() + res.float()).to(torch.float16)
+    st = ops.new_status()
+    for _ in range(10):
+        assert torch.equal(ops.fp4_conv(q, dm, n_ptr, wq, status=st), want)
+        assert torch.equal(ops.fp4_conv(q, dm, n_ptr, wq, res=res, status=st), want_res)
+    assert int(st[0]) == 0
+
+
 @pytest.mark.parametrize("out_fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("rows,cin,cout", [(1, 64, 64), (130, 128, 72), (37, 320, 256), (257, 64, 24), (5, 2048, 130),
@@ -479,6 +513,24 @@ def test_residual_may_be_the_output(fmt):
     want = ops.fp4_conv(q, m, n_ptr, wq, res=res, res_relu=True)
     ops.fp4_conv(q, m, n_ptr, wq, res=res, res_relu=True, out=res)
     assert torch.equal(res, want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("n", [40000, 39990, 31])
+def test_wide_conv_over_its_own_residual(fmt, n):
+    """The residual is the output, rows behind the count stay, a slice of a larger buffer around them does too."""
+    ops = _ops()
+    cap, c = 40000, 128
+    q, xv, wq, wv, alpha, bias = _conv_problem(fmt, cap, c, c, 3)
+    m, n_ptr = _dev(_map(cap, 3, 5)), ops.device_count(n)
+    buf = torch.randn((cap + 2, c), dtype=torch.float32, device="cuda").to(torch.float16)
+    buf[:1], buf[-1:] = 7.0, 9.0
+    before = buf.clone()
+    apart = ops.fp4_conv(q, m, n_ptr, wq, res=before[1:-1].contiguous(), res_relu=True)
+    mine = buf[1:-1]
+    assert ops.fp4_conv(q, m, n_ptr, wq, res=mine, res_relu=True, out=mine) is mine
+    assert torch.equal(buf[1:n + 1], apart[:n])
+    assert torch.equal(buf[n + 1:], before[n + 1:]) and torch.equal(buf[:1], before[:1])
 
 
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
