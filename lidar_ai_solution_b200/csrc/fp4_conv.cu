@@ -11,7 +11,7 @@
 //   16     allocates tensor memory, copies a chunk's scales there, issues its MMAs
 //   17     one lane: the weights, a bulk copy of codes and scales a chunk, or once where all chunks fit
 //   18-25  producers, two groups of four that take the chunks in turn; a warp owns 32 rows, a thread one 16-byte segment of 8
-//          of them, and the words of scales that go with it: cp.async of 16 and of 4 bytes, which arrive on the stage's barrier by
+//          of them, and words of scales: cp.async of 16 and of 4 bytes, which arrive on the stage's barrier by
 //          themselves.  A missing neighbour has zeros for scales; its codes stay what they were (any sixteen values are numbers, and times
 //          an e4m3 scale of 0 they are 0), except in MXFP4, whose smallest scale is not 0
 //   26     64 channels: every second stage's copies and MMAs, into accumulators of its own, which the epilogue adds to the others (a sum of
@@ -20,15 +20,15 @@
 // What bounds it.  A chunk of 128 rows costs the tensor pipe 331 cycles (128 channels) or 267 (64), its 48 copies about 400 in the
 // load-store pipe, and shared memory about 600 in the wide layer (18 KB of rows and 18 of weights written, 32 read by the MMAs); in the kernel
 // it takes 690.  120 000 rows, us, MXFP4 / NVFP4: 64 -> 64 24.3 / 23.1 (with one warp for the MMAs 25.2 / 24.3, 4-bit rows out 24.0 / 23.7 and
-// 26.1 / 26.4), 128 -> 128 42.5 / 44.0 (twice the scale words), with a residual 25.7 / 24.1 and 46.0 / 47.8; 14 000 rows 64 -> 64 6.6.
+// 26.1 / 26.4), 128 -> 128 41.1 / 42.0 (twice the scale words), with a residual 25.7 / 24.1 and 44.6 / 45.7; 14 000 rows 64 -> 64 6.6.
 // Without the gather of the codes 64 -> 64 takes 19.9, without the scales' 21.0, without the output 20.7: they share the SM's issue slots and
 // its load-store pipe.  Zeros for the codes of missing neighbours, too, cost NVFP4 4 %.  Stages of two chunks because every wait,
 // fence and commit is paid once a stage (one chunk a stage: 28.7, 55.9).  128 channels with two warps for the MMAs take 45.7 / 46.5: their four
 // accumulators leave no room for scales, and a single pair is drained with no MMA beside it.  With a tile on two SMs that share the weights
 // they take 41.4 / 43.8, and 14 000 rows 10.4 / 10.9 in place of 9.4 / 10.0.
 //
-// Within the 32 rows of a warp, row 8 slot + i of the tile lies at 4 i + slot of the operand: the words of scales that
-// the 32 lanes write at the same time then lie in eight groups of four banks and not in two.
+// Rows lie in another order in the operand than in the tile, chosen so that words of scales that the 32 lanes write at the same time lie
+// in many banks (kSpread says how); the epilogue puts them back.
 #include "fp4_epilogue.cuh"
 
 namespace spconvb {
@@ -79,6 +79,10 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
   constexpr uint32_t W = FMT == SPCONVB_MXFP4 && CP != 64 ? 2 : 4;  // scale words a row and chunk
   constexpr uint32_t WPT = W / OPC;                // and tap
   constexpr uint32_t kPitch = 4 * WPT;             // bytes of a row's scales
+  // Where row 8 slot + i of a producer warp's 32 lies in the operand: with kSpread at 32 slot + 8 warp + i, so that a warp's copies of the
+  // same scale word of its rows are 128 bytes in a row; else at 32 warp + 4 i + slot, eight groups of four banks.  (120 000 rows 128 -> 128
+  // with a residual 47.4 us, so 45.8; 64 -> 64 to 4 bits 22.4 and 23.2: a row's indices are read once more for it.)
+  constexpr bool kSpread = CP != 64;
   constexpr uint32_t kSteps = 4 / W;               // MMAs a word
   constexpr uint32_t kRecord = 128 * 128 + W * kAtomBytes;          // a chunk in the weights' image
   constexpr uint32_t kWeightBytes = COUT * 128 + W * kAtomBytes;     // and in shared memory
@@ -88,9 +92,6 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
   constexpr uint32_t kSfCols = kPair * 8 * W;  // of a stage in tensor memory: rows, weights, chunk by chunk
   constexpr uint32_t kDrain = COUT / 32 * 4;   // warps that drain a tile
   constexpr uint32_t kMmas = COUT == 64 ? 2 : 1;   // warps that issue MMAs, each into an accumulator of its own
-  // Rows that lie eight apart in neighbouring lanes meet in a bank on the way to a tensor copy: 64 channels do without it (24.4 us, with
-  // it 24.7), 128 gain (44.0, with it 43.2).
-  constexpr bool kBulk = COUT == 128;
   constexpr uint32_t kAccCols = 2 * kMmas * COUT;  // accumulators of two tiles
   constexpr uint32_t kDeepest = (kTmemCols - kAccCols) / kSfCols < kMaxStages / kMmas ? (kTmemCols - kAccCols) / kSfCols : kMaxStages / kMmas;
 
@@ -263,10 +264,11 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
     const uint32_t seg_tap = seg / SPO, seg_in = seg % SPO;
     const uint32_t row_in_tile = pw * 32u + slot * 8u;
     const bool vec_ok = (a.cap & 7u) == 0u && ((uintptr_t)a.map & 15u) == 0u;
-    // Scales: of the tap's SPO segments x 8 rows, this thread copies word `word` of rows part, part + kParts, ...
-    constexpr uint32_t kParts = SPO / WPT;  // threads that share a word
-    const uint32_t word = seg_in % WPT, part = seg_in / WPT;
-    const uint32_t sf_dst = kSfOff + (seg_tap * WPT + word) * kAtomBytes + pw * 4u + slot * 16u;
+    // Scales: with kSpread this thread copies the words of one row, for all taps of a chunk; else its tap's word of every second row.
+    static_assert(kSpread || (SPO == 2 && WPT == 1), "two threads share a row's word");
+    const uint32_t own_row = row_in_tile + seg;
+    const uint32_t sf_dst = kSfOff + (kSpread ? (pw * 8u + seg) * 16u + slot * 4u
+                                              : seg_tap * kAtomBytes + pw * 4u + slot * 16u + seg_in * 64u);
 
     auto load_idx = [&](uint32_t tile, int j, int32_t (&v)[8]) {
       const int k = j * OPC + (int)seg_tap;
@@ -296,10 +298,22 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
     uint32_t ntile = tile;
     int nj = j;
     uint32_t it = grp, b = grp, ph = 0u;
-    int32_t idx[kPair][8];
+    int32_t idx[kPair][8], own[kPair][OPC];
     auto load_pair = [&]() {
 #pragma unroll
       for (uint32_t c = 0; c < kPair; ++c) load_idx(ntile, nj * (int)kPair + (int)c, idx[c]);
+      if (kSpread) {
+        const uint32_t row = ntile * tile_rows + own_row;
+        const bool live = ntile < ntiles && row < n_out;
+#pragma unroll
+        for (uint32_t c = 0; c < kPair; ++c) {
+#pragma unroll
+          for (int t = 0; t < OPC; ++t) {
+            const int k = (nj * (int)kPair + (int)c) * OPC + t;
+            own[c][t] = live && k < a.kvol ? __ldg(a.map + (size_t)k * a.cap + row) : -1;
+          }
+        }
+      }
       advance(ntile, nj, kGroups);
     };
     auto step = [&]() -> bool {
@@ -320,22 +334,29 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
 #pragma unroll
           for (uint32_t i = 0; i < 8; ++i) {
             const int32_t sr = idx[c][i];
-            const uint32_t r = 4u * (i & 1u) + slot;  // row of its group of 8
-            const uint32_t to = stage + (pw * 4u + (i >> 1)) * 1024u + r * 128u + ((seg ^ r) << 4);
+            const uint32_t r = kSpread ? i : 4u * (i & 1u) + slot;  // row of its group of 8
+            const uint32_t to = stage + (kSpread ? slot * 4u + pw : pw * 4u + (i >> 1)) * 1024u + r * 128u + ((seg ^ r) << 4);
             const bool there = (uint32_t)sr < a.in_rows;
             if (FMT == SPCONVB_NVFP4) cp_async16_if(there, to, src + (int64_t)sr * RB);
             else cp_async16(to, src + (int64_t)sr * RB, there ? 16u : 0u);
           }
         }
         // (taps past the last one have indices -1, and zeros for scales)
-        const uint8_t* src = a.scales + word * 4u;
         const uint32_t to = sR + s * kRowStage + sf_dst + c * W * kAtomBytes;
+        if (kSpread) {
 #pragma unroll
-        for (uint32_t i = 0; i < 8 / kParts; ++i) {
-          int32_t sr = idx[c][kParts * i];
+          for (int t = 0; t < OPC; ++t) {
+            const uint8_t* src = a.scales + (int64_t)own[c][t] * kPitch;
+            const uint32_t bytes = (uint32_t)own[c][t] < a.in_rows ? 4u : 0u;
 #pragma unroll
-          for (uint32_t p = 1; p < kParts; ++p) sr = part == p ? idx[c][kParts * i + p] : sr;
-          cp_async4(to + (kParts * i + part) * 64u, src + (int64_t)sr * kPitch, (uint32_t)sr < a.in_rows ? 4u : 0u);
+            for (uint32_t w = 0; w < WPT; ++w) cp_async4(to + (t * WPT + w) * kAtomBytes, src + 4u * w, bytes);
+          }
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < 8; i += 2) {
+            const int32_t sr = seg_in ? idx[c][i + 1] : idx[c][i];
+            cp_async4(to + i * 64u, a.scales + (int64_t)sr * kPitch, (uint32_t)sr < a.in_rows ? 4u : 0u);
+          }
         }
       }
       if (!(a.wait_test > 0 && it + 1u >= (uint32_t)a.wait_test)) cp_async_arrive_noinc(bar_full + 8 * b);
@@ -361,9 +382,9 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
     constexpr uint32_t kTurns = kEpiWarps / kDrain;  // sets of warps that take the tiles in turn
     const uint32_t turn = set / (COUT / 32u);
     Patch p;
-    // lane 4 i + slot of a quadrant is row 8 slot + i of its 32
-    p.own = (lane & 3u) * 8u + (lane >> 2);
     p.col = set % (COUT / 32u) * 32u;
+    // (without kSpread lane 4 i + slot of a quadrant is row 8 slot + i of its 32)
+    p.own = kSpread ? lane : (lane & 3u) * 8u + (lane >> 2);
     p.lane = lane;
     p.stage = sW + kRingBytes + (uint32_t)warp * kPatchBytes;
     p.bias = sW + kRingBytes + kEpiWarps * kPatchBytes + (uint32_t)warp * kBiasBytes;
@@ -372,10 +393,10 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
     uint32_t tl = turn;
     for (uint32_t tile = blockIdx.x + turn * gridDim.x; tile < ntiles; tile += kTurns * gridDim.x, tl += kTurns) {
       const uint32_t buf = tl & 1u;
-      p.row0 = (uint64_t)tile * tile_rows + 32u * q;
+      p.row0 = (uint64_t)tile * tile_rows + (kSpread ? 8u : 32u) * q;
       p.rows = min((uint64_t)n_out, (uint64_t)tile * tile_rows + tile_rows);  // rows of the tile end here
       const bool any = p.row0 < p.rows && cols;
-      if (RES && any) prefetch_residual<kBulk>(a.o, p);
+      if (RES && any) prefetch_residual<kSpread, kSpread ? 32 : 8>(a.o, p);
       uint32_t ok = 1u;
       if (lane == 0) ok = mbar_wait(bar_tfull + 8 * buf, (tl >> 1) & 1u, abort_flag, a.status, 34u) ? 1u : 0u;
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -400,9 +421,9 @@ __global__ void __launch_bounds__(cta_threads(COUT), 1) fp4_conv_kernel(const Co
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
-      if (any) emit32<RES, kBulk>(a.o, v, p, &out_map);
+      if (any) emit32<RES, kSpread, kSpread ? 32 : 8>(a.o, v, p, &out_map);
     }
-    if (kBulk) stores_done(a.o, p);
+    if (kSpread) stores_done(a.o, p);
     if (RES) cp_async_wait_all();  // nothing of this thread may still be writing when the CTA exits
   }
 
@@ -490,7 +511,7 @@ int spconvb_fp4_conv(const spconvb_fp4_params* p, const void* codes, const void*
   a.wait_test = p->wait_test;
   const uint32_t cp = cpad((uint32_t)p->cin);
   CUtensorMap out_map{};
-  a.o.bulk = p->cout > 64 && encode_out(out_map, a.o, cap);
+  a.o.bulk = cp != 64u && encode_out(out_map, a.o, cap, 8);
   return p->format == SPCONVB_MXFP4 ? launch_cin<SPCONVB_MXFP4>(cp, a, out_map, launch_rows, (cudaStream_t)stream)
                                     : launch_cin<SPCONVB_NVFP4>(cp, a, out_map, launch_rows, (cudaStream_t)stream);
 }

@@ -37,20 +37,43 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
   return v;
 }
 
-// Where a warp's 32 rows x 32 channels are: rows row0 .. (those below `rows` exist; this lane has row0 + own), channels col ..
+// Where a warp's 32 rows x 32 channels are: four times eight rows from row0 on, which begin APART rows from each other (those below `rows`
+// exist; row `own` of the 32 is this lane's), channels col ..
 struct Patch {
   uint64_t row0, rows;
-  uint32_t col, own, lane, stage, bias;  // (the last two: where in shared memory)
+  template <int APART>
+  __device__ __forceinline__ uint64_t row(uint32_t r) const {
+    return row0 + (APART == 8 ? r : r / 8u * APART + r % 8u);
+  }
+  uint32_t col, own, lane, stage, bias;  // (the last two: addresses in shared memory)
 };
 
 // Of fp16 results, a patch all of whose rows exist leaves as one tensor copy of 32 x 32, which the next patch waits for before it writes
 // there: the lanes' four loads and stores and the wait between them are out of the way of the next tile (32 400 x 256 -> 512 12.3 us, this way
-// 9.8; 120 000 x 256 -> 256 19.9 and 15.6; 100 x 256 -> 128 3.8 and 3.6).  Its pieces lie as that copy wants them: piece c of row r at c ^ (r / 2) % 4.
+// 9.8; 120 000 x 256 -> 256 19.9 and 15.6; 100 x 256 -> 128 3.8 and 3.6).  Its pieces lie as that copy wants them: piece c of row r
+// at c ^ (r / 2) % 4.  (Rows that begin 32 from each other leave as four copies of eight.)
 __device__ __forceinline__ uint32_t copied_at(uint32_t r, uint32_t c) { return r * 64u + ((c ^ (r >> 1 & 3u)) << 4); }
+template <int APART>
+__device__ __forceinline__ bool patch_whole(const Patch& p) {  // every box of it: there, or not there
+  if (APART == 8) return p.row0 + 32u <= p.rows;
+  bool whole = true;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    const uint64_t row = p.row<APART>(8u * k);
+    whole = whole && (row + 8u <= p.rows || row >= p.rows);
+  }
+  return whole;
+}
+template <int APART>
 __device__ __forceinline__ void store_patch(const CUtensorMap* map, const Patch& p) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"((int32_t)p.col),
-               "r"((int32_t)p.row0), "r"(p.stage)
-               : "memory");
+#pragma unroll
+  for (uint32_t k = 0; k < (APART == 8 ? 1u : 4u); ++k) {
+    const uint64_t row = p.row<APART>(8u * k);
+    if (k == 0 || row < p.rows)
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map),
+                   "r"((int32_t)p.col), "r"((int32_t)row), "r"(p.stage + k * 512u)
+                   : "memory");
+  }
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 // By all lanes: what this warp has stored has left shared memory; and, before the CTA ends, has been written.
@@ -74,7 +97,7 @@ __device__ __forceinline__ void stage_bias(const Patch& p, float b) {
 
 // The residual on its way into the patch's shared memory, in program order: it may be what the launch before wrote.  (Rows that do
 // not start on 16 bytes go by pairs of channels, two rows an instruction, or by single ones.)
-template <bool BULK>
+template <bool BULK, int APART>
 __device__ __forceinline__ void prefetch_residual(const Output& o, const Patch& p) {
   patch_free<BULK>(o, p);  // what was there is read
   if (o.access >= 16) {
@@ -82,8 +105,8 @@ __device__ __forceinline__ void prefetch_residual(const Output& o, const Patch& 
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
       const uint32_t r = 8u * k + p.lane / 4u;
-      const bool there = p.row0 + r < p.rows && c < o.cout;
-      cp_async16(p.stage + staged_at(r, p.lane % 4u), o.res + (there ? (p.row0 + r) * o.cout + c : 0u), there ? 16u : 0u);
+      const bool there = p.row<APART>(r) < p.rows && c < o.cout;
+      cp_async16(p.stage + staged_at(r, p.lane % 4u), o.res + (there ? p.row<APART>(r) * o.cout + c : 0u), there ? 16u : 0u);
     }
     return;
   }
@@ -92,8 +115,8 @@ __device__ __forceinline__ void prefetch_residual(const Output& o, const Patch& 
 #pragma unroll 8
   for (uint32_t k = 0; k < lanes; ++k) {
     const uint32_t r = k * per + p.lane / lanes;
-    const bool there = p.row0 + r < p.rows && p.col + at < o.cout;
-    const __half* from = o.res + (p.row0 + r) * o.cout + p.col + at;
+    const bool there = p.row<APART>(r) < p.rows && p.col + at < o.cout;
+    const __half* from = o.res + p.row<APART>(r) * o.cout + p.col + at;
     const uint32_t to = p.stage + staged_at(r, at / 8u) + at % 8u * 2u;
     if (per == 2u) {
       const uint32_t v = there ? load_in_order((const uint32_t*)from) : 0u;
@@ -130,9 +153,9 @@ __device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
 
 // Sums of 32 channels of this lane's row to results in memory: alpha, bias, activation, residual, fp16 or 4 bits.
 // `col` is a multiple of 32 below cout rounded up to 64.
-template <bool RES, bool BULK>
+template <bool RES, bool BULK, int APART>
 __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const Patch& p, const CUtensorMap* out_map) {
-  const uint64_t row = p.row0 + p.own;
+  const uint64_t row = p.row<APART>(p.own);
   const bool live = row < p.rows;
   if (RES) cp_async_wait_all();
   patch_free<BULK>(o, p);  // residual and bias are there, and what was there is read
@@ -177,13 +200,13 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
       }
     }
     if (o.mode == 0) {
-      if (BULK && o.bulk && p.row0 + 32u <= p.rows) {
+      if (BULK && o.bulk && patch_whole<APART>(p)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           st_shared16(p.stage + copied_at(p.own, c), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
         fence_proxy_async();
         __syncwarp();
-        if (p.lane == 0 && p.col < o.cout) store_patch(out_map, p);
+        if (p.lane == 0 && p.col < o.cout) store_patch<APART>(out_map, p);
         return;
       }
 #pragma unroll
@@ -194,11 +217,11 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
         const uint32_t per = o.access == 4 ? 2u : 1u, lanes = 32u / per;
         const uint32_t at = p.lane % lanes * per;
         if (p.col + at >= o.cout) return;
-        __half* to = (__half*)o.out + (p.row0 + p.lane / lanes) * o.cout + p.col + at;
 #pragma unroll 8
-        for (uint32_t k = 0; k < lanes; ++k, to += per * o.cout) {
+        for (uint32_t k = 0; k < lanes; ++k) {
           const uint32_t r = k * per + p.lane / lanes;
-          if (p.row0 + r >= p.rows) break;
+          if (p.row<APART>(r) >= p.rows) break;
+          __half* to = (__half*)o.out + p.row<APART>(r) * o.cout + p.col + at;
           const uint32_t from = p.stage + staged_at(r, at / 8u) + at % 8u * 2u;
           if (per == 2u) {
             uint32_t v;
@@ -217,11 +240,11 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
       for (uint32_t k = 0; k < 4; ++k) t[k] = ld_shared16(p.stage + staged_at(8u * k + p.lane / 4u, p.lane % 4u));
       const uint32_t c = p.col + 8u * (p.lane % 4u);
       const uint64_t at = p.row0 + p.lane / 4u;
-      const uint32_t left = c < o.cout && at < p.rows ? (uint32_t)min(p.rows - at, (uint64_t)32u) : 0u;
+      const uint32_t left = c < o.cout && at < p.rows ? (uint32_t)min(p.rows - at, (uint64_t)(4 * APART)) : 0u;
       __half* to = (__half*)o.out + at * o.cout + c;
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k)
-        if (8u * k < left) *(uint4*)(to + 8u * k * o.cout) = t[k];
+        if (APART * k < left) *(uint4*)(to + APART * k * o.cout) = t[k];
       return;
     }
   }
@@ -292,9 +315,9 @@ inline bool make_output(const spconvb_fp4_params& p, const float* bias, void* ou
 }
 
 // Host: the map of fp16 results, where their rows can be copied so.
-inline bool encode_out(CUtensorMap& map, const Output& o, uint32_t rows) {
+inline bool encode_out(CUtensorMap& map, const Output& o, uint32_t rows, uint32_t box_rows) {
   return o.mode == 0 && o.access == 16 && o.cout >= 32u &&
-         encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.out, o.cout, rows, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+         encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.out, o.cout, rows, 32, box_rows, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 }  // namespace fp4

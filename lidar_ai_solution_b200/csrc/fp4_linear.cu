@@ -381,7 +381,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
           p.col = col + 32u * g;
           __syncwarp();  // the bias before is read
           stage_bias(p, bias[g]);
-          if (p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false, !SPLIT>(a.o, v[g], p, &out_map);
+          if (p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false, !SPLIT, 8>(a.o, v[g], p, &out_map);
         }
       }
     }
@@ -418,7 +418,7 @@ fp4_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap rows_m
         }
       }
       __syncwarp();
-      if (epi && p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false, !SPLIT>(a.o, part, p, &out_map);
+      if (epi && p.row0 < n && p.col < ((a.o.cout + 63u) & ~63u)) emit32<false, !SPLIT, 8>(a.o, part, p, &out_map);
     }
     __syncwarp();
     cluster_sync();  // nobody leaves while its part is read
@@ -513,7 +513,7 @@ extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes
   if (!encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, cp / 2u, launch_rows, 128, kTileM, CU_TENSOR_MAP_SWIZZLE_128B))
     return encode_tiled() ? SPCONVB_E_ARG : SPCONVB_E_UNSUPPORTED;
   CUtensorMap out_map{};
-  a.o.bulk = encode_out(out_map, a.o, launch_rows);
+  a.o.bulk = encode_out(out_map, a.o, launch_rows, 32);
   return p->format == SPCONVB_MXFP4 ? launch_shape<SPCONVB_MXFP4>(a, map, out_map, launch_rows, (cudaStream_t)stream)
                                     : launch_shape<SPCONVB_NVFP4>(a, map, out_map, launch_rows, (cudaStream_t)stream);
 }
