@@ -280,6 +280,7 @@ def voxelize(points, params, status=None):
 # ------------------------------------------------------------- 4-bit floating point
 _FP4_KIND = {torch.float16: F16, torch.float32: F32, torch.int8: I8}
 _FP4_MAX_CHANNELS = 65536
+_INT32, _FLOAT16, _empty_strided = torch.int32, torch.float16, torch.empty_strided
 
 
 def _fp4_pitches(fmt, channels):
@@ -291,16 +292,15 @@ def _fp4_pitches(fmt, channels):
 
 
 def _fp4_device(dev, count, *others):
-    """The index of a tensor's device, which has to be the current one (the library enqueues there) and that of the row
+    """Checks a tensor's device, which has to be the current one (the library enqueues there) and that of the row
     count (int32) and of the others."""
     if dev < 0 or dev != _current_device():
         raise ValueError("a tensor on device %d where the current CUDA device's is wanted" % dev)
-    if count.dtype is not torch.int32 or count.get_device() != dev or not count.numel():
+    if count.dtype is not _INT32 or count.get_device() != dev or not count.numel():
         raise ValueError("a row count is an int32 on the rows' device (device_count)")
     for o in others:
         if o is not None and o.get_device() != dev:
             raise ValueError("tensors of different devices")
-    return dev
 
 
 def _fp4_tensor_scale(fmt, g):
@@ -339,17 +339,18 @@ class Fp4Rows:
     @classmethod
     def empty(cls, rows, channels, fmt, tensor_scale=1.0, device="cuda"):
         """Rows with uninitialised contents."""
-        return cls._beside(torch.empty(0, dtype=torch.uint8, device=device), rows, channels, fmt, tensor_scale)
+        t = torch.empty(0, dtype=torch.uint8, device=device)
+        return cls._beside(t, rows, channels, fmt, tensor_scale, t.get_device())
 
     @classmethod
-    def _beside(cls, t, rows, channels, fmt, tensor_scale):
+    def _beside(cls, t, rows, channels, fmt, tensor_scale, dev):
         """Uninitialised rows on t's device: one buffer, of which ``codes`` and ``scales`` are made when asked for."""
         q = cls.__new__(cls)
         cp, sp = q._pitches = _fp4_pitches(fmt, channels)
         q._hold = buf = t.new_empty(rows * (cp + sp), dtype=torch.uint8)
         q.codes_ptr = at = buf.data_ptr()
         q.scales_ptr = at + rows * cp
-        q.rows, q.channels, q.fmt, q.tensor_scale, q.device_index = rows, channels, fmt, float(tensor_scale), buf.get_device()
+        q.rows, q.channels, q.fmt, q.tensor_scale, q.device_index = rows, channels, fmt, float(tensor_scale), dev
         return q
 
     @property
@@ -378,16 +379,19 @@ def fp4_quantize(x, n_ptr, fmt, tensor_scale=1.0, in_scale=1.0, out=None):
     kind = _FP4_KIND.get(x.dtype)
     if kind is None or x.dim() != 2 or not x.is_contiguous():
         raise ValueError("x: a contiguous [rows, channels] tensor of fp16, fp32 or int8")
-    dev = _fp4_device(x.get_device(), n_ptr)
+    dev = x.get_device()
+    _fp4_device(dev, n_ptr)
     rows, ch = x.shape
     if out is None:
-        out = Fp4Rows._beside(x, rows, ch, fmt, tensor_scale)
+        out = Fp4Rows._beside(x, rows, ch, fmt, tensor_scale, dev)
     else:
         out._check(rows, ch, fmt, tensor_scale, dev)
     if rows:
-        cabi.check(cabi.lib().spconvb_fp4_quantize(
+        code = cabi.lib().spconvb_fp4_quantize(
             fmt, x.data_ptr(), kind, in_scale, ch, tensor_scale, n_ptr.data_ptr(), rows,
-            out.codes_ptr, out.scales_ptr, _fp4_stream(dev)), "fp4_quantize")
+            out.codes_ptr, out.scales_ptr, _fp4_stream(dev))
+        if code:
+            cabi.check(code, "fp4_quantize")
     return out
 
 
@@ -396,16 +400,19 @@ def fp4_dequantize(q, n_ptr, out_kind=F16, out=None):
     rows, dt = q.rows, torch.float32 if out_kind == F32 else torch.float16
     if out is None:
         buf = q._buffer()
-        out = torch.empty_strided((rows, q.channels), (q.channels, 1), dtype=dt, device=buf.device)
+        out = _empty_strided((rows, q.channels), (q.channels, 1), dtype=dt, device=buf.device)
     else:
         _fp4_tensor(out, dt, rows, q.channels, "out")
-    dev = _fp4_device(out.get_device(), n_ptr)
+    dev = out.get_device()
+    _fp4_device(dev, n_ptr)
     if q.device_index != dev:
         raise ValueError("tensors of different devices")
     if rows:
-        cabi.check(cabi.lib().spconvb_fp4_dequantize(
+        code = cabi.lib().spconvb_fp4_dequantize(
             q.fmt, q.codes_ptr, q.scales_ptr, q.channels, q.tensor_scale, out_kind,
-            n_ptr.data_ptr(), rows, out.data_ptr(), _fp4_stream(dev)), "fp4_dequantize")
+            n_ptr.data_ptr(), rows, out.data_ptr(), _fp4_stream(dev))
+        if code:
+            cabi.check(code, "fp4_dequantize")
     return out
 
 
@@ -441,7 +448,7 @@ class Fp4Weights:
         else:
             rows._check(flat, self.cin, fmt, tensor_scale, torch.cuda.current_device())
         self.packed = rows._buffer().new_empty(nbytes, dtype=torch.uint8)
-        self.device_index = rows.device_index
+        self.device_index, self._device = rows.device_index, self.packed.device
         cabi.check(lib.spconvb_fp4_pack_weights(fmt, self.cin, self.cout, self.kvol, rows.codes_ptr, rows.scales_ptr,
                                                 _ptr(self.packed), _stream()), "fp4_pack")
         self.bias = None
@@ -463,14 +470,14 @@ def _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out):
         p.act = act
     if out_fmt is None:
         if out is None:
-            out = torch.empty_strided((rows, wts.cout), (wts.cout, 1), dtype=torch.float16, device=wts.packed.device)
+            out = _empty_strided((rows, wts.cout), (wts.cout, 1), dtype=_FLOAT16, device=wts._device)
         else:
             _fp4_tensor(out, torch.float16, rows, wts.cout, "out")
             if out.get_device() != wts.device_index:
                 raise ValueError("tensors of different devices")
         return p, out, out.data_ptr()
     if out is None:
-        out = Fp4Rows._beside(wts.packed, rows, wts.cout, out_fmt, out_tensor_scale)
+        out = Fp4Rows._beside(wts.packed, rows, wts.cout, out_fmt, out_tensor_scale, wts.device_index)
     else:
         out._check(rows, wts.cout, out_fmt, out_tensor_scale, wts.device_index)
     p.out_fp4, p.out_format, p.out_tensor_scale, p.out_scales = 1, out_fmt, out_tensor_scale, out.scales_ptr
@@ -481,14 +488,17 @@ def fp4_linear(q, n_ptr, wts: Fp4Weights, act=ACT_NONE, out_fmt=None, out_tensor
                status=None, wait_test=0):
     """act(x W^T + bias) of 4-bit rows: fp16 [rows, cout], or :class:`Fp4Rows` of ``out_fmt``."""
     rows = q.rows
-    dev = _fp4_device(wts.device_index, n_ptr, status)
+    dev = wts.device_index
+    _fp4_device(dev, n_ptr, status)
     p, out, at = _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out)
     if wait_test:
         p.wait_test = wait_test
     if rows:
-        cabi.check(cabi.lib().spconvb_fp4_linear(
+        code = cabi.lib().spconvb_fp4_linear(
             C.byref(p), q.codes_ptr, q.scales_ptr, n_ptr.data_ptr(), rows, wts.packed.data_ptr(),
-            _ptr(wts.bias), at, _ptr(status), _fp4_stream(dev)), "fp4_linear")
+            _ptr(wts.bias), at, _ptr(status), _fp4_stream(dev))
+        if code:
+            cabi.check(code, "fp4_linear")
     return out
 
 
@@ -499,7 +509,8 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     if m.dtype != torch.int32 or m.dim() != 2 or m.shape[0] != wts.kvol or not m.is_contiguous():
         raise ValueError("m is a contiguous int32 [kvol, cap]")
     cap = m.shape[1]
-    dev = _fp4_device(wts.device_index, n_out_ptr, m, res, status)
+    dev = wts.device_index
+    _fp4_device(dev, n_out_ptr, m, res, status)
     p, out, at = _fp4_product(q, wts, act, cap, out_fmt, out_tensor_scale, out)
     if res is not None:
         _fp4_tensor(res, torch.float16, cap, wts.cout, "res")
@@ -508,7 +519,9 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     if wait_test:
         p.wait_test = wait_test
     if cap:
-        cabi.check(cabi.lib().spconvb_fp4_conv(
+        code = cabi.lib().spconvb_fp4_conv(
             C.byref(p), q.codes_ptr, q.scales_ptr, m.data_ptr(), cap, n_out_ptr.data_ptr(), launch_rows,
-            wts.packed.data_ptr(), _ptr(wts.bias), at, _ptr(status), _fp4_stream(dev)), "fp4_conv")
+            wts.packed.data_ptr(), _ptr(wts.bias), at, _ptr(status), _fp4_stream(dev))
+        if code:
+            cabi.check(code, "fp4_conv")
     return out
