@@ -128,7 +128,7 @@ __device__ __forceinline__ uint32_t scale_nv(uint32_t amax_bits, const TensorSca
     s = 0.f;
     return 0x7fu;
   }
-  const bool fast = t.inv_six != 0.f && amax < 1e30f;
+  const bool fast = t.inv_six != 0.f && amax * t.inv_six < 1e30f;  // (a quotient beyond fp32 is for the division: infinity, then 448)
   const float ratio = fast ? quotient(amax, t.six, t.inv_six) : __fdiv_rn(amax, t.six);
   uint16_t two;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(ratio));

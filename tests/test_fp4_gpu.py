@@ -818,3 +818,41 @@ def test_few_rows_of_extreme_scales():
         y = ops.fp4_linear(q, ops.device_count(rows), ops.Fp4Weights(w, ref.MX)).cpu().numpy()
         assert np.array_equal(y[:2], (x.astype(np.float64) @ w.T.astype(np.float64)).astype(np.float16)), rows
         assert not y[2:].any()
+
+
+@pytest.mark.parametrize("g,top", [(1e-20, 1e20), (1e-20, 1e19), (1e-27, 1e29), (2e-28, 3.4e38), (1e-27, 2e3), (1e-20, 3e18), (1.0, 3e38)])
+def test_scales_saturate_however_far_a_block_is_from_its_tensor_scale(g, top):
+    """amax / (6 g) up to the border of fp32 and beyond it is 448, and not NaN: of rows in fp32 and scaled int8."""
+    ops = _ops()
+    x = np.zeros((5, 100), np.float32)
+    x[0], x[1, ::16] = np.linspace(-top, top, 100), top
+    x[2], x[3, 7] = 6 * 448 * np.float32(g) * np.linspace(-1, 1, 100), np.float32(top) / 2
+    codes, scales = ref.quantize(x, ref.NV, g)
+    assert (scales[:2, :7] == 0x7e).all() and not (scales == 0x7f).any()
+    n = ops.device_count(5)
+    q = ops.fp4_quantize(_dev(x), n, ref.NV, g)
+    _check_codes(q, codes, scales)
+    assert torch.isfinite(ops.fp4_dequantize(q, n, ops.F32)).all()
+    xi = np.arange(-100, 100, 1, np.int8).reshape(2, 100)
+    in_scale = float(np.float32(top / 128))
+    codes, scales = ref.quantize(xi.astype(np.float32) * np.float32(in_scale), ref.NV, g)
+    _check_codes(ops.fp4_quantize(_dev(xi), ops.device_count(2), ref.NV, g, in_scale=in_scale), codes, scales)
+
+
+@pytest.mark.parametrize("rows", [37, 20000])
+def test_outputs_saturate_however_far_they_are_from_their_tensor_scale(rows):
+    """The same of a product's 4-bit rows: sums that are exact, times 2^80."""
+    ops = _ops()
+    x, w = _exact_rows(rows, 64, 1), _exact_rows(72, 64, 2)
+    codes, scales = ref.quantize(x, ref.NV, 1.0)
+    big = ops.Fp4Rows(_dev(codes), _dev(scales), 64, ref.NV, 2.0 ** 40)
+    wr = ops.fp4_quantize(_dev(w), ops.device_count(72), ref.NV, 1.0)
+    wq = ops.Fp4Weights((72, 64), ref.NV, 2.0 ** 40, rows=ops.Fp4Rows(wr.codes, wr.scales, 64, ref.NV, 2.0 ** 40))
+    y = (x.astype(np.float64) @ w.T.astype(np.float64) * 2.0 ** 80).astype(np.float32)
+    for g in (2.0 ** -66, 2.0 ** -80, 2.0 ** 60, 2.0 ** 80):
+        got = ops.fp4_linear(big, ops.device_count(rows), wq, out_fmt=ref.NV, out_tensor_scale=g)
+        _check_codes(got, *ref.quantize(y, ref.NV, g))
+    cw = ops.Fp4Weights((72, 1, 64), ref.NV, 2.0 ** 40, rows=ops.Fp4Rows(wr.codes, wr.scales, 64, ref.NV, 2.0 ** 40))
+    m = torch.arange(rows, dtype=torch.int32, device="cuda")[None].contiguous()
+    got = ops.fp4_conv(big, m, ops.device_count(rows), cw, out_fmt=ref.NV, out_tensor_scale=2.0 ** -66)
+    _check_codes(got, *ref.quantize(y, ref.NV, 2.0 ** -66))
