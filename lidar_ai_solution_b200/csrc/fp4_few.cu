@@ -45,6 +45,14 @@ __device__ __forceinline__ float dot16(const uint32_t (&a)[2], const uint32_t (&
   return f.x + f.y;
 }
 
+// The scale that a sum is multiplied by first, and the one after it.  Powers of two between 2^-127 and 2^127: times the smaller one a sum (a
+// multiple of 1/4 up to 576) loses no bit, and is infinite only where the product of all three is.  (A NaN is the larger one.)  e4m3
+// numbers are far from either end, in any order.
+template <int FMT>
+__device__ __forceinline__ float first_of(float s, float x) { return FMT == SPCONVB_MXFP4 ? fminf(s, x) : s; }
+template <int FMT>
+__device__ __forceinline__ float then_of(float s, float x) { return FMT == SPCONVB_MXFP4 ? max_nan(s, x) : x; }
+
 template <int FMT, int R>
 __global__ void __launch_bounds__(512) fp4_few_kernel(const FewArgs a) {
   __shared__ float sums[16][R][8];
@@ -90,8 +98,8 @@ __global__ void __launch_bounds__(512) fp4_few_kernel(const FewArgs a) {
         const float d0 = dot16(lo, b0), d1 = dot16(hi, b1);
         const float x0 = scale_value(FMT, xb & 255u, 1.f), x1 = FMT == SPCONVB_NVFP4 ? scale_value(FMT, xb >> 8, 1.f) : x0;
         // (a sum and two scales are at most 20 bits: exact, and a sum of 0 stays one where the scales' product would overflow)
-        acc[r] = fmaf(__fmul_rn(d0, s0), x0, acc[r]);
-        acc[r] = fmaf(__fmul_rn(d1, s1), x1, acc[r]);
+        acc[r] = fmaf(__fmul_rn(d0, first_of<FMT>(s0, x0)), then_of<FMT>(s0, x0), acc[r]);
+        acc[r] = fmaf(__fmul_rn(d1, first_of<FMT>(s1, x1)), then_of<FMT>(s1, x1), acc[r]);
       }
     }
   }

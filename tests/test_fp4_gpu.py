@@ -856,3 +856,22 @@ def test_outputs_saturate_however_far_they_are_from_their_tensor_scale(rows):
     m = torch.arange(rows, dtype=torch.int32, device="cuda")[None].contiguous()
     got = ops.fp4_conv(big, m, ops.device_count(rows), cw, out_fmt=ref.NV, out_tensor_scale=2.0 ** -66)
     _check_codes(got, *ref.quantize(y, ref.NV, 2.0 ** -66))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 4, 8, 9])
+def test_scales_that_bring_each_other_back(rows):
+    """Blocks near either end of fp32 whose products lie in the middle of it (every sum is exact), on the CUDA cores and the tensor cores."""
+    ops = _ops()
+    x, w = np.zeros((rows, 96), np.float32), np.zeros((24, 96), np.float32)
+    for r in range(rows):
+        x[r, 32 * (r % 3):32 * (r % 3) + 32] = 6 * 2.0 ** ((-122, 120, -118)[r % 3])
+    w[0, :32], w[1, :32], w[2, :32] = 6 * 2.0 ** 122, 2.0 ** 110, -6 * 2.0 ** 121
+    w[3, 32:64], w[4, 32:64], w[5, 32:64] = 6 * 2.0 ** -120, 2.0 ** -123, -3 * 2.0 ** -119
+    w[6, 64:], w[7, 64:], w[8, 64:], w[9, 64:] = 6 * 2.0 ** 118, 3 * 2.0 ** 119, -2.0 ** 117, np.nan
+    q, xv = _quantized(x, ref.MX, 1.0)
+    wv = ref.values(*ref.quantize(w, ref.MX), ref.MX, 96)
+    y = ops.fp4_linear(q, ops.device_count(rows), ops.Fp4Weights(w, ref.MX)).cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want = (xv @ wv.T).astype(np.float16)
+    assert np.isfinite(np.delete(want, 9, 1)).all() and np.abs(want[0, :3]).min() > 0 and np.isnan(want[:, 9]).all()
+    assert np.array_equal(y, want, equal_nan=True)
