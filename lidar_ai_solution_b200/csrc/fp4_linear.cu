@@ -463,16 +463,17 @@ int launch_linear(const LinearArgs& a, const CUtensorMap& map, const CUtensorMap
 template <int FMT>
 int launch_shape(LinearArgs a, const CUtensorMap& map, const CUtensorMap& out_map, uint32_t rows, cudaStream_t st) {
   auto tiles = [&](uint64_t tm, uint64_t tn) { return (rows + tm - 1) / tm * ((a.o.cout + tn - 1) / tn); };
-  a.split = 1;
-  auto cost = [&](uint64_t t, uint64_t places, uint64_t tile, uint64_t chunk) {
-    return (t + places - 1) / places * (tile + chunk * a.nchunk);
-  };
-  if (a.o.cout > 128u &&
-      cost(tiles(256, 256), kSmCount / 2, 5000, 580) + 1500u < cost(tiles(128, 128), kSmCount, 2000, 600))
-    return launch_linear<FMT, 256, false>(a, map, out_map, (uint32_t)tiles(256, 256), st);
   const uint64_t t = tiles(128, 128);
+  a.split = 1;
   if (a.nchunk >= 32u)
     while (a.split < 8u && 2u * a.split * t <= (uint64_t)kSmCount && a.nchunk >= 8u * a.split) a.split *= 2u;
+  auto cost = [&](uint64_t n, uint64_t places, uint64_t tile, uint64_t chunk) {
+    return (n + places - 1) / places * (tile + chunk * a.nchunk);
+  };
+  // (Where K is split, even in two, that is ahead of pairs: us, split / pairs, 64 x 57 664 -> 256 20 / 80, 1 000 x 57 664 -> 1 024 43 / 83.)
+  if (a.split == 1u && a.o.cout > 128u &&
+      cost(tiles(256, 256), kSmCount / 2, 5000, 580) + 1500u < cost(t, kSmCount, 2000, 600))
+    return launch_linear<FMT, 256, false>(a, map, out_map, (uint32_t)tiles(256, 256), st);
   return a.split > 1u ? launch_linear<FMT, 128, true>(a, map, out_map, (uint32_t)t, st)
                       : launch_linear<FMT, 128, false>(a, map, out_map, (uint32_t)t, st);
 }

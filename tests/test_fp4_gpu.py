@@ -875,3 +875,67 @@ def test_scales_that_bring_each_other_back(rows):
         want = (xv @ wv.T).astype(np.float16)
     assert np.isfinite(np.delete(want, 9, 1)).all() and np.abs(want[0, :3]).min() > 0 and np.isnan(want[:, 9]).all()
     assert np.array_equal(y, want, equal_nan=True)
+
+
+def _random_product(fmt, rows, cin, cout):
+    """Rows, weights and their codes of a layer whose sums are exact: scales of 1, a fifth of the codes not zero."""
+    ops = _ops()
+    gen = torch.Generator(device="cuda").manual_seed(rows + cin + cout)
+
+    def some(n):
+        q = ops.Fp4Rows.empty(n, cin, fmt)
+        keep = torch.rand(q.codes.shape, generator=gen, device="cuda") < 0.2
+        q.codes.copy_(torch.randint(0, 256, q.codes.shape, generator=gen, device="cuda", dtype=torch.uint8) * keep)
+        q.codes.view(n, -1, 32)[:, cin // 64:, (cin % 64 + 1) // 2:] = 0
+        q.scales.fill_(127 if fmt == ref.MX else 56)
+        return q
+    return some(rows), some(cout)
+
+
+def _exact_values(q):
+    table = torch.tensor(ref.VALUES, device="cuda")
+    return table[torch.stack((q.codes & 15, q.codes >> 4), 2).long()].view(q.rows, -1)[:, :q.channels]
+
+
+def _time(f, launches=10):
+    """Device microseconds of a launch among others, the median of five."""
+    took = []
+    for _ in range(6):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        torch.cuda._sleep(1_000_000)
+        a.record()
+        for _ in range(launches):
+            f()
+        b.record()
+        torch.cuda.synchronize()
+        took.append(a.elapsed_time(b) / launches * 1e3)
+    return sorted(took[1:])[2]
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("rows,cin,cout", [(64, 57600, 256), (64, 57664, 256), (30, 65536, 200), (300, 65536, 512), (9, 65536, 128),
+                                           (2, 65536, 100), (8, 32768, 65), (5, 16384, 130), (40, 64, 65536)])
+def test_linear_of_the_widest_layers(fmt, rows, cin, cout):
+    """Up to the most channels there are, bit for bit: quarters whose sums stay below 2^22."""
+    ops = _ops()
+    q, w = _random_product(fmt, rows, cin, cout)
+    wq = ops.Fp4Weights((cout, cin), fmt, rows=w)
+    st = ops.new_status()
+    got = ops.fp4_linear(q, ops.device_count(rows), wq, status=st)
+    x, y = _exact_values(q), _exact_values(w)
+    assert float((x.abs() @ y.abs().T).max()) < 2 ** 22
+    assert torch.equal(got, (x @ y.T).to(torch.float16)) and int(st[0]) == 0
+
+
+@pytest.mark.parametrize("rows,cout", [(64, 256), (300, 512), (1000, 1024)])
+def test_a_split_of_k_does_not_end_where_k_gets_longer(rows, cout):
+    """57 664 channels are one chunk in 226 more than 57 600, and take as long but for that (twice is a wrong choice of tiles)."""
+    ops = _ops()
+    took = []
+    for cin in (57600, 57664):
+        q, w = _random_product(ref.NV, rows, cin, cout)
+        wq, n = ops.Fp4Weights((cout, cin), ref.NV, rows=w), ops.device_count(rows)
+        out = ops.fp4_linear(q, n, wq)
+        took.append(_time(lambda: ops.fp4_linear(q, n, wq, out=out)))
+    assert took[1] < 1.5 * took[0], took
