@@ -44,9 +44,13 @@ int linear_few(int format, const void* codes, const void* scales, uint32_t cin, 
 namespace {
 
 // What goes to the CUDA cores: up to 8 rows, as long as the products are few (us there / here: 1 x 4 096 -> 4 096 5.2 / 8.8, 4 x
-// 4 096 -> 4 096 8.9 / 8.8, 8 x 4 096 -> 512 5.8 / 8.6, 8 x 4 096 -> 4 096 13.9 / 8.8, 1 x 8 192 -> 8 192 12.2 / 15.5).
+// 4 096 -> 4 096 8.9 / 8.8, 8 x 4 096 -> 512 5.8 / 8.6, 8 x 4 096 -> 4 096 13.9 / 8.8, 1 x 8 192 -> 8 192 12.2 / 15.5), and as long as
+// a warp's share of K is short: 16 warps have 8 channels' whole K there, however few channels there are, and split it over SMs here (rows x chunks a
+// warp, us NVFP4, MXFP4: 1 x 16 12.5 / 19.0, 16.2 / 19.0; 2 x 8 10.4 / 14.7, 12.4 / 14.7; 4 x 4 9.4 / 12.6, 11.5 / 12.6; 8 x 2 9.7 / 11.5, 10.8 / 11.4;
+// and 2 x 16 18.6 / 19.0, 22.6 / 19.1; 4 x 8 16.5 / 14.8, 20.8 / 14.8; 8 x 4 17.4 / 12.6, 19.5 / 12.6).
 constexpr uint32_t kFewRows = 8;
 constexpr uint64_t kFewProducts = 1ull << 26;
+constexpr uint32_t kFewShare = 16;  // rows x chunks a warp
 constexpr int kEpiWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kScaleWarp0 = 18, kWeightWarp = 22;
 constexpr int kCtaThreads = 32 * 23;
 constexpr uint32_t kTileM = 128;
@@ -496,12 +500,13 @@ extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)packed) & 15u || !make_output(*p, bias, out, a.o)) return SPCONVB_E_ARG;
   if (((uint64_t)launch_rows + kTileM - 1) / kTileM * (((uint64_t)p->cout + 127) / 128) > 0x7fffffffu)
     return SPCONVB_E_RANGE;  // more tiles than a 32-bit number counts
-  if (launch_rows <= kFewRows && (uint64_t)launch_rows * (uint32_t)p->cin * (uint32_t)p->cout <= kFewProducts && !p->out_fp4 && p->wait_test == 0)
+  const uint32_t cp = cpad((uint32_t)p->cin), nchunk = (cp + kChunkK - 1) / kChunkK;
+  if (launch_rows <= kFewRows && (uint64_t)launch_rows * (uint32_t)p->cin * (uint32_t)p->cout <= kFewProducts &&
+      launch_rows * ((nchunk + 15u) / 16u) <= kFewShare && !p->out_fp4 && p->wait_test == 0)
     return linear_few(p->format, codes, scales, (uint32_t)p->cin, n_ptr, launch_rows, packed, a.o, (cudaStream_t)stream);
-  const uint32_t cp = cpad((uint32_t)p->cin);
   a.scales = (const uint8_t*)scales;
   a.spitch = scale_pitch(p->format, (uint32_t)p->cin);
-  a.nchunk = (cp + kChunkK - 1) / kChunkK;
+  a.nchunk = nchunk;
   a.last_steps = (cp - (a.nchunk - 1) * kChunkK) / 64u;
   a.n_ptr = n_ptr;
   a.cap = launch_rows;

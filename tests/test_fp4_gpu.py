@@ -939,3 +939,17 @@ def test_a_split_of_k_does_not_end_where_k_gets_longer(rows, cout):
         out = ops.fp4_linear(q, n, wq)
         took.append(_time(lambda: ops.fp4_linear(q, n, wq, out=out)))
     assert took[1] < 1.5 * took[0], took
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("rows,cin,cout", [(8, 65536, 128), (4, 65536, 64), (8, 32768, 8), (8, 32768, 256)])
+def test_fewer_rows_of_a_long_k_take_no_longer(fmt, rows, cin, cout):
+    """Few rows never take much longer than nine, which have all SMs split K (half as long again is a wrong choice of kernel)."""
+    ops = _ops()
+    took = []
+    for r in (rows, 9):
+        q, w = _random_product(fmt, r, cin, cout)
+        wq, n = ops.Fp4Weights((cout, cin), fmt, rows=w), ops.device_count(r)
+        out = ops.fp4_linear(q, n, wq)
+        took.append(_time(lambda: ops.fp4_linear(q, n, wq, out=out)))
+    assert took[0] < 1.5 * took[1], took
