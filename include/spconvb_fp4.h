@@ -57,7 +57,8 @@ SPCONVB_API int spconvb_fp4_dequantize(int32_t format, const void* codes, const 
                                        const uint32_t* n_ptr, uint32_t launch_rows, void* out,
                                        void* stream);
 
-/* Weights: [cout][kvol][cin] quantised as cout * kvol rows of cin channels, laid out once for the products below. */
+/* Weights: [cout][kvol][cin] quantised as cout * kvol rows of cin channels, laid out once for the products below.  kvol 1 in any
+ * sizes, for spconvb_fp4_linear; more taps where spconvb_fp4_conv_supported() says 1 (else SPCONVB_E_UNSUPPORTED). */
 SPCONVB_API size_t spconvb_fp4_packed_bytes(int32_t format, int32_t cin, int32_t cout, int32_t kvol);
 SPCONVB_API int spconvb_fp4_pack_weights(int32_t format, int32_t cin, int32_t cout, int32_t kvol,
                                          const void* codes, const void* scales, void* packed,

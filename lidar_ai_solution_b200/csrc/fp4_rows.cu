@@ -514,7 +514,7 @@ bool aligned16(const void* a, const void* b = nullptr, const void* c = nullptr) 
 
 }  // namespace
 
-// Elements of an image of packed weights and its size; 0 for shapes that no product takes.
+// Chunks of an image of packed weights, over all blocks of 128 channels; 0 for numbers that no image has.
 uint64_t packed_records(int cin, int cout, int kvol) {
   if (!channels_ok(cin) || !channels_ok(cout) || kvol < 1 || kvol > 27) return 0;
   const uint64_t nchunk = ((uint64_t)kvol * cpad(cin) + kChunkK - 1) / kChunkK;
@@ -580,6 +580,9 @@ int spconvb_fp4_pack_weights(int32_t format, int32_t cin, int32_t cout, int32_t 
   if (!codes || !scales || !packed || !format_ok(format)) return SPCONVB_E_ARG;
   const uint64_t records = packed_records(cin, cout, kvol);
   if (records == 0 || !aligned16(codes, scales, packed)) return SPCONVB_E_ARG;
+  // What no product takes is refused here and not at the first product.  (With more than one tap an image also wants a whole number of scale
+  // words a tap, which MXFP4 rows of 129 to 192 channels do not have.)
+  if (kvol > 1 && !spconvb_fp4_conv_supported(cin, cout, kvol)) return SPCONVB_E_UNSUPPORTED;
   const uint64_t total = records * (1024u + words_per_chunk(format, cpad((uint32_t)cin)) * 128u);
   const uint64_t blocks = (total + 255u) / 256u;
   fp4_pack_kernel<<<(int)(blocks < kSmCount * 32u ? blocks : kSmCount * 32u), 256, 0, (cudaStream_t)stream>>>(

@@ -441,6 +441,8 @@ class Fp4Weights:
         nbytes = lib.spconvb_fp4_packed_bytes(fmt, self.cin, self.cout, self.kvol)
         if nbytes == 0:
             raise ValueError("no 4-bit weights [%d, %d, %d] in format %s" % (self.cout, self.kvol, self.cin, fmt))
+        if self.kvol > 1 and not lib.spconvb_fp4_conv_supported(self.cin, self.cout, self.kvol):
+            raise ValueError("the convolution takes no 4-bit weights [%d, %d, %d]" % (self.cout, self.kvol, self.cin))
         flat = self.cout * self.kvol
         if rows is None:
             w = w.to(device).reshape(flat, self.cin).contiguous()

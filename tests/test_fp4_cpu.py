@@ -150,3 +150,17 @@ def test_definition_keeps_what_it_can_hold(fmt):
     grid = np.sort(np.unique(ref.VALUES))
     nearest = np.abs(x[..., None] / s[..., None] - grid).min(2)
     assert np.allclose(np.abs(x - got) / s, nearest, atol=1e-6)
+
+
+@pytest.mark.parametrize("fmt", [ref.MX, ref.NV])
+@pytest.mark.parametrize("cin,cout,kvol", [(192, 64, 27), (129, 64, 2), (320, 64, 27), (64, 129, 27), (257, 1, 3)])
+def test_weights_that_no_product_takes_are_refused_when_they_are_laid_out(fmt, cin, cout, kvol):
+    torch = pytest.importorskip("torch")
+    from lidar_ai_solution_b200 import ops
+    cabi, lib = _lib()
+    assert lib.spconvb_fp4_pack_weights(fmt, cin, cout, kvol, FAKE, FAKE, FAKE, None) == -5
+    for w in (torch.zeros(cout, kvol, cin), torch.zeros(cout, kvol, cin).numpy()):
+        with pytest.raises(ValueError, match="the convolution takes no"):
+            ops.Fp4Weights(w, fmt, device="cpu")
+    with pytest.raises(ValueError, match="the convolution takes no"):
+        ops.Fp4Weights((cout, kvol, cin), fmt, rows=ops.Fp4Rows.empty(cout * kvol, cin, fmt, device="cpu"))
