@@ -79,7 +79,8 @@ typedef struct spconvb_fp4_params {
   const void* res;
   int32_t res_relu;
   int32_t wait_test;      /* 0 in normal use; as in spconvb_conv_params */
-  uint32_t in_rows;       /* rows of `codes` and `scales` (spconvb_fp4_conv only): what the map says beyond them is missing */
+  uint32_t in_rows;       /* rows of `codes` and `scales` (spconvb_fp4_conv only), at least 1: what the map says beyond them is missing.
+                             (An input without rows is one row of zeros, which add nothing.) */
 } spconvb_fp4_params;
 
 /* out[r] = act(alpha * W . x[r] + bias), kvol = 1, any cin and cout up to SPCONVB_FP4_MAX_CHANNELS.  bias: fp32 [cout]

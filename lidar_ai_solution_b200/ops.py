@@ -517,6 +517,9 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     if res is not None:
         _fp4_tensor(res, torch.float16, cap, wts.cout, "res")
         p.res, p.res_relu = res.data_ptr(), res_relu
+    if not q.rows:  # the library wants a row: one of zeros adds nothing, whatever the map says of it
+        q = Fp4Rows._beside(wts.packed, 1, q.channels, q.fmt, q.tensor_scale, dev)
+        q._hold.zero_()
     p.in_rows = q.rows
     if wait_test:
         p.wait_test = wait_test

@@ -953,3 +953,25 @@ def test_fewer_rows_of_a_long_k_take_no_longer(fmt, rows, cin, cout):
         out = ops.fp4_linear(q, n, wq)
         took.append(_time(lambda: ops.fp4_linear(q, n, wq, out=out)))
     assert took[0] < 1.5 * took[1], took
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("cin,cout", [(64, 64), (100, 128), (256, 40)])
+def test_conv_of_no_rows_gives_the_bias(fmt, cin, cout):
+    """An input without rows, whatever the map says: act(bias) and the residual."""
+    ops = _ops()
+    cap, kvol = 300, 27
+    rng = np.random.default_rng(1)
+    bias = rng.standard_normal(cout).astype(np.float32)
+    wq = ops.Fp4Weights(_features(cout * kvol, cin, 2, 0.3).reshape(cout, kvol, cin), fmt, 1.0, bias)
+    empty, n = ops.Fp4Rows.empty(0, cin, fmt), ops.device_count(cap)
+    m = rng.integers(-3, 9, (kvol, cap)).astype(np.int32)
+    m[0, :3] = 0, 2 ** 31 - 1, -2 ** 31
+    want = torch.from_numpy(np.maximum(bias, 0)).cuda().half().expand(cap, cout)
+    got = ops.fp4_conv(empty, _dev(m), n, wq, act=ops.ACT_RELU)
+    assert torch.equal(got, want)
+    res = torch.randn(cap, cout, device="cuda").half()
+    got = ops.fp4_conv(empty, _dev(m), n, wq, act=ops.ACT_RELU, res=res, res_relu=True)
+    assert torch.equal(got, torch.relu((want.float() + res.float()).half()))
+    got = ops.fp4_conv(ops.fp4_quantize(torch.zeros(0, cin, device="cuda"), n, fmt), _dev(m), n, wq, out_fmt=fmt)
+    _check_codes(got, *ref.quantize(np.broadcast_to(bias, (cap, cout)), fmt))
