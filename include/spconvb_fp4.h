@@ -3,9 +3,10 @@
  *
  * The precision below int8: e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with a scale for every
  * 16 or 32 channels of a row, multiplied by the block-scaled tensor-core instructions of sm_100a with fp32
- * accumulators.  The conventions are those of spconvb.h: stream-ordered, row counts in device memory
- * (rows [0, min(*n_ptr, launch_rows)) are processed and rows behind them left as they were), no allocation,
- * no synchronisation, capturable.  Buffers may not overlap unless a comment says so.
+ * accumulators.  The conventions are those of spconvb.h: stream-ordered, row counts in device memory, no allocation,
+ * no synchronisation, capturable.  Rows, quantised or not, and the linear layer: rows [0, min(*n_ptr, launch_rows)) are processed, the
+ * buffers hold launch_rows rows.  The convolution: rows [0, min(*n_out_ptr, cap)), the buffers hold cap rows, launch_rows only
+ * sizes the grid.  Rows behind those are left as they were.  Buffers may not overlap unless a comment says so.
  *
  * Formats
  *   SPCONVB_MXFP4  blocks of 32 channels; scale byte e8m0 = exponent + 127 of 2^(floor(log2 amax) - 2), the
@@ -94,8 +95,9 @@ SPCONVB_API int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* code
  * codes), cout <= 128, kvol <= 27. */
 SPCONVB_API int spconvb_fp4_conv_supported(int32_t cin, int32_t cout, int32_t kvol);
 
-/* out[o] = act(alpha * sum_k W[:, k, :] . in[map[k * cap + o]] + bias), then the residual.  map, cap, n_out_ptr and
- * launch_rows as in spconvb_conv_forward; an entry of the map that is not below in_rows is a missing neighbour. */
+/* out[o] = act(alpha * sum_k W[:, k, :] . in[map[k * cap + o]] + bias), then the residual, for the min(*n_out_ptr, cap) rows that there
+ * are, whatever launch_rows says (it only sizes the grid; 0: cap), as in spconvb_conv_forward: out, out_scales and res
+ * hold cap rows.  An entry of the map that is not below in_rows is a missing neighbour. */
 SPCONVB_API int spconvb_fp4_conv(const spconvb_fp4_params* p, const void* codes, const void* scales,
                                  const int32_t* map, uint32_t cap, const uint32_t* n_out_ptr,
                                  uint32_t launch_rows, const void* packed, const float* bias,

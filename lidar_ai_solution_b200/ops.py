@@ -507,7 +507,8 @@ def fp4_linear(q, n_ptr, wts: Fp4Weights, act=ACT_NONE, out_fmt=None, out_tensor
 def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=False, out_fmt=None,
              out_tensor_scale=1.0, out=None, status=None, launch_rows=0, wait_test=0):
     """Sparse convolution of 4-bit rows over the map ``m`` [kvol, cap] (as ``conv_forward``): bias,
-    activation, fp16 residual [cap, cout]; fp16 [cap, cout] or :class:`Fp4Rows` of ``out_fmt``."""
+    activation, fp16 residual [cap, cout]; fp16 [cap, cout] or :class:`Fp4Rows` of ``out_fmt``.  ``launch_rows`` only sizes
+    the grid."""
     if m.dtype != torch.int32 or m.dim() != 2 or m.shape[0] != wts.kvol or not m.is_contiguous():
         raise ValueError("m is a contiguous int32 [kvol, cap]")
     cap = m.shape[1]

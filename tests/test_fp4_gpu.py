@@ -975,3 +975,26 @@ def test_conv_of_no_rows_gives_the_bias(fmt, cin, cout):
     assert torch.equal(got, torch.relu((want.float() + res.float()).half()))
     got = ops.fp4_conv(ops.fp4_quantize(torch.zeros(0, cin, device="cuda"), n, fmt), _dev(m), n, wq, out_fmt=fmt)
     _check_codes(got, *ref.quantize(np.broadcast_to(bias, (cap, cout)), fmt))
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("cin,cout", [(64, 64), (128, 128), (128, 98)])
+@pytest.mark.parametrize("launch_rows", [1, 31, 200])
+def test_conv_processes_the_count_whatever_rows_the_launch_is_for(fmt, cin, cout, launch_rows):
+    """A hint far below the count and the capacity: all rows of the count are written, with and without a residual and in 4 bits."""
+    ops = _ops()
+    cap, n = 3000, 2790
+    q, xv, wq, wv, alpha, bias = _conv_problem(fmt, cap, cin, cout, 9)
+    m, n_ptr = _dev(_map(cap, 9, 5)), ops.device_count(n)
+    res = torch.randn(cap, cout, device="cuda").half()
+    for kw in (dict(), dict(res=res, res_relu=True)):
+        out = torch.full((cap, cout), 7.0, dtype=torch.float16, device="cuda")
+        ops.fp4_conv(q, m, n_ptr, wq, out=out, launch_rows=launch_rows, **kw)
+        assert torch.equal(out[:n], ops.fp4_conv(q, m, n_ptr, wq, **kw)[:n]) and bool((out[n:] == 7).all())
+    h = ops.Fp4Rows.empty(cap, cout, fmt)
+    h.codes.fill_(0xa5)
+    h.scales.fill_(0x5a)
+    ops.fp4_conv(q, m, n_ptr, wq, out_fmt=fmt, out=h, launch_rows=launch_rows)
+    want = ops.fp4_conv(q, m, n_ptr, wq, out_fmt=fmt)
+    assert torch.equal(h.codes[:n], want.codes[:n]) and torch.equal(h.scales[:n], want.scales[:n])
+    assert bool((h.codes[n:] == 0xa5).all()) and bool((h.scales[n:] == 0x5a).all())
