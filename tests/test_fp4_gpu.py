@@ -998,3 +998,32 @@ def test_conv_processes_the_count_whatever_rows_the_launch_is_for(fmt, cin, cout
     want = ops.fp4_conv(q, m, n_ptr, wq, out_fmt=fmt)
     assert torch.equal(h.codes[:n], want.codes[:n]) and torch.equal(h.scales[:n], want.scales[:n])
     assert bool((h.codes[n:] == 0xa5).all()) and bool((h.scales[n:] == 0x5a).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("cin,cout", [(64, 64), (128, 128), (256, 72)])
+def test_conv_reads_no_row_behind_the_input(fmt, cin, cout):
+    """Every kind of entry that is no row of the input, one by one, beside rows of NaN right behind it: reading any of them would show."""
+    ops = _ops()
+    n_in, n, kvol = 300, 900, 27
+    q, xv, wq, wv, alpha, bias = _conv_problem(fmt, n_in, cin, cout, kvol)
+    codes = torch.full((2 * n_in, q.codes.shape[1]), 0x77, dtype=torch.uint8, device="cuda")
+    scales = torch.full((2 * n_in, q.scales.shape[1]), 0xff if fmt == ref.MX else 0x7f, dtype=torch.uint8, device="cuda")
+    codes[:n_in], scales[:n_in] = q.codes, q.scales
+    mine = ops.Fp4Rows(codes[:n_in], scales[:n_in], cin, fmt, q.tensor_scale)
+    m = _map(n, kvol, 5, n_in=n_in)
+    rng = np.random.default_rng(1)
+    at = rng.random(m.shape) < 0.2
+    m[at] = rng.choice([n_in, n_in + 1, n_in + 2, 2 * n_in - 1, 2 ** 31 - 1, -2, -2 ** 31], at.sum())
+    for v in (n_in, n_in + 1, -2):
+        assert (m == v).sum() > 100
+    m[4, :9] = n_in - 1                       # the last row is one of the input's
+    y, off = ref.product(_gather(xv, np.where((m < 0) | (m >= n_in), -1, m)), wv, alpha, bias, False)
+    got = ops.fp4_conv(mine, _dev(m), ops.device_count(n), wq).cpu().numpy().astype(np.float64)
+    assert (np.abs(got - y) <= off).all()
+    # and the guard is one: an input of one row more has it
+    m[:] = -1
+    m[0, ::2] = n_in
+    more = ops.Fp4Rows(codes[:n_in + 1], scales[:n_in + 1], cin, fmt, q.tensor_scale)
+    got = torch.isnan(ops.fp4_conv(more, _dev(m), ops.device_count(n), wq)).all(1).cpu().numpy()
+    assert got[::2].all() and not got[1::2].any()
