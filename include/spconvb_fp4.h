@@ -15,7 +15,8 @@
  *                  saturated at 448; tensor_scale is one positive fp32 number a tensor.
  *   A block's scale is S = 2^e, or e4m3 * tensor_scale rounded to fp32; its codes are x / S (in fp32, to the last bit, and
  *   exactly on the borders between codes) rounded to nearest even and saturated at 6, all 0 where S is 0 (the sign of a zero is not specified).  A block that holds an infinity or a NaN gets the NaN scale
- *   (0xff, 0x7f) and codes 0, so that it stays visible: it reads as NaN, and so does every product with it.
+ *   (0xff, 0x7f) and codes 0, so that it stays visible: it reads as NaN, and so does every product with it.  (Of
+ *   weights: its output channel, in every row, also where a convolution's row lacks that neighbour.)
  *
  * Layout of rows (all pointers 16-byte aligned)
  *   codes   uint8 [rows][cpad / 2], cpad = channels rounded up to 64; code = sign << 3 | index of the value, the even

@@ -1027,3 +1027,22 @@ def test_conv_reads_no_row_behind_the_input(fmt, cin, cout):
     more = ops.Fp4Rows(codes[:n_in + 1], scales[:n_in + 1], cin, fmt, q.tensor_scale)
     got = torch.isnan(ops.fp4_conv(more, _dev(m), ops.device_count(n), wq)).all(1).cpu().numpy()
     assert got[::2].all() and not got[1::2].any()
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("cin,cout", [(64, 64), (128, 128), (256, 72)])
+def test_a_block_of_weights_that_is_not_finite_shows_in_every_row(fmt, cin, cout):
+    """Its output channel is NaN, in rows without that neighbour too, and no other channel is."""
+    ops = _ops()
+    n, kvol = 300, 27
+    q, _ = _quantized(_features(n, cin, 1, 0.3), fmt, 1.0)
+    w = _features(cout * kvol, cin, 2, 0.3).reshape(cout, kvol, cin)
+    w[5, 3, 7], w[cout - 1, 26, cin - 1] = np.nan, np.inf
+    m = _map(n, kvol, 3, 0.05)
+    assert 0 < (m[3] >= 0).sum() < n
+    bad = torch.isnan(ops.fp4_conv(q, _dev(m), ops.device_count(n), ops.Fp4Weights(w, fmt))).cpu().numpy()
+    assert bad[:, [5, cout - 1]].all() and bad.sum() == 2 * n
+    for rows in (3, 300):                     # the linear layer: on the CUDA cores, and on the tensor cores
+        few = ops.Fp4Rows(q.codes[:rows], q.scales[:rows], cin, fmt)
+        bad = torch.isnan(ops.fp4_linear(few, ops.device_count(rows), ops.Fp4Weights(w[:, 3].copy(), fmt))).cpu().numpy()
+        assert bad[:, 5].all() and bad.sum() == rows
