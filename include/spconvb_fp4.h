@@ -12,7 +12,7 @@
  *   SPCONVB_MXFP4  blocks of 32 channels; scale byte e8m0 = exponent + 127 of 2^(floor(log2 amax) - 2), the
  *                  exponent clamped to -127 (amax = 0 gives byte 0).  No tensor scale: pass 1.
  *   SPCONVB_NVFP4  blocks of 16 channels; scale byte e4m3 = amax / (6 * tensor_scale), rounded to nearest even and
- *                  saturated at 448; tensor_scale is one positive fp32 number a tensor.
+ *                  saturated at 448; tensor_scale is one positive fp32 number a tensor, from 1.2e-38 to 7.5e35.
  *   A block's scale is S = 2^e, or e4m3 * tensor_scale rounded to fp32; its codes are x / S (in fp32, to the last bit, and
  *   exactly on the borders between codes) rounded to nearest even and saturated at 6, all 0 where S is 0 (the sign of a zero is not specified).  A block that holds an infinity or a NaN gets the NaN scale
  *   (0xff, 0x7f) and codes 0, so that it stays visible: it reads as NaN, and so does every product with it.  (Of
@@ -69,7 +69,7 @@ SPCONVB_API int spconvb_fp4_pack_weights(int32_t format, int32_t cin, int32_t co
 typedef struct spconvb_fp4_params {
   int32_t format;         /* of rows and weights */
   int32_t cin, cout, kvol;
-  float alpha;            /* tensor scale of the rows times that of the weights */
+  float alpha;            /* tensor scale of the rows times that of the weights; finite */
   int32_t act;            /* SPCONVB_ACT_* */
   /* Output: fp16 [rows][cout], or 4-bit rows of `out_format` and `out_tensor_scale` with their scales in out_scales. */
   int32_t out_fp4;        /* 0: fp16 */

@@ -289,6 +289,7 @@ __device__ __forceinline__ void emit32(const Output& o, uint32_t (&v)[32], const
 // Host: the output's part of a call's parameters; false where they are not valid.
 inline bool make_output(const spconvb_fp4_params& p, const float* bias, void* out, Output& o) {
   if (p.act != SPCONVB_ACT_NONE && p.act != SPCONVB_ACT_RELU) return false;
+  if (!(p.alpha >= -3.4028235e38f && p.alpha <= 3.4028235e38f)) return false;  // times a sum of 0 it would be a NaN
   if (p.out_fp4 && (!p.out_scales || !format_ok(p.out_format) || !tensor_scale_ok(p.out_format, p.out_tensor_scale)))
     return false;
   if ((uintptr_t)out & (p.out_fp4 ? 15u : 1u) || (p.out_fp4 && (uintptr_t)p.out_scales & 15u) || (uintptr_t)bias & 3u ||

@@ -280,6 +280,8 @@ def voxelize(points, params, status=None):
 # ------------------------------------------------------------- 4-bit floating point
 _FP4_KIND = {torch.float16: F16, torch.float32: F32, torch.int8: I8}
 _FP4_MAX_CHANNELS = 65536
+_FP4_SCALES = 2.0 ** -126, 3.4e38 / 448         # the tensor scales that the library takes
+_FP32_NORMAL, _FP32_MAX = 2.0 ** -126, (2 - 2.0 ** -23) * 2.0 ** 127
 _INT32, _FLOAT16, _empty_strided = torch.int32, torch.float16, torch.empty_strided
 
 
@@ -304,8 +306,8 @@ def _fp4_device(dev, count, *others):
 
 
 def _fp4_tensor_scale(fmt, g):
-    if not (g == 1 if fmt == MXFP4 else 0 < g < math.inf):
-        raise ValueError("a tensor scale is a positive number, and 1 for MXFP4")
+    if not (g == 1 if fmt == MXFP4 else _FP4_SCALES[0] <= g <= _FP4_SCALES[1]):
+        raise ValueError("a tensor scale is a positive number from 1.2e-38 to 7.5e35, and 1 for MXFP4")
 
 
 def _fp4_stream(dev):
@@ -467,7 +469,10 @@ def _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out):
     if q.fmt != wts.fmt or q.channels != wts.cin or q.device_index != wts.device_index:
         raise ValueError("rows and weights of different formats, channels or devices")
     p = cabi.Fp4Params.from_buffer_copy(wts._params)
-    p.alpha = q.tensor_scale * wts.tensor_scale
+    alpha = p.alpha = q.tensor_scale * wts.tensor_scale
+    # (below fp32's normal numbers every sum is 0 in fp16 all the same)
+    if alpha > _FP32_MAX or alpha < _FP32_NORMAL and out_fmt is not None:
+        raise ValueError("the product of the tensor scales is beyond fp32")
     if act:
         p.act = act
     if out_fmt is None:

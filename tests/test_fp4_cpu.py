@@ -164,3 +164,26 @@ def test_weights_that_no_product_takes_are_refused_when_they_are_laid_out(fmt, c
             ops.Fp4Weights(w, fmt, device="cpu")
     with pytest.raises(ValueError, match="the convolution takes no"):
         ops.Fp4Weights((cout, kvol, cin), fmt, rows=ops.Fp4Rows.empty(cout * kvol, cin, fmt, device="cpu"))
+
+
+def test_factors_that_are_not_finite_are_refused():
+    cabi, lib = _lib()
+    p = cabi.Fp4Params()
+    p.format, p.cin, p.cout, p.kvol, p.in_rows = 1, 64, 64, 1, 10
+    for alpha in (float("inf"), float("-inf"), float("nan")):
+        p.alpha = alpha
+        assert lib.spconvb_fp4_linear(C.byref(p), FAKE, FAKE, FAKE, 10, FAKE, None, FAKE, None, None) == -1
+        assert lib.spconvb_fp4_conv(C.byref(p), FAKE, FAKE, FAKE, 10, FAKE, 0, FAKE, None, FAKE, None, None) == -1
+
+
+def test_tensor_scales_that_the_library_does_not_take_are_refused_at_once():
+    torch = pytest.importorskip("torch")
+    from lidar_ai_solution_b200 import ops
+    codes, scales = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.uint8)
+    for g in (1e-39, 1e-45, 7.7e35, 1e37):
+        with pytest.raises(ValueError, match="tensor scale"):
+            ops.Fp4Rows(codes, scales, 64, ops.NVFP4, g)
+        with pytest.raises(ValueError, match="tensor scale"):
+            ops.Fp4Weights((8, 64), ops.NVFP4, g, rows=ops.Fp4Rows(codes, scales, 64, ops.NVFP4, 1.0))
+    for g in (1.2e-38, 7.5e35, 1):
+        assert ops.Fp4Rows(codes, scales, 64, ops.NVFP4, g).tensor_scale == g

@@ -1046,3 +1046,28 @@ def test_a_block_of_weights_that_is_not_finite_shows_in_every_row(fmt, cin, cout
         few = ops.Fp4Rows(q.codes[:rows], q.scales[:rows], cin, fmt)
         bad = torch.isnan(ops.fp4_linear(few, ops.device_count(rows), ops.Fp4Weights(w[:, 3].copy(), fmt))).cpu().numpy()
         assert bad[:, 5].all() and bad.sum() == rows
+
+
+def test_tensor_scales_whose_product_is_beyond_fp32():
+    """Refused where results would be wrong: above fp32, where a sum of 0 would be NaN, and below it for 4-bit rows."""
+    ops = _ops()
+    n, m = ops.device_count(40), torch.zeros((1, 40), dtype=torch.int32, device="cuda")
+    codes, scales = ref.quantize(_features(40, 64, 1), ref.NV, 0.01)
+    wr = ops.fp4_quantize(_dev(_features(24, 64, 2)), ops.device_count(24), ref.NV, 0.01)
+    bias = np.linspace(-1, 1, 24).astype(np.float32)
+
+    def both(gx, gw, **kw):
+        q = ops.Fp4Rows(_dev(codes), _dev(scales), 64, ref.NV, gx)
+        w = ops.Fp4Weights((24, 64), ref.NV, gw, bias, rows=ops.Fp4Rows(wr.codes, wr.scales, 64, ref.NV, gw))
+        return [lambda: ops.fp4_linear(q, n, w, **kw), lambda: ops.fp4_conv(q, m, n, w, **kw)]
+    for gx, gw in ((1e30, 1e30), (7.5e35, 1e3)):
+        for kw in ({}, dict(out_fmt=ref.MX), dict(out_fmt=ref.NV, out_tensor_scale=1e30)):
+            for call in both(gx, gw, **kw):
+                with pytest.raises(ValueError, match="beyond fp32"):
+                    call()
+    for gx, gw in ((1e-30, 1e-30), (1e-20, 1e-19)):
+        for call in both(gx, gw, out_fmt=ref.MX):
+            with pytest.raises(ValueError, match="beyond fp32"):
+                call()
+        for call in both(gx, gw):             # in fp16 the sums are 0 beside the bias
+            assert torch.equal(call(), _dev(bias).half().expand(40, 24))
