@@ -314,6 +314,12 @@ def _fp4_stream(dev):
     return _stream() if _raw_stream is None else _raw_stream(dev)
 
 
+def _fp4_rows(rows):
+    if rows > 0xffffffff:  # the library counts in 32 bits, and ctypes would cut it off
+        raise ValueError("more rows than 32 bits count")
+    return rows
+
+
 def _fp4_tensor(t, dtype, rows, width, what):
     if t.dtype != dtype or t.dim() != 2 or not t.is_contiguous() or t.shape[0] != rows or t.shape[1] != width:
         raise ValueError("%s: a contiguous %s [%d, %d] is wanted" % (what, dtype, rows, width))
@@ -328,7 +334,7 @@ class Fp4Rows:
 
     def __init__(self, codes, scales, channels, fmt, tensor_scale=1.0):
         cp, sp = self._pitches = _fp4_pitches(fmt, channels)
-        self.rows = codes.shape[0] if codes.dim() else -1
+        self.rows = _fp4_rows(codes.shape[0]) if codes.dim() else -1
         _fp4_tensor(codes, torch.uint8, self.rows, cp, "codes")
         _fp4_tensor(scales, torch.uint8, self.rows, sp, "scales")
         if codes.device != scales.device:
@@ -347,6 +353,7 @@ class Fp4Rows:
     @classmethod
     def _beside(cls, t, rows, channels, fmt, tensor_scale, dev):
         """Uninitialised rows on t's device: one buffer, of which ``codes`` and ``scales`` are made when asked for."""
+        _fp4_rows(rows)
         q = cls.__new__(cls)
         cp, sp = q._pitches = _fp4_pitches(fmt, channels)
         q._hold = buf = t.new_empty(rows * (cp + sp), dtype=torch.uint8)
@@ -516,7 +523,7 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     the grid."""
     if m.dtype != torch.int32 or m.dim() != 2 or m.shape[0] != wts.kvol or not m.is_contiguous():
         raise ValueError("m is a contiguous int32 [kvol, cap]")
-    cap = m.shape[1]
+    cap = _fp4_rows(m.shape[1])
     dev = wts.device_index
     _fp4_device(dev, n_out_ptr, m, res, status)
     p, out, at = _fp4_product(q, wts, act, cap, out_fmt, out_tensor_scale, out)

@@ -187,3 +187,18 @@ def test_tensor_scales_that_the_library_does_not_take_are_refused_at_once():
             ops.Fp4Weights((8, 64), ops.NVFP4, g, rows=ops.Fp4Rows(codes, scales, 64, ops.NVFP4, 1.0))
     for g in (1.2e-38, 7.5e35, 1):
         assert ops.Fp4Rows(codes, scales, 64, ops.NVFP4, g).tensor_scale == g
+
+
+@pytest.mark.parametrize("rows", [2 ** 32, 2 ** 32 + 5, 2 ** 40])
+def test_rows_beyond_32_bits_are_refused_and_not_cut_off(rows):
+    torch = pytest.importorskip("torch")
+    from lidar_ai_solution_b200 import ops
+    meta = dict(dtype=torch.uint8, device="meta")          # shapes without memory
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.Fp4Rows(torch.empty(rows, 32, **meta), torch.empty(rows, 4, **meta), 64, ops.NVFP4)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.Fp4Rows.empty(rows, 64, ops.NVFP4, device="meta")
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.fp4_conv(None, torch.empty(1, rows, dtype=torch.int32, device="meta"), None,
+                     type("Weights", (), dict(kvol=1, device_index=0)))
+    assert ops.Fp4Rows.empty(2 ** 32 - 1, 64, ops.NVFP4, device="meta").rows == 2 ** 32 - 1
