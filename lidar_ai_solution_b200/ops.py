@@ -305,6 +305,11 @@ def _fp4_device(dev, count, *others):
             raise ValueError("tensors of different devices")
 
 
+def _fp4_status(status):
+    if status.dtype is not _INT32 or status.numel() < 4 or not status.is_contiguous():
+        raise ValueError("a status block is four int32 in a row (new_status)")
+
+
 def _fp4_tensor_scale(fmt, g):
     if not (g == 1 if fmt == MXFP4 else _FP4_SCALES[0] <= g <= _FP4_SCALES[1]):
         raise ValueError("a tensor scale is a positive number from 1.2e-38 to 7.5e35, and 1 for MXFP4")
@@ -504,6 +509,8 @@ def fp4_linear(q, n_ptr, wts: Fp4Weights, act=ACT_NONE, out_fmt=None, out_tensor
     rows = q.rows
     dev = wts.device_index
     _fp4_device(dev, n_ptr, status)
+    if status is not None:
+        _fp4_status(status)
     p, out, at = _fp4_product(q, wts, act, rows, out_fmt, out_tensor_scale, out)
     if wait_test:
         p.wait_test = wait_test
@@ -526,6 +533,8 @@ def fp4_conv(q, m, n_out_ptr, wts: Fp4Weights, act=ACT_NONE, res=None, res_relu=
     cap = _fp4_rows(m.shape[1])
     dev = wts.device_index
     _fp4_device(dev, n_out_ptr, m, res, status)
+    if status is not None:
+        _fp4_status(status)
     p, out, at = _fp4_product(q, wts, act, cap, out_fmt, out_tensor_scale, out)
     if res is not None:
         _fp4_tensor(res, torch.float16, cap, wts.cout, "res")

@@ -1071,3 +1071,20 @@ def test_tensor_scales_whose_product_is_beyond_fp32():
                 call()
         for call in both(gx, gw):             # in fp16 the sums are 0 beside the bias
             assert torch.equal(call(), _dev(bias).half().expand(40, 24))
+
+
+def test_a_status_block_is_four_words():
+    """A smaller one, or one of another type, would be written past its end when a wait runs out."""
+    ops = _ops()
+    q, _ = _quantized(_features(8, 64, 1), ref.NV, 0.01)
+    n, m = ops.device_count(8), torch.zeros((1, 8), dtype=torch.int32, device="cuda")
+    w = ops.Fp4Weights(_features(24, 64, 2), ref.NV, 0.01)
+    for bad in (torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.uint8, device="cuda"),
+                torch.zeros(8, dtype=torch.int32, device="cuda")[::2], torch.zeros(4, device="cuda")):
+        for call in (lambda: ops.fp4_linear(q, n, w, status=bad), lambda: ops.fp4_conv(q, m, n, w, status=bad)):
+            with pytest.raises(ValueError, match="status block"):
+                call()
+    for good in (ops.new_status(), torch.zeros(9, dtype=torch.int32, device="cuda")[3:]):
+        ops.fp4_linear(q, n, w, status=good)
+        ops.fp4_conv(q, m, n, w, status=good)
+        assert not bool(good.any())
