@@ -1088,3 +1088,36 @@ def test_a_status_block_is_four_words():
         ops.fp4_linear(q, n, w, status=good)
         ops.fp4_conv(q, m, n, w, status=good)
         assert not bool(good.any())
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("kind", ["f16", "f32", "i8"])
+@pytest.mark.parametrize("channels", [65536, 65535, 65432, 65473])
+def test_rows_of_the_most_channels(fmt, kind, channels):
+    """Rows of 128 KB of fp16: flat, aligned and staged ways, there and back, and rows behind the count."""
+    ops = _ops()
+    rows, n = 7, 5
+    x = _features(rows, channels, channels)
+    in_scale = 1.0
+    if kind == "i8":
+        in_scale = float(np.float32(np.abs(x).max() / 127))
+        xi = np.clip(np.rint(x / np.float32(in_scale)), -128, 127).astype(np.int8)
+        dev, x = _dev(xi), xi.astype(np.float32) * np.float32(in_scale)
+    else:
+        dev = _dev(x.astype(np.float16 if kind == "f16" else np.float32))
+        x = dev.cpu().numpy().astype(np.float32)
+    g = _scale(x, fmt)
+    codes, scales = ref.quantize(x, fmt, g)
+    out = ops.Fp4Rows.empty(rows, channels, fmt, g)
+    out.codes.fill_(0xa5)
+    out.scales.fill_(0x5a)
+    count = ops.device_count(n)
+    ops.fp4_quantize(dev, count, fmt, g, in_scale=in_scale, out=out)
+    assert np.array_equal(out.scales[:n].cpu().numpy(), scales[:n])
+    assert np.array_equal(ref.magnitude_codes(out.codes[:n].cpu().numpy()), ref.magnitude_codes(codes[:n]))
+    assert bool((out.codes[n:] == 0xa5).all()) and bool((out.scales[n:] == 0x5a).all())
+    for out_kind, dt in ((ops.F16, np.float16), (ops.F32, np.float32)):
+        want = ref.values(codes, scales, fmt, channels, g).astype(np.float32).astype(dt)
+        y = torch.full((rows, channels), 7.0, dtype=torch.float16 if out_kind == ops.F16 else torch.float32, device="cuda")
+        ops.fp4_dequantize(out, count, out_kind, out=y)
+        assert np.array_equal(y[:n].cpu().numpy(), want[:n]) and bool((y[n:] == 7).all())
