@@ -93,7 +93,7 @@ SPCONVB_API int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* code
                                    uint32_t* status, void* stream);
 
 /* 1 where spconvb_fp4_conv covers these sizes: cin <= 64, 65..128 or 193..256 (rows of 32, 64 or 128 bytes of
- * codes), cout <= 128, kvol <= 27. */
+ * codes), cout <= 128, kvol <= 27.  Fewer than 64 channels cost what 64 do. */
 SPCONVB_API int spconvb_fp4_conv_supported(int32_t cin, int32_t cout, int32_t kvol);
 
 /* out[o] = act(alpha * sum_k W[:, k, :] . in[map[k * cap + o]] + bias), then the residual, for the min(*n_out_ptr, cap) rows that there

@@ -18,8 +18,12 @@
 //          two, whichever is which).  One warp's waits, fences and commits for a stage then pass beside the other's MMAs
 //
 // What bounds it.  A chunk of 128 rows costs the tensor pipe 331 cycles (128 channels) or 267 (64), its 48 copies about 400 in the
-// load-store pipe, and shared memory about 600 in the wide layer (18 KB of rows and 18 of weights written, 32 read by the MMAs); in the kernel
-// it takes 690.  120 000 rows, us, MXFP4 / NVFP4: 64 -> 64 24.3 / 23.1 (with one warp for the MMAs 25.2 / 24.3, 4-bit rows out 24.0 / 23.7 and
+// load-store pipe, and shared memory 544 in the wide layer (18 KB of rows and 18 of weights written, 32 read by the MMAs, at 128 bytes a cycle).  In
+// the kernel it takes 665 (64: 570-600), counted in the issuing warp from the first full stage to the last MMA.  Of 120 000 rows 128 -> 128 the
+// longest CTA walks 7 tiles of 14 chunks: 33.2 us of the 42.0 at 1 965 MHz (the clock under this load; with a residual 1 942); 5 000 cycles,
+// 2.5 us, go by from its start to the first full stage, the rest is the launch and the last tile's way out.  Every tile walks all 27 taps: of a
+// benchmark frame's (tile, tap) pairs 9 % have no neighbour at 120 000 rows, 21 % at 60 000 and 52 % at 14 000 (tiles of 96), and are walked all
+// the same.  120 000 rows, us, MXFP4 / NVFP4: 64 -> 64 24.3 / 23.1 (with one warp for the MMAs 25.2 / 24.3, 4-bit rows out 24.0 / 23.7 and
 // 26.1 / 26.4), 128 -> 128 41.1 / 42.0 (twice the scale words), with a residual 25.7 / 24.1 and 44.6 / 45.7; 14 000 rows 64 -> 64 6.6.
 // Without the gather of the codes 64 -> 64 takes 19.9, without the scales' 21.0, without the output 20.7: they share the SM's issue slots and
 // its load-store pipe.  Zeros for the codes of missing neighbours, too, cost NVFP4 4 %.  Stages of two chunks because every wait,

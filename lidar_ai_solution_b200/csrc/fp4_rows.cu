@@ -10,7 +10,8 @@
 //            shared memory in 16-byte pieces
 //
 // Measured: 480 000 x 128 fp16 -> NVFP4 25.4 us (6.2 TB/s, 96 % of a copy's rate), 120 000 x 128 -> MXFP4 5.5 us (out of L2); 960 000 x 64
-// int8 -> NVFP4 21.7 us (4.4 TB/s: two thirds of the issue slots and of the integer pipe, whatever the occupancy); back to fp16 25.8 us
+// int8 -> NVFP4 21.7 us (4.4 TB/s; two thirds of the issue slots and of the integer pipe, whatever the occupancy, so that neither is
+// the limit by itself); back to fp16 25.8 us
 // (6.1 TB/s); 200 000 rows of 100 channels, staged, 20.6 us and back 15.4.  A grid of 32 blocks an SM: with 16, a block had one turn or
 // two, and the last ones ran alone (back to fp16 27.5; with 6 33.5, with as many as there are turns 25.8).
 #include "fp4.cuh"
