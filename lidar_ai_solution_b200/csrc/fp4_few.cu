@@ -9,7 +9,7 @@
 // The lanes of a channel and then the warps are added in a fixed order.  Measured, NVFP4, us a launch in a chain: 1 row x 4 096 -> 4 096
 // 5.1 (9.5 MB; 2.4 of it are a launch that reads next to nothing), 1 x 8 192 -> 8 192 12.2 (3.1 TB/s): what bounds it there is the
 // conversion of codes, done again for every channel on the rows' side.  A long K stays with 16 warps, 0.5 to 0.6 us a chunk of each and row (1 x 65 536 -> 128
-// 12.5, 2 x 18.6): the linear layer's rule sends more than 16 rows x chunks elsewhere.
+// 12.5, 2 x 18.6): the linear layer's rule sends longer shares elsewhere.
 #include "fp4_epilogue.cuh"
 
 namespace spconvb {

@@ -45,12 +45,16 @@ namespace {
 
 // What goes to the CUDA cores: up to 8 rows, as long as the products are few (us there / here: 1 x 4 096 -> 4 096 5.2 / 8.8, 4 x
 // 4 096 -> 4 096 8.9 / 8.8, 8 x 4 096 -> 512 5.8 / 8.6, 8 x 4 096 -> 4 096 13.9 / 8.8, 1 x 8 192 -> 8 192 12.2 / 15.5), and as long as
-// a warp's share of K is short: 16 warps have 8 channels' whole K there, however few channels there are, and split it over SMs here (rows x chunks a
-// warp, us NVFP4, MXFP4: 1 x 16 12.5 / 19.0, 16.2 / 19.0; 2 x 8 10.4 / 14.7, 12.4 / 14.7; 4 x 4 9.4 / 12.6, 11.5 / 12.6; 8 x 2 9.7 / 11.5, 10.8 / 11.4;
-// and 2 x 16 18.6 / 19.0, 22.6 / 19.1; 4 x 8 16.5 / 14.8, 20.8 / 14.8; 8 x 4 17.4 / 12.6, 19.5 / 12.6).
+// a warp's share of K is short: 16 warps have 8 channels' whole K there, however few channels there are, and it is split over SMs here.  A chunk a warp
+// costs 0.2 + 0.42 a row there (NVFP4; MXFP4 0.4 + 0.48), 0.55 here, and 7.8 to 8.1 more for the split (rows x chunks a warp, us there / here, NVFP4 and MXFP4: 1 x 16
+// 12.5 / 19.0 and 16.2 / 19.0; 2 x 9 11.4 / 15.2 and 13.7 / 15.1; 2 x 12 14.4 / 16.8 and 17.5 / 16.7; 3 x 6 10.8 / 13.6 and 13.8 / 13.5; 4 x 4 9.4 / 12.6 and 11.5 / 12.6;
+// 5 x 4 12.2 / 12.5 and 14.0 / 12.4; 8 x 2 9.7 / 11.5 and 10.8 / 11.4; 8 x 3 12.9 / 11.9 and 14.6 / 11.9; 4 x 8 16.5 / 14.8 and 20.8 / 14.8).
 constexpr uint32_t kFewRows = 8;
 constexpr uint64_t kFewProducts = 1ull << 26;
-constexpr uint32_t kFewShare = 16;  // rows x chunks a warp
+inline bool short_share(int format, uint32_t rows, uint32_t nchunk) {
+  const uint32_t share = (nchunk + 15u) / 16u;
+  return share * (format == SPCONVB_NVFP4 ? 42u * rows - 35u : 48u * rows - 15u) <= 810u;  // hundredths of a us
+}
 constexpr int kEpiWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kScaleWarp0 = 18, kWeightWarp = 22;
 constexpr int kCtaThreads = 32 * 23;
 constexpr uint32_t kTileM = 128;
@@ -502,7 +506,7 @@ extern "C" int spconvb_fp4_linear(const spconvb_fp4_params* p, const void* codes
     return SPCONVB_E_RANGE;  // more tiles than a 32-bit number counts
   const uint32_t cp = cpad((uint32_t)p->cin), nchunk = (cp + kChunkK - 1) / kChunkK;
   if (launch_rows <= kFewRows && (uint64_t)launch_rows * (uint32_t)p->cin * (uint32_t)p->cout <= kFewProducts &&
-      launch_rows * ((nchunk + 15u) / 16u) <= kFewShare && !p->out_fp4 && p->wait_test == 0)
+      short_share(p->format, launch_rows, nchunk) && !p->out_fp4 && p->wait_test == 0)
     return linear_few(p->format, codes, scales, (uint32_t)p->cin, n_ptr, launch_rows, packed, a.o, (cudaStream_t)stream);
   a.scales = (const uint8_t*)scales;
   a.spitch = scale_pitch(p->format, (uint32_t)p->cin);
